@@ -24,8 +24,10 @@ LIB = LIB_DIR / "libfcai_b200.so"
 SOURCES = [
     "warp_div.cu",
     "conv_tc.cu",
+    "linear_tc.cu",
+    "rowwise.cu",
 ]
-HEADERS = ["fcai_common.h", "tc_ptx.h"]
+HEADERS = ["fcai_common.h", "tc_ptx.h", "layers_common.cuh"]
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-lineinfo", "-std=c++17", "-Xcompiler", "-fPIC,-O2", "--expt-relaxed-constexpr"]
 

@@ -1,0 +1,188 @@
+// layers_common.cuh -- element types, activations and 8-bit blocks shared by
+// the pointwise layers (linear_tc.cu, rowwise.cu).
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <float.h>
+#include <stdint.h>
+
+#include "../../include/fcai_layers.h"
+#include "fcai_common.h"
+
+namespace ly {
+
+// ---- element types ----------------------------------------------------------
+template <typename T> __device__ __forceinline__ float to_f32(T v);
+template <> __device__ __forceinline__ float to_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ float to_f32<__half>(__half v) { return __half2float(v); }
+template <> __device__ __forceinline__ float to_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v);
+template <> __device__ __forceinline__ float from_f32<float>(float v) { return v; }
+template <> __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
+template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+__device__ __forceinline__ uint32_t pack2(float a, float b, __nv_bfloat16) {
+    __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+__device__ __forceinline__ uint32_t pack2(float a, float b, __half) {
+    __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<uint32_t *>(&v);
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) {
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
+}
+__device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
+    return __half22float2(*reinterpret_cast<__half2 *>(&w));
+}
+
+// Eight consecutive elements from / to a 16-byte aligned address (f32: two
+// 16-byte accesses).
+template <typename T> struct Vec8 {
+    static __device__ __forceinline__ void load(const T *p, float (&v)[8]) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+        unpack(q, v);
+    }
+    static __device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8]) {
+        const float2 a = unpack2(q.x, T()), b = unpack2(q.y, T()), c = unpack2(q.z, T()), d = unpack2(q.w, T());
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+    }
+    static __device__ __forceinline__ void store(T *p, const float (&v)[8]) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
+                                                   pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    }
+};
+template <> struct Vec8<float> {
+    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+
+// ---- activations --------------------------------------------------------------
+__device__ __forceinline__ float ex2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The normal distribution's upper tail Q(t) = erfc(t / sqrt 2) / 2, t >= 0, as
+// e * R(u) with e = exp(-t^2 / 2), u = 1 / (1 + 0.24 t) and R a polynomial
+// without constant term, the form of Hastings' approximations (Approximations
+// for Digital Computers, 1955).  The coefficients are a fit of this project's
+// own: iteratively reweighted least squares of R against Q e^(t^2/2) on
+// t in [0, 40], largest relative error 7.6e-7 evaluated in fp32.  `e` comes
+// back for the density.  15 instructions, two of them of the special function
+// unit, which keeps the elementwise kernels bound by memory.
+__device__ __forceinline__ float normal_tail(float t, float &e) {
+    e = ex2_approx(-0.72134752f * t * t);  // log2(e) / 2
+    const float u = rcp_approx(fmaf(0.24f, t, 1.f));
+    float r = fmaf(u, -0.0529928472f, 0.152797519f);
+    r = fmaf(u, r, -0.0657069748f);
+    r = fmaf(u, r, 0.118390834f);
+    r = fmaf(u, r, 0.0633970503f);
+    r = fmaf(u, r, 0.0928386496f);
+    r = fmaf(u, r, 0.0955221622f);
+    r = fmaf(u, r, 0.0957537928f);
+    return e * (u * r);
+}
+
+template <int kAct>
+__device__ __forceinline__ float act(float x) {
+    if (kAct == FCAI_ACT_RELU) return x < 0.f ? 0.f : x;  // a NaN stays
+    if (kAct == FCAI_ACT_GELU) {
+        float e;
+        const float q = normal_tail(fabsf(x), e);
+        return x * (x < 0.f ? q : 1.f - q);
+    }
+    if (kAct == FCAI_ACT_SILU) return x * rcp_approx(1.f + ex2_approx(-1.44269504f * x));
+    return x;
+}
+template <int kAct>
+__device__ __forceinline__ float act_grad(float x) {
+    if (kAct == FCAI_ACT_RELU) return x > 0.f ? 1.f : 0.f;
+    if (kAct == FCAI_ACT_GELU) {
+        float e;
+        const float q = normal_tail(fabsf(x), e);
+        return fmaf(x * e, 0.398942280f, x < 0.f ? q : 1.f - q);  // Phi(x) + x phi(x)
+    }
+    if (kAct == FCAI_ACT_SILU) {
+        const float s = rcp_approx(1.f + ex2_approx(-1.44269504f * x));
+        return s * fmaf(x, 1.f - s, 1.f);
+    }
+    return 1.f;
+}
+// The same with the activation chosen at run time (uniform over the kernel).
+__device__ __forceinline__ float act_rt(int kind, float x) {
+    switch (kind) {
+        case FCAI_ACT_RELU: return act<FCAI_ACT_RELU>(x);
+        case FCAI_ACT_GELU: return act<FCAI_ACT_GELU>(x);
+        case FCAI_ACT_SILU: return act<FCAI_ACT_SILU>(x);
+        default: return x;
+    }
+}
+
+// ---- 8-bit blocks ---------------------------------------------------------------
+// The scale of a block from its largest magnitude (given NaN or infinity when
+// the block holds one), and the reciprocal its values are multiplied by.
+template <bool kE4m3>
+__device__ __forceinline__ float block_scale(float amax) {
+    constexpr float kInvTop = kE4m3 ? 1.f / 448.f : 1.f / 127.f;
+    const float s = fmaxf(__fmul_rn(amax, kInvTop), FLT_MIN);
+    return amax <= FLT_MAX ? s : __int_as_float(0x7FC00000);
+}
+// max that keeps a NaN of either side.
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
+    return y;
+}
+template <bool kE4m3>
+__device__ __forceinline__ uint32_t encode4(const float *v, float inv) {
+    if (kE4m3) {
+        const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3);
+        const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3);
+        return (uint32_t)a | ((uint32_t)b << 16);
+    }
+    uint32_t w = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int q = max(-127, min(127, __float2int_rn(v[i] * inv)));  // a NaN converts to 0
+        w |= (uint32_t)(q & 0xFF) << (8 * i);
+    }
+    return w;
+}
+template <bool kE4m3>
+__device__ __forceinline__ void decode4(uint32_t w, float scale, float *v) {
+    if (kE4m3) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * h)), __NV_E4M3);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
+            v[2 * h] = f.x * scale;
+            v[2 * h + 1] = f.y * scale;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i)) * scale;
+    }
+}
+
+inline int dtype_size(int dtype) { return dtype == FCAI_DTYPE_F32 ? 4 : 2; }
+inline bool aligned16(const void *p, int64_t ld, int dtype) {
+    return ((reinterpret_cast<uintptr_t>(p) | (uintptr_t)(ld * dtype_size(dtype))) & 15) == 0;
+}
+
+}  // namespace ly

@@ -436,6 +436,24 @@ __host__ __device__ constexpr uint32_t idesc_bf16(int M, int N) {
            | ((uint32_t)(M >> 4) << 24);     // M / 16
 }
 
+// Whether a 16-bit element type is bf16 (else f16).
+template <typename T> struct T16;
+
+// Instruction descriptor of kind::f16 for operands of one 16-bit type (bf16 or
+// f16), fp32 D; mn_a / mn_b: the operand's tile is MN-major (its M or N axis
+// is contiguous in shared memory).
+template <typename T>
+__host__ __device__ constexpr uint32_t idesc_f16kind(int M, int N, bool mn_a, bool mn_b) {
+    constexpr uint32_t fmt = T16<T>::kBf16 ? 1u : 0u;
+    return (1u << 4)                         // D format: f32
+           | (fmt << 7)                      // A format: f16 (0) or bf16 (1)
+           | (fmt << 10)                     // B format
+           | ((mn_a ? 1u : 0u) << 15)        // A major: K (0) or MN (1)
+           | ((mn_b ? 1u : 0u) << 16)        // B major
+           | ((uint32_t)(N >> 3) << 17)      // N / 8
+           | ((uint32_t)(M >> 4) << 24);     // M / 16
+}
+
 // Instruction descriptor of kind::f8f6f4 with e4m3 A and B (format code 0),
 // fp32 D, both K-major.
 __host__ __device__ constexpr uint32_t idesc_e4m3(int M, int N) {

@@ -1,6 +1,7 @@
 """fast_compressai (B200 build): the FactorizedPrior compress/decompress hot
 path of fast-compressai with sm_100a kernels behind the reference's API."""
 
+from . import layers
 from .api import AccelerationReport, CompileReport, FastModel, accelerate, compile, optimize
 from .coders import (
     BitstreamError,
@@ -47,6 +48,7 @@ __all__ = [
     "compile",
     "create_coder",
     "default_p_candidates",
+    "layers",
     "legal_p_candidates",
     "optimize",
     "sweep_p_ch",
