@@ -21,49 +21,58 @@ using namespace ly;
 constexpr int kThreads = 256;
 constexpr int kBlock = FCAI_KEEP_BLOCK;
 constexpr int kRowsIter = kThreads / 16;  // rows a strip CTA handles at a time
+constexpr int kUnroll = 4;                // rows a strip thread has in flight
 
-// Eight channels from col on (zeros past the row's end).
-template <typename T>
-__device__ __forceinline__ void load8(const T *row, int col, int n, bool vec, float (&v)[8]) {
-    if (vec) {
-        if (col < n) Vec8<T>::load(row + col, v);
+// The eight channels a thread holds of its group's 8 * g: consecutive ones where
+// rows take 16-byte accesses (kV), else every g-th, so that neighbouring lanes
+// still touch neighbouring elements.
+template <bool kV>
+struct Cols {
+    int first, step;
+    __device__ __forceinline__ Cols(int base, int l, int g) : first(kV ? base + l * 8 : base + l), step(kV ? 1 : g) {}
+    __device__ __forceinline__ int operator[](int i) const { return first + i * step; }
+};
+template <typename T, bool kV>
+__device__ __forceinline__ void load8(const T *row, const Cols<kV> &c, int n, bool in, float (&v)[8]) {
+    if (kV) {
+        if (in && c.first < n) Vec8<T>::load(row + c.first, v);
         else
             for (int i = 0; i < 8; ++i) v[i] = 0.f;
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = col + i < n ? to_f32(row[col + i]) : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] = in && c[i] < n ? to_f32(row[c[i]]) : 0.f;
     }
 }
-template <typename T>
-__device__ __forceinline__ void store8(T *row, int col, int n, bool vec, const float (&v)[8]) {
-    if (vec) {
-        if (col < n) Vec8<T>::store(row + col, v);
+template <typename T, bool kV>
+__device__ __forceinline__ void store8(T *row, const Cols<kV> &c, int n, bool in, const float (&v)[8]) {
+    if (kV) {
+        if (in && c.first < n) Vec8<T>::store(row + c.first, v);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (col + i < n) row[col + i] = from_f32<T>(v[i]);
+            if (in && c[i] < n) row[c[i]] = from_f32<T>(v[i]);
     }
 }
-__device__ __forceinline__ void load_codes(const uint8_t *row, int col, int n, bool vec, uint32_t &lo, uint32_t &hi) {
-    lo = hi = 0;
-    if (vec) {
-        if (col < n) {
-            const uint2 q = __ldg(reinterpret_cast<const uint2 *>(row + col));
-            lo = q.x, hi = q.y;
-        }
+template <bool kV>
+__device__ __forceinline__ uint2 load_codes(const uint8_t *row, const Cols<kV> &c, int n, bool in) {
+    uint2 q = make_uint2(0u, 0u);
+    if (kV) {
+        if (in && c.first < n) q = __ldg(reinterpret_cast<const uint2 *>(row + c.first));
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (col + i < n) (i < 4 ? lo : hi) |= (uint32_t)row[col + i] << (8 * (i & 3));
+            if (in && c[i] < n) (i < 4 ? q.x : q.y) |= (uint32_t)row[c[i]] << (8 * (i & 3));
     }
+    return q;
 }
-__device__ __forceinline__ void store_codes(uint8_t *row, int col, int n, bool vec, uint32_t lo, uint32_t hi) {
-    if (vec) {
-        if (col < n) *reinterpret_cast<uint2 *>(row + col) = make_uint2(lo, hi);
+template <bool kV>
+__device__ __forceinline__ void store_codes(uint8_t *row, const Cols<kV> &c, int n, bool in, uint2 q) {
+    if (kV) {
+        if (in && c.first < n) *reinterpret_cast<uint2 *>(row + c.first) = q;
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (col + i < n) row[col + i] = (uint8_t)((i < 4 ? lo : hi) >> (8 * (i & 3)));
+            if (in && c[i] < n) row[c[i]] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
     }
 }
 
@@ -75,55 +84,79 @@ struct Kept {
     const float *scales;
     int keep;
 };
-template <typename T>
-__device__ __forceinline__ void load_kept(const Kept &k, int64_t row, int col, int n, int nblk, bool vec, float (&v)[8]) {
-    if (k.keep == FCAI_KEEP_FULL) {
-        load8(static_cast<const T *>(k.x) + row * k.ldx, col, n, vec, v);
+__device__ __forceinline__ void decode8(int keep, uint2 q, float s, float (&v)[8]) {
+    if (keep == FCAI_KEEP_E4M3) {
+        decode4<true>(q.x, s, v);
+        decode4<true>(q.y, s, v + 4);
     } else {
-        uint32_t lo, hi;
-        load_codes(k.codes + row * n, col, n, vec, lo, hi);
-        const float s = col < n ? __ldg(k.scales + row * nblk + col / kBlock) : 0.f;
-        if (k.keep == FCAI_KEEP_E4M3) {
-            decode4<true>(lo, s, v);
-            decode4<true>(hi, s, v + 4);
-        } else {
-            decode4<false>(lo, s, v);
-            decode4<false>(hi, s, v + 4);
-        }
+        decode4<false>(q.x, s, v);
+        decode4<false>(q.y, s, v + 4);
     }
 }
+// A kept value's bits as they are loaded, before they are decoded: loads of several rows go out together.
+template <typename T, bool kV, bool k8>
+struct KeptRaw {
+    float v[k8 ? 1 : 8];
+    uint2 q;
+    float s;
+    __device__ __forceinline__ void load(const Kept &k, int64_t row, const Cols<kV> &c, int n, int nblk, bool in) {
+        if constexpr (k8) {
+            q = load_codes(k.codes + row * n, c, n, in);
+            s = in && c.first < n ? __ldg(k.scales + row * nblk + c.first / kBlock) : 0.f;
+        } else {
+            load8(static_cast<const T *>(k.x) + row * k.ldx, c, n, in, v);
+        }
+    }
+    __device__ __forceinline__ void get(const Kept &k, float (&o)[8]) const {
+        if constexpr (k8) {
+            decode8(k.keep, q, s, o);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = v[i];
+        }
+    }
+};
 
-// A block's codes and scale, from the 16 lanes that hold its channels (8 each).
-template <bool kE4m3>
-__device__ __forceinline__ void keep_block(const float (&v)[8], uint8_t *codes_row, float *scale, int col, int n, bool vec) {
+// A block's codes and scale, from the kLanes (at most 16) lanes that hold its
+// channels, 8 each; the whole warp calls it.
+template <int kLanes, bool kV>
+__device__ __forceinline__ void keep_block(int keep, const float (&v)[8], uint8_t *codes_row, float *scale, const Cols<kV> &c,
+                                           int n, bool in) {
     float amax = fabsf(v[0]);
 #pragma unroll
     for (int i = 1; i < 8; ++i) amax = max_nan(amax, fabsf(v[i]));
 #pragma unroll
-    for (int d = 8; d >= 1; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
-    const float s = block_scale<kE4m3>(amax);
-    const float inv = __frcp_rn(s);
-    store_codes(codes_row, col, n, vec, encode4<kE4m3>(v, inv), encode4<kE4m3>(v + 4, inv));
-    if ((threadIdx.x & 15) == 0 && col < n) *scale = s;
+    for (int d = (kLanes < 16 ? kLanes : 16) / 2; d >= 1; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
+    uint2 q;
+    float s;
+    if (keep == FCAI_KEEP_E4M3) {
+        s = block_scale<true>(amax);
+        const float inv = __frcp_rn(s);
+        q = make_uint2(encode4<true>(v, inv), encode4<true>(v + 4, inv));
+    } else {
+        s = block_scale<false>(amax);
+        const float inv = __frcp_rn(s);
+        q = make_uint2(encode4<false>(v, inv), encode4<false>(v + 4, inv));
+    }
+    store_codes(codes_row, c, n, in, q);
+    if (in && c.first % kBlock == 0 && c.first < n) *scale = s;
 }
 
-__device__ __forceinline__ void act8(int kind, const float (&x)[8], float (&y)[8]) {
+__device__ __forceinline__ void act8(int kind, float (&y)[8]) {
     switch (kind) {
         case FCAI_ACT_RELU:
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_RELU>(x[i]);
+            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_RELU>(y[i]);
             break;
         case FCAI_ACT_GELU:
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_GELU>(x[i]);
+            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_GELU>(y[i]);
             break;
         case FCAI_ACT_SILU:
 #pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_SILU>(x[i]);
+            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_SILU>(y[i]);
             break;
-        default:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = x[i];
+        default: break;
     }
 }
 __device__ __forceinline__ void act_grad8(int kind, const float (&x)[8], float (&g)[8]) {
@@ -144,189 +177,416 @@ __device__ __forceinline__ void act_grad8(int kind, const float (&x)[8], float (
     }
 }
 
-// ---- activation forward, checkpoint load -------------------------------------
-// One (row, block) per 16 lanes and step.
-template <typename T>
+// ---- strips: activations, checkpoint load ------------------------------------
+// grid (row shares, strips): with the shares in x the launch has no limit of 65535 there.
+template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads)
     act_forward_kernel(const T *__restrict__ x, int64_t ldx, T *__restrict__ y, int64_t ldy, uint8_t *__restrict__ codes,
-                       float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep, int vec) {
-    const int64_t items = rows * nblk;
+                       float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep) {
+    const int strip = blockIdx.y;
+    const Cols<kV> c(strip * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.x * kRowsIter;
-    // both halves of a warp run the same number of steps: the shuffles of a block need the whole warp
-    for (int64_t base = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 5) * 2; base < items; base += step) {
-        const int64_t it = base + ((threadIdx.x >> 4) & 1);
-        const bool in = it < items;
-        const int64_t row = in ? it / nblk : 0;
-        const int blk = (int)(it - row * nblk);
-        const int col = in ? blk * kBlock + (threadIdx.x & 15) * 8 : n;
-        float v[8];
-        load8(x + row * ldx, col, n, vec, v);
-        if (keep == FCAI_KEEP_INT8) keep_block<false>(v, codes + row * n, scales + it, col, n, vec);
-        else if (keep == FCAI_KEEP_E4M3) keep_block<true>(v, codes + row * n, scales + it, col, n, vec);
-        if (y) {
-            float o[8];
-            act8(act, v, o);
-            store8(y + row * ldy, col, n, vec, o);
+    const int sub = (threadIdx.x >> 4) & 1;
+    // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
+    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 5) * 2; r0 < rows; r0 += step * kUnroll) {
+        float v[kUnroll][8];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t row = r0 + u * step + sub;
+            load8(x + row * ldx, c, n, row < rows, v[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t row = r0 + u * step + sub;
+            const bool in = row < rows;
+            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, v[u], codes + row * n, scales + row * nblk + strip, c, n, in);
+            if (y) {
+                act8(act, v[u]);
+                store8(y + row * ldy, c, n, in, v[u]);
+            }
         }
     }
 }
 
-template <typename T>
+template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads)
-    checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk, int vec) {
-    const int64_t items = rows * nblk;
-    for (int64_t it = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); it < items; it += (int64_t)gridDim.x * kRowsIter) {
-        const int64_t row = it / nblk;
-        const int col = (int)(it - row * nblk) * kBlock + (threadIdx.x & 15) * 8;
-        float v[8];
-        load_kept<T>(k, row, col, n, nblk, vec, v);
-        store8(out + row * ldo, col, n, vec, v);
+    checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
+    const Cols<kV> c(blockIdx.y * kBlock, threadIdx.x & 15, 16);
+    const int64_t step = (int64_t)gridDim.x * kRowsIter;
+    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
+        KeptRaw<T, kV, true> raw[kUnroll];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) raw[u].load(k, r0 + u * step, c, n, nblk, r0 + u * step < rows);
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            float v[8];
+            raw[u].get(k, v);
+            store8(out + (r0 + u * step) * ldo, c, n, r0 + u * step < rows, v);
+        }
     }
 }
 
-// ---- strips --------------------------------------------------------------------
-// Adds the 16 row groups' sums of a strip CTA and writes its partial row.
-__device__ __forceinline__ void strip_sums(const float (&acc)[8], float *partial_row, int col, int n, float (*sh)[kBlock]) {
-    const int g = threadIdx.x >> 4, l = threadIdx.x & 15;
+// Adds the sums of a CTA's groups of kLanes threads (8 * kLanes channels from
+// base on) and writes them to a partial row.
+template <int kLanes, int kCta, bool kV>
+__device__ __forceinline__ void group_sums(const float (&acc)[8], float *partial_row, int base, int n, float *sh) {
+    constexpr int kSpan = kLanes * 8;
+    const int g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
+    const Cols<kV> c(0, l % 16 + (kV ? l / 16 * 16 : 0), kLanes < 16 ? kLanes : 16);
+    const int blk = kV ? 0 : l / 16 * kBlock;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sh[g][l * 8 + i] = acc[i];
+    for (int i = 0; i < 8; ++i) sh[g * kSpan + blk + c[i]] = acc[i];
     __syncthreads();
-    if (threadIdx.x < kBlock) {
+    for (int j = threadIdx.x; j < kSpan; j += kCta) {
         float s = 0.f;
 #pragma unroll
-        for (int i = 0; i < kRowsIter; ++i) s += sh[i][threadIdx.x];
-        const int c = col - l * 8 + threadIdx.x;
-        if (c < n) partial_row[c] = s;
+        for (int i = 0; i < kCta / kLanes; ++i) s += sh[i * kSpan + j];
+        if (base + j < n) partial_row[base + j] = s;
     }
 }
 
-// dx = dy act'(x); grid (strips, row shares)
-template <typename T>
+// dx = dy act'(x) and partial sums of it over the CTA's rows
+template <typename T, bool kV, bool k8>
 __global__ void __launch_bounds__(kThreads)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
-                        float *__restrict__ partial, int64_t rows, int n, int nblk, int act, int vec) {
-    __shared__ float sh[kRowsIter][kBlock];
-    const int col = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+                        float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
+    __shared__ float sh[kThreads * 8];
+    const Cols<kV> c(blockIdx.y * kBlock, threadIdx.x & 15, 16);
+    const int64_t step = (int64_t)gridDim.x * kRowsIter;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.y * kRowsIter) {
-        float g[8], x[8];
-        load8(dy + row * lddy, col, n, vec, g);
-        if (act != FCAI_ACT_NONE) {
-            load_kept<T>(k, row, col, n, nblk, vec, x);
-            act_grad8(act, x, g);
-        }
-        if (dx) store8(dx + row * lddx, col, n, vec, g);
+    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
+        float g[kUnroll][8];
+        KeptRaw<T, kV, k8> raw[kUnroll];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] += g[i];
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t row = r0 + u * step;
+            load8(dy + row * lddy, c, n, row < rows, g[u]);
+            if (act != FCAI_ACT_NONE) raw[u].load(k, row, c, n, nblk, row < rows);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int64_t row = r0 + u * step;
+            if (act != FCAI_ACT_NONE) {
+                float x[8];
+                raw[u].get(k, x);
+                act_grad8(act, x, g[u]);
+            }
+            if (dx) store8(dx + row * lddx, c, n, row < rows, g[u]);
+            if (row < rows) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) acc[i] += g[u][i];
+            }
+        }
     }
-    if (partial) strip_sums(acc, partial + (int64_t)blockIdx.y * n, col, n, sh);
+    if (partial) group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.x * n, blockIdx.y * kBlock, n, sh);
 }
 
-// out[c] = sum over the partial rows, in order.
+// Column sums of partial[rows][stride], in a fixed order: columns [0, n0) to
+// out0, [n0, n0 + n1) to out1.  32 columns a CTA, 16 threads down the rows.
 template <typename T>
-__global__ void colsum_kernel(const float *__restrict__ partial, int rows, int64_t stride, T *__restrict__ out, int n) {
-    const int c = blockIdx.x * blockDim.x + threadIdx.x;
-    if (c >= n) return;
+__global__ void __launch_bounds__(512)
+    colsum_kernel(const float *__restrict__ partial, int rows, int64_t stride, T *__restrict__ out0, int n0, T *__restrict__ out1,
+                  int n1) {
+    __shared__ float sh[16][33];
+    const int col = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
-    for (int r = 0; r < rows; ++r) s += partial[r * stride + c];
-    out[c] = from_f32<T>(s);
+    if (col < n0 + n1) {
+#pragma unroll 8
+        for (int r = threadIdx.y; r < rows; r += 16) s += partial[r * stride + col];
+    }
+    sh[threadIdx.y][threadIdx.x] = s;
+    __syncthreads();
+    if (threadIdx.y == 0 && col < n0 + n1) {
+        s = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s += sh[i][threadIdx.x];
+        if (col < n0) {
+            if (out0) out0[col] = from_f32<T>(s);
+        } else if (out1) {
+            out1[col - n0] = from_f32<T>(s);
+        }
+    }
 }
 
 // ---- layer norm ----------------------------------------------------------------
-// Sums over the CTA; every thread gets them.
-__device__ __forceinline__ float2 block_sum2(float a, float b, float2 *sh) {
+// A group of kLanes threads holds a row in registers, kChunks x 8 channels a
+// thread, and reads it from memory once.  Up to 32 lanes the group is part of a
+// warp and sums with shuffles; above, it is the whole CTA and one exchange
+// through shared memory follows (two buffers in turn, so that a sum needs one
+// barrier).
+template <int kLanes>
+struct Group {
+    static constexpr int kCta = kLanes <= 32 ? kThreads : kLanes;
+    static constexpr int kGroups = kCta / kLanes;
+    static constexpr int kWarpsRow = kLanes <= 32 ? 1 : kLanes / 32;
+};
+template <int kLanes>
+__device__ __forceinline__ float2 group_sum2(float a, float b, float2 (*sh)[16], int &turn) {
 #pragma unroll
-    for (int d = 16; d >= 1; d >>= 1) {
+    for (int d = (kLanes < 32 ? kLanes : 32) / 2; d >= 1; d >>= 1) {
         a += __shfl_xor_sync(0xffffffffu, a, d);
         b += __shfl_xor_sync(0xffffffffu, b, d);
     }
-    __syncthreads();  // the previous sums have been read
-    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = make_float2(a, b);
-    __syncthreads();
-    float2 s = make_float2(0.f, 0.f);
+    if constexpr (kLanes > 32) {
+        if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = make_float2(a, b);
+        __syncthreads();
+        a = b = 0.f;
 #pragma unroll
-    for (int w = 0; w < kThreads / 32; ++w) s.x += sh[w].x, s.y += sh[w].y;
-    return s;
+        for (int w = 0; w < kLanes / 32; ++w) a += sh[turn][w].x, b += sh[turn][w].y;
+        turn ^= 1;
+    }
+    return make_float2(a, b);
 }
+template <int kLanes, bool kV>
+__device__ __forceinline__ Cols<kV> chunk_cols(int chunk) {
+    const int l = threadIdx.x % kLanes;
+    if (kLanes <= 16) return Cols<kV>(0, l, kLanes);
+    return Cols<kV>(chunk * kLanes * 8 + l / 16 * kBlock, l % 16, 16);
+}
+
 struct Affine {
     const void *w, *b;
     int f32, vec;
 };
-template <typename T>
-__device__ __forceinline__ void load_affine(const Affine &a, const void *p, int col, int n, float dflt, float (&v)[8]) {
+template <typename T, bool kV>
+__device__ __forceinline__ void load_affine(const Affine &a, const void *p, const Cols<kV> &c, int n, float dflt, float (&v)[8]) {
     if (!p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = dflt;
-    } else if (a.f32) {
-        load8(static_cast<const float *>(p), col, n, a.vec, v);
+    } else if (kV && a.vec) {
+        if (a.f32) load8(static_cast<const float *>(p), c, n, true, v);
+        else load8(static_cast<const T *>(p), c, n, true, v);
     } else {
-        load8(static_cast<const T *>(p), col, n, a.vec, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            v[i] = c[i] >= n ? 0.f : a.f32 ? static_cast<const float *>(p)[c[i]] : to_f32(static_cast<const T *>(p)[c[i]]);
     }
 }
 
-// A CTA per row; the row is read three times (from cache after the first).
-template <typename T>
-__global__ void __launch_bounds__(kThreads)
+// kRows rows a group and step.
+template <typename T, bool kV, int kLanes, int kChunks, int kRows>
+__global__ void __launch_bounds__(Group<kLanes>::kCta)
     norm_forward_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
                         float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
-                        float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep, int vec) {
-    __shared__ float2 sh[kThreads / 32];
+                        float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
+    using G = Group<kLanes>;
+    __shared__ float2 sh[2][16];
+    int turn = 0;
+    const float inv_n = 1.f / n;
+    const int64_t step = (int64_t)gridDim.x * G::kGroups * kRows;
+    // the loop runs on the CTA's first row: shuffles and barriers need everyone
+    for (int64_t r0 = (int64_t)blockIdx.x * G::kGroups * kRows; r0 < rows; r0 += step) {
+        float v[kRows][kChunks][8];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t row = r0 + u * G::kGroups + threadIdx.x / kLanes;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) load8(x + row * ldx, chunk_cols<kLanes, kV>(j), n, row < rows, v[u][j]);
+        }
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t row = r0 + u * G::kGroups + threadIdx.x / kLanes;
+            const bool in = row < rows;
+            float s = 0.f;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += v[u][j][i];
+            const float mean = group_sum2<kLanes>(s, 0.f, sh, turn).x * inv_n;
+            s = 0.f;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float d = (kV ? c.first : c[i]) < n ? v[u][j][i] - mean : 0.f;
+                    s = fmaf(d, d, s);
+                }
+            }
+            const float rstd = 1.f / sqrtf(fmaf(group_sum2<kLanes>(s, 0.f, sh, turn).x, inv_n, eps));
+            if (mean_out && in && threadIdx.x % kLanes == 0) {
+                mean_out[row] = mean;
+                rstd_out[row] = rstd;
+            }
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+                if (keep >= FCAI_KEEP_INT8)
+                    keep_block<kLanes>(keep, v[u][j], codes + row * n, scales + row * nblk + c.first / kBlock, c, n, in);
+                float w[8], b[8];
+                load_affine<T>(af, af.w, c, n, 1.f, w);
+                load_affine<T>(af, af.b, c, n, 0.f, b);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) v[u][j][i] = fmaf((v[u][j][i] - mean) * rstd, w[i], b[i]);
+                store8(y + row * ldy, c, n, in, v[u][j]);
+            }
+        }
+    }
+}
+
+// dx, and the CTA's sums of dy xhat and dy over its rows in partial[CTA][2][n].
+// Each thread keeps its channels' sums in registers from row to row; the next
+// row's loads go out before this row's sums are exchanged.
+template <typename T, bool kV, bool k8, int kLanes, int kChunks>
+__global__ void __launch_bounds__(Group<kLanes>::kCta)
+    norm_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
+                         const float *__restrict__ rstd, Affine af, T *__restrict__ dx, int64_t lddx,
+                         float *__restrict__ partial, int64_t rows, int n, int nblk) {
+    using G = Group<kLanes>;
+    __shared__ float2 sh[2][16];
+    __shared__ float sums[G::kGroups > 1 ? kThreads * 8 : 1];
+    int turn = 0;
+    const float inv_n = 1.f / n;
+    float aw[kChunks][8], ab[kChunks][8];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
+    const int64_t step = (int64_t)gridDim.x * G::kGroups;
+    const int sub = threadIdx.x / kLanes;
+    int64_t r0 = (int64_t)blockIdx.x * G::kGroups;
+    float g[kChunks][8];
+    KeptRaw<T, kV, k8> raw[kChunks];
+    float mu = 0.f, rs = 0.f;
+    auto fetch = [&](int64_t row) {
+        const bool in = row < rows;
+        mu = in ? __ldg(mean + row) : 0.f;
+        rs = in ? __ldg(rstd + row) : 0.f;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+            load8(dy + row * lddy, c, n, in, g[j]);
+            raw[j].load(k, row, c, n, nblk, in);
+        }
+    };
+    fetch(r0 + sub);
+    for (; r0 < rows; r0 += step) {
+        const int64_t row = r0 + sub;
+        const bool in = row < rows;
+        const float rs0 = rs;
+        float t[kChunks][8], xh[kChunks][8];
+        float s1 = 0.f, s2 = 0.f;
+#pragma unroll
+        for (int j = 0; j < kChunks; ++j) {
+            const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+            float w[8];
+            load_affine<T>(af, af.w, c, n, 1.f, w);
+            raw[j].get(k, xh[j]);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                // past the row's end dy is zero; xhat there is kept out of the sums by that
+                xh[j][i] = (xh[j][i] - mu) * rs0;
+                t[j][i] = g[j][i] * w[i];
+                s1 += t[j][i];
+                s2 = fmaf(t[j][i], xh[j][i], s2);
+                aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
+                ab[j][i] += g[j][i];
+            }
+        }
+        if (r0 + step < rows) fetch(row + step);
+        const float2 m = group_sum2<kLanes>(s1, s2, sh, turn);
+        if (dx) {
+            const float m1 = m.x * inv_n, m2 = m.y * inv_n;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) t[j][i] = rs0 * (t[j][i] - m1 - xh[j][i] * m2);
+                store8(dx + row * lddx, chunk_cols<kLanes, kV>(j), n, in, t[j]);
+            }
+        }
+    }
+    if (!partial) return;
+    float *pr = partial + (int64_t)blockIdx.x * 2 * n;
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+        if constexpr (G::kGroups > 1) {
+            group_sums<kLanes, kThreads, kV>(aw[j], pr, j * kLanes * 8, n, sums);
+            group_sums<kLanes, kThreads, kV>(ab[j], pr + n, j * kLanes * 8, n, sums);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (c[i] < n) {
+                    pr[c[i]] = aw[j][i];
+                    pr[n + c[i]] = ab[j][i];
+                }
+        }
+    }
+}
+
+// Rows of more than kMaxHeld channels: a CTA per row that reads it again (from
+// cache) for each step.
+constexpr int kMaxHeld = 16384;
+template <bool kV>
+__device__ __forceinline__ Cols<kV> wide_cols(int c0) {  // c0: a multiple of the CTA's 2048 channels
+    return Cols<kV>(c0 + (threadIdx.x / 16) * kBlock, threadIdx.x & 15, 16);
+}
+template <typename T, bool kV>
+__global__ void __launch_bounds__(kThreads)
+    norm_forward_wide_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
+                             float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
+                             float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
+    __shared__ float2 sh[2][16];
+    int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * ldx;
         float s = 0.f, v[8];
-        for (int col = threadIdx.x * 8; col < n; col += kThreads * 8) {
-            load8(xr, col, n, vec, v);
+        for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
+            load8(xr, wide_cols<kV>(c0), n, true, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) s += v[i];
         }
-        const float mean = block_sum2(s, 0.f, sh).x / n;
+        const float mean = group_sum2<kThreads>(s, 0.f, sh, turn).x / n;
         s = 0.f;
-        for (int col = threadIdx.x * 8; col < n; col += kThreads * 8) {
-            load8(xr, col, n, vec, v);
+        for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
+            const Cols<kV> c = wide_cols<kV>(c0);
+            load8(xr, c, n, true, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float d = col + i < n ? v[i] - mean : 0.f;
+                const float d = c[i] < n ? v[i] - mean : 0.f;
                 s = fmaf(d, d, s);
             }
         }
-        const float rstd = 1.f / sqrtf(block_sum2(s, 0.f, sh).x / n + eps);
+        const float rstd = 1.f / sqrtf(group_sum2<kThreads>(s, 0.f, sh, turn).x / n + eps);
         if (threadIdx.x == 0 && mean_out) {
             mean_out[row] = mean;
             rstd_out[row] = rstd;
         }
-        // whole warps stay in the loop: a block's shuffles need them
-        for (int c0 = (threadIdx.x & ~31) * 8; c0 < n; c0 += kThreads * 8) {
-            const int col = c0 + (threadIdx.x & 31) * 8;
-            load8(xr, col, n, vec, v);
-            float *sc = scales + row * nblk + col / kBlock;
-            if (keep == FCAI_KEEP_INT8) keep_block<false>(v, codes + row * n, sc, col, n, vec);
-            else if (keep == FCAI_KEEP_E4M3) keep_block<true>(v, codes + row * n, sc, col, n, vec);
+        for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
+            const Cols<kV> c = wide_cols<kV>(c0);
+            load8(xr, c, n, true, v);
+            if (keep >= FCAI_KEEP_INT8)
+                keep_block<16>(keep, v, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, true);
             float w[8], b[8];
-            load_affine<T>(af, af.w, col, n, 1.f, w);
-            load_affine<T>(af, af.b, col, n, 0.f, b);
+            load_affine<T>(af, af.w, c, n, 1.f, w);
+            load_affine<T>(af, af.b, c, n, 0.f, b);
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
-            store8(y + row * ldy, col, n, vec, v);
+            store8(y + row * ldy, c, n, true, v);
         }
     }
 }
 
 // Per row: mean(t), mean(t xhat) into stats.
-template <typename T>
+template <typename T, bool kV, bool k8>
 __global__ void __launch_bounds__(kThreads)
     norm_backward_stats_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
                                const float *__restrict__ rstd, Affine af, float2 *__restrict__ stats, int64_t rows, int n,
-                               int nblk, int vec) {
-    __shared__ float2 sh[kThreads / 32];
+                               int nblk) {
+    __shared__ float2 sh[2][16];
+    int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const float mu = mean[row], rs = rstd[row];
         float s1 = 0.f, s2 = 0.f;
-        for (int col = threadIdx.x * 8; col < n; col += kThreads * 8) {
+        for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
+            const Cols<kV> c = wide_cols<kV>(c0);
             float g[8], x[8], w[8];
-            load8(dy + row * lddy, col, n, vec, g);
-            load_kept<T>(k, row, col, n, nblk, vec, x);
-            load_affine<T>(af, af.w, col, n, 1.f, w);
+            KeptRaw<T, kV, k8> raw;
+            load8(dy + row * lddy, c, n, true, g);
+            raw.load(k, row, c, n, nblk, true);
+            raw.get(k, x);
+            load_affine<T>(af, af.w, c, n, 1.f, w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float t = g[i] * w[i];  // zero past the row's end: g is
@@ -334,40 +594,42 @@ __global__ void __launch_bounds__(kThreads)
                 s2 = fmaf(t, (x[i] - mu) * rs, s2);
             }
         }
-        const float2 s = block_sum2(s1, s2, sh);
+        const float2 s = group_sum2<kThreads>(s1, s2, sh, turn);
         if (threadIdx.x == 0) stats[row] = make_float2(s.x / n, s.y / n);
     }
 }
 
-template <typename T>
+template <typename T, bool kV, bool k8>
 __global__ void __launch_bounds__(kThreads)
     norm_backward_strip_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
                                const float *__restrict__ rstd, Affine af, const float2 *__restrict__ stats,
-                               T *__restrict__ dx, int64_t lddx, float *__restrict__ partial, int64_t rows, int n, int nblk,
-                               int vec) {
-    __shared__ float sh[kRowsIter][kBlock];
-    const int col = blockIdx.x * kBlock + (threadIdx.x & 15) * 8;
+                               T *__restrict__ dx, int64_t lddx, float *__restrict__ partial, int64_t rows, int n, int nblk) {
+    __shared__ float sh[kThreads * 8];
+    const int base = blockIdx.y * kBlock;
+    const Cols<kV> c(base, threadIdx.x & 15, 16);
     float w[8], aw[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ab[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    load_affine<T>(af, af.w, col, n, 1.f, w);
-    for (int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.y * kRowsIter) {
+    load_affine<T>(af, af.w, c, n, 1.f, w);
+    for (int64_t row = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.x * kRowsIter) {
         const float mu = mean[row], rs = rstd[row];
         const float2 m = stats[row];
-        float g[8], x[8], o[8];
-        load8(dy + row * lddy, col, n, vec, g);
-        load_kept<T>(k, row, col, n, nblk, vec, x);
+        float g[8], x[8];
+        KeptRaw<T, kV, k8> raw;
+        load8(dy + row * lddy, c, n, true, g);
+        raw.load(k, row, c, n, nblk, true);
+        raw.get(k, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             const float xh = (x[i] - mu) * rs;
-            o[i] = rs * (g[i] * w[i] - m.x - xh * m.y);
             aw[i] = fmaf(g[i], xh, aw[i]);
             ab[i] += g[i];
+            x[i] = rs * (g[i] * w[i] - m.x - xh * m.y);
         }
-        if (dx) store8(dx + row * lddx, col, n, vec, o);
+        if (dx) store8(dx + row * lddx, c, n, true, x);
     }
     if (partial) {
-        float *pr = partial + (int64_t)blockIdx.y * 2 * n;
-        strip_sums(aw, pr, col, n, sh);
-        strip_sums(ab, pr + n, col, n, sh);
+        float *pr = partial + (int64_t)blockIdx.x * 2 * n;
+        group_sums<16, kThreads, kV>(aw, pr, base, n, sh);
+        group_sums<16, kThreads, kV>(ab, pr + n, base, n, sh);
     }
 }
 
@@ -379,14 +641,43 @@ static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 static int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
 static bool codes_vec(const void *codes, int n) { return !codes || ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && n % 8 == 0); }
 
-// CTAs down the rows for `strips` strips: about 4 per SM in all, none without rows.
-static int row_shares(int64_t rows, int strips) {
-    const int64_t want = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 4 + strips - 1) / strips);
-    return (int)std::max<int64_t>(1, std::min<int64_t>({want, (rows + kRowsIter - 1) / kRowsIter, 65535}));
+// Row shares of the strip kernels.  Without sums over rows: shares of kUnroll
+// steps, so that every thread has its kUnroll rows in flight once.  With sums:
+// about 8 CTAs per SM in all, since every share leaves a partial row.
+static int row_shares(int64_t rows, int strips, bool sums) {
+    const int64_t steps = (rows + kRowsIter - 1) / kRowsIter;
+    const int64_t fill = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 8 + strips - 1) / strips);
+    if (sums || steps <= fill) return (int)std::min(steps, fill);
+    return (int)std::max(fill, (steps + kUnroll - 1) / kUnroll);
 }
-static int64_t act_workspace(int64_t rows, int n) { return round256((int64_t)row_shares(rows, blocks_of(n)) * n * 4); }
+// How the layer norm runs rows of n channels: threads a row, 8-channel chunks a thread.
+struct Held {
+    int lanes, chunks;
+};
+static Held held(int n) {
+    if (n <= 32) return {4, 1};
+    if (n <= 128) return {16, 1};
+    if (n <= 256) return {32, 1};
+    if (n <= 512) return {32, 2};
+    if (n <= 1024) return {128, 1};
+    if (n <= 2048) return {256, 1};
+    if (n <= 4096) return {512, 1};
+    if (n <= 8192) return {512, 2};
+    return {512, 4};
+}
+static int norm_backward_grid(int64_t rows, int n) {
+    const Held h = held(n);
+    const int groups = h.lanes <= 32 ? kThreads / h.lanes : 1;
+    const int per_sm = h.lanes <= 32 ? 4 : 1024 / h.lanes / h.chunks > 0 ? 1024 / h.lanes / h.chunks : 1;
+    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
+}
+static int64_t act_workspace(int64_t rows, int n) {
+    return rows ? round256((int64_t)row_shares(rows, blocks_of(n), true) * n * 4) : 0;
+}
 static int64_t norm_workspace(int64_t rows, int n) {
-    return round256(rows * 8) + round256((int64_t)row_shares(rows, blocks_of(n)) * 2 * n * 4);
+    if (rows == 0) return 0;
+    if (n <= kMaxHeld) return round256((int64_t)norm_backward_grid(rows, n) * 2 * n * 4);
+    return round256(rows * 8) + round256((int64_t)row_shares(rows, blocks_of(n), true) * 2 * n * 4);
 }
 
 static int check_sizes(const char *op, int64_t rows, int n, int dtype) {
@@ -415,14 +706,16 @@ static int check_ws(const char *op, int64_t need, const void *ws, int64_t bytes)
         return fcai::fail(FCAI_ERR_WORKSPACE, "%s: needs a 256-byte aligned workspace of %lld bytes", op, (long long)need);
     return FCAI_OK;
 }
-static int item_grid(int64_t rows, int nblk) {
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows * nblk + kRowsIter - 1) / kRowsIter, (int64_t)fcai::sm_count() * 8));
-}
-static int colsum(const float *partial, int rows, int64_t stride, void *out, int n, int dtype, cudaStream_t st) {
-    const int grid = (n + 127) / 128;
-    if (dtype == FCAI_DTYPE_BF16) colsum_kernel<<<grid, 128, 0, st>>>(partial, rows, stride, static_cast<__nv_bfloat16 *>(out), n);
-    else if (dtype == FCAI_DTYPE_F16) colsum_kernel<<<grid, 128, 0, st>>>(partial, rows, stride, static_cast<__half *>(out), n);
-    else colsum_kernel<<<grid, 128, 0, st>>>(partial, rows, stride, static_cast<float *>(out), n);
+static int colsum(const float *partial, int rows, int64_t stride, void *out0, int n0, void *out1, int n1, int dtype,
+                  cudaStream_t st) {
+    const dim3 block(32, 16);
+    const int grid = (n0 + n1 + 31) / 32;
+    if (dtype == FCAI_DTYPE_BF16)
+        colsum_kernel<<<grid, block, 0, st>>>(partial, rows, stride, static_cast<__nv_bfloat16 *>(out0), n0, static_cast<__nv_bfloat16 *>(out1), n1);
+    else if (dtype == FCAI_DTYPE_F16)
+        colsum_kernel<<<grid, block, 0, st>>>(partial, rows, stride, static_cast<__half *>(out0), n0, static_cast<__half *>(out1), n1);
+    else
+        colsum_kernel<<<grid, block, 0, st>>>(partial, rows, stride, static_cast<float *>(out0), n0, static_cast<float *>(out1), n1);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
@@ -432,42 +725,134 @@ template <typename T>
 static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *codes, float *scales, int64_t rows, int n,
                        int dtype, int act, int keep, cudaStream_t st) {
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
-    const int vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
-    act_forward_kernel<T><<<item_grid(rows, blocks_of(n)), kThreads, 0, st>>>(
-        static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales, rows, n, blocks_of(n), act,
-        keep, vec);
+    const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
+    const int strips = blocks_of(n);
+    const dim3 grid(row_shares(rows, strips, false), strips);
+    auto kernel = vec ? act_forward_kernel<T, true> : act_forward_kernel<T, false>;
+    kernel<<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales,
+                                      rows, n, strips, act, q ? keep : FCAI_KEEP_NONE);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
 template <typename T>
 static int act_backward(const void *dy, int64_t lddy, const Kept &k, void *dx, int64_t lddx, void *bias_grad, int64_t rows, int n,
                         int dtype, int act, float *ws, cudaStream_t st) {
-    const int strips = blocks_of(n), shares = row_shares(rows, strips);
-    const bool full = k.keep == FCAI_KEEP_FULL;
-    const int vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
-                    (act == FCAI_ACT_NONE || (full ? aligned16(k.x, k.ldx, dtype) : codes_vec(k.codes, n)));
-    act_backward_kernel<T><<<dim3(strips, shares), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
-                                                                    bias_grad ? ws : nullptr, rows, n, strips, act, vec);
+    const int strips = blocks_of(n), shares = row_shares(rows, strips, bias_grad != nullptr);
+    const bool k8 = act != FCAI_ACT_NONE && k.keep != FCAI_KEEP_FULL;
+    const bool vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
+                     (act == FCAI_ACT_NONE || (k8 ? codes_vec(k.codes, n) : aligned16(k.x, k.ldx, dtype)));
+    auto kernel = k8 ? (vec ? act_backward_kernel<T, true, true> : act_backward_kernel<T, false, true>)
+                     : (vec ? act_backward_kernel<T, true, false> : act_backward_kernel<T, false, false>);
+    kernel<<<dim3(shares, strips), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
+                                                      bias_grad ? ws : nullptr, rows, n, strips, act);
     FCAI_CUDA_TRY(cudaGetLastError());
-    return bias_grad ? colsum(ws, shares, n, bias_grad, n, dtype, st) : FCAI_OK;
+    return bias_grad ? colsum(ws, shares, n, bias_grad, n, nullptr, 0, dtype, st) : FCAI_OK;
 }
 template <typename T>
 static int load_checkpoint(const Kept &k, void *out, int64_t ldo, int64_t rows, int n, int dtype, cudaStream_t st) {
-    const int vec = n % 8 == 0 && aligned16(out, ldo, dtype) && codes_vec(k.codes, n);
-    checkpoint_load_kernel<T><<<item_grid(rows, blocks_of(n)), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, blocks_of(n),
-                                                                                vec);
+    const bool vec = n % 8 == 0 && aligned16(out, ldo, dtype) && codes_vec(k.codes, n);
+    const int strips = blocks_of(n);
+    auto kernel = vec ? checkpoint_load_kernel<T, true> : checkpoint_load_kernel<T, false>;
+    kernel<<<dim3(row_shares(rows, strips, false), strips), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
+
+struct NormForward {
+    const void *x, *w, *b;
+    int64_t ldx, ldy, rows;
+    void *y, *codes;
+    float *mean, *rstd, *scales, eps;
+    int n, keep;
+    Affine af;
+    cudaStream_t st;
+};
+template <typename T, bool kV, int kLanes, int kChunks>
+static int launch_norm_forward(const NormForward &a) {
+    // rows in flight: 4 x 8 values a thread, as far as one row leaves room
+    constexpr int kRows = kLanes > 32 ? 1 : 4 / kChunks;
+    constexpr int64_t kPerCta = (int64_t)Group<kLanes>::kGroups * kRows;
+    const int64_t want = (a.rows + kPerCta - 1) / kPerCta;
+    const int grid = (int)std::min<int64_t>(want, kLanes > 32 ? (int64_t)fcai::sm_count() * (2048 / kLanes) : 0x7FFFFFFF);
+    norm_forward_kernel<T, kV, kLanes, kChunks, kRows><<<grid, Group<kLanes>::kCta, 0, a.st>>>(
+        static_cast<const T *>(a.x), a.ldx, a.af, static_cast<T *>(a.y), a.ldy, a.mean, a.rstd, static_cast<uint8_t *>(a.codes),
+        a.scales, a.rows, a.n, blocks_of(a.n), a.eps, a.keep);
+    FCAI_CUDA_TRY(cudaGetLastError());
+    return FCAI_OK;
+}
+struct NormBackward {
+    const void *dy;
+    int64_t lddy, lddx, rows;
+    Kept k;
+    const float *mean, *rstd;
+    Affine af;
+    void *dx;
+    float *partial;
+    int n;
+    cudaStream_t st;
+};
+template <typename T, bool kV, bool k8, int kLanes, int kChunks>
+static int launch_norm_backward(const NormBackward &a) {
+    norm_backward_kernel<T, kV, k8, kLanes, kChunks><<<norm_backward_grid(a.rows, a.n), Group<kLanes>::kCta, 0, a.st>>>(
+        static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, static_cast<T *>(a.dx), a.lddx, a.partial, a.rows, a.n,
+        blocks_of(a.n));
+    FCAI_CUDA_TRY(cudaGetLastError());
+    return FCAI_OK;
+}
+#define RW_BY_HELD(call)                                             \
+    switch (h.lanes * 8 + h.chunks) {                                \
+        case 4 * 8 + 1: return call(4, 1);                           \
+        case 16 * 8 + 1: return call(16, 1);                         \
+        case 32 * 8 + 1: return call(32, 1);                         \
+        case 32 * 8 + 2: return call(32, 2);                         \
+        case 128 * 8 + 1: return call(128, 1);                       \
+        case 256 * 8 + 1: return call(256, 1);                       \
+        case 512 * 8 + 1: return call(512, 1);                       \
+        case 512 * 8 + 2: return call(512, 2);                       \
+        default: return call(512, 4);                                \
+    }
+template <typename T, bool kV>
+static int norm_forward_held(const NormForward &a) {
+    const Held h = held(a.n);
+#define CALL(lanes, chunks) launch_norm_forward<T, kV, lanes, chunks>(a)
+    RW_BY_HELD(CALL)
+#undef CALL
+}
+template <typename T, bool kV, bool k8>
+static int norm_backward_held(const NormBackward &a) {
+    const Held h = held(a.n);
+#define CALL(lanes, chunks) launch_norm_backward<T, kV, k8, lanes, chunks>(a)
+    RW_BY_HELD(CALL)
+#undef CALL
+}
+
 template <typename T>
 static int norm_forward(const void *x, int64_t ldx, Affine af, int wdtype, void *y, int64_t ldy, float *mean, float *rstd,
                         void *codes, float *scales, int64_t rows, int n, float eps, int dtype, int keep, cudaStream_t st) {
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
-    const int vec = n % 8 == 0 && aligned16(x, ldx, dtype) && aligned16(y, ldy, dtype) && (!q || codes_vec(codes, n));
+    const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && aligned16(y, ldy, dtype) && (!q || codes_vec(codes, n));
     af.vec = n % 8 == 0 && affine_vec(af.w, wdtype) && affine_vec(af.b, wdtype);
-    const int grid = (int)std::min<int64_t>(rows, (int64_t)fcai::sm_count() * 8);
-    norm_forward_kernel<T><<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, af, static_cast<T *>(y), ldy, mean, rstd,
-                                                    static_cast<uint8_t *>(codes), scales, rows, n, blocks_of(n), eps, keep, vec);
+    if (n <= kMaxHeld) {
+        const NormForward a{x, af.w, af.b, ldx, ldy, rows, y, codes, mean, rstd, scales, eps, n, keep, af, st};
+        return vec ? norm_forward_held<T, true>(a) : norm_forward_held<T, false>(a);
+    }
+    auto kernel = vec ? norm_forward_wide_kernel<T, true> : norm_forward_wide_kernel<T, false>;
+    kernel<<<(int)std::min<int64_t>(rows, (int64_t)fcai::sm_count() * 8), kThreads, 0, st>>>(
+        static_cast<const T *>(x), ldx, af, static_cast<T *>(y), ldy, mean, rstd, static_cast<uint8_t *>(codes), scales, rows, n,
+        blocks_of(n), eps, keep);
+    FCAI_CUDA_TRY(cudaGetLastError());
+    return FCAI_OK;
+}
+template <typename T, bool kV, bool k8>
+static int norm_backward_any(const NormBackward &a, float2 *stats, int shares) {
+    if (a.n <= kMaxHeld) return norm_backward_held<T, kV, k8>(a);
+    const int strips = blocks_of(a.n);
+    norm_backward_stats_kernel<T, kV, k8><<<(int)std::min<int64_t>(a.rows, (int64_t)fcai::sm_count() * 8), kThreads, 0, a.st>>>(
+        static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, stats, a.rows, a.n, strips);
+    FCAI_CUDA_TRY(cudaGetLastError());
+    norm_backward_strip_kernel<T, kV, k8><<<dim3(shares, strips), kThreads, 0, a.st>>>(
+        static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, stats, static_cast<T *>(a.dx), a.lddx, a.partial, a.rows,
+        a.n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
@@ -475,23 +860,23 @@ template <typename T>
 static int norm_backward(const void *dy, int64_t lddy, const Kept &k, const float *mean, const float *rstd, Affine af, int wdtype,
                          void *dx, int64_t lddx, void *dweight, void *dbias, int64_t rows, int n, int dtype, unsigned char *ws,
                          cudaStream_t st) {
-    const int strips = blocks_of(n), shares = row_shares(rows, strips);
-    const int vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
-                    (k.keep == FCAI_KEEP_FULL ? aligned16(k.x, k.ldx, dtype) : codes_vec(k.codes, n));
+    const bool k8 = k.keep != FCAI_KEEP_FULL;
+    const bool vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
+                     (k8 ? codes_vec(k.codes, n) : aligned16(k.x, k.ldx, dtype));
     af.vec = n % 8 == 0 && affine_vec(af.w, wdtype);
-    float2 *stats = reinterpret_cast<float2 *>(ws);
-    float *partial = reinterpret_cast<float *>(ws + round256(rows * 8));
-    norm_backward_stats_kernel<T><<<(int)std::min<int64_t>(rows, (int64_t)fcai::sm_count() * 8), kThreads, 0, st>>>(
-        static_cast<const T *>(dy), lddy, k, mean, rstd, af, stats, rows, n, strips, vec);
-    FCAI_CUDA_TRY(cudaGetLastError());
-    norm_backward_strip_kernel<T><<<dim3(strips, shares), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, mean, rstd, af, stats,
-                                                                           static_cast<T *>(dx), lddx,
-                                                                           dweight || dbias ? partial : nullptr, rows, n, strips, vec);
-    FCAI_CUDA_TRY(cudaGetLastError());
-    int rc = FCAI_OK;
-    if (dweight) rc = colsum(partial, shares, 2 * (int64_t)n, dweight, n, wdtype, st);
-    if (!rc && dbias) rc = colsum(partial + n, shares, 2 * (int64_t)n, dbias, n, wdtype, st);
-    return rc;
+    float2 *stats = nullptr;
+    int parts = norm_backward_grid(rows, n);
+    if (n > kMaxHeld) {
+        stats = reinterpret_cast<float2 *>(ws);
+        ws += round256(rows * 8);
+        parts = row_shares(rows, blocks_of(n), true);
+    }
+    float *partial = dweight || dbias ? reinterpret_cast<float *>(ws) : nullptr;
+    const NormBackward a{dy, lddy, lddx, rows, k, mean, rstd, af, dx, partial, n, st};
+    const int rc = k8 ? (vec ? norm_backward_any<T, true, true>(a, stats, parts) : norm_backward_any<T, false, true>(a, stats, parts))
+                      : (vec ? norm_backward_any<T, true, false>(a, stats, parts) : norm_backward_any<T, false, false>(a, stats, parts));
+    if (rc || !partial) return rc;
+    return colsum(partial, parts, 2 * (int64_t)n, dweight, n, dbias, n, wdtype, st);
 }
 
 // Sums over no rows.

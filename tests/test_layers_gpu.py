@@ -282,7 +282,8 @@ def test_layer_norm(cuda_device, rows, n, dtype, keep):
     if keep != "full":
         kept = saved.kept.load(torch.float32)
         assert torch.equal(kept, R.keep8(x, keep)[0])
-    grads = layers.layer_norm_backward(_sliced(dy) if keep == "int8" else dy, saved, w)
+    dy = _sliced(dy) if keep == "int8" else dy
+    grads = layers.layer_norm_backward(dy, saved, w)
     for name, t, (g, e) in zip(("dx", "dw", "db"), grads, R.norm_grads(dy, kept, x, w, 1e-4, dtype, wdtype)):
         assert t.dtype == (dtype if name == "dx" else wdtype)
         R.check(t, g, e, name)
