@@ -78,60 +78,127 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
+// Two fp32 values in a register pair: sm_100 computes both with one
+// instruction, which halves the arithmetic of the epilogues and elementwise
+// kernels (they are otherwise bound by instruction issue with GELU).
+struct F2 {
+    uint64_t r;
+};
+__device__ __forceinline__ F2 f2(float a, float b) {
+    F2 v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v.r) : "f"(a), "f"(b));
+    return v;
+}
+__device__ __forceinline__ F2 f2(float a) { return f2(a, a); }
+__device__ __forceinline__ float2 split(F2 v) {
+    float2 o;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(o.x), "=f"(o.y) : "l"(v.r));
+    return o;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 v;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(v.r) : "l"(a.r), "l"(b.r), "l"(c.r));
+    return v;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 v;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(v.r) : "l"(a.r), "l"(b.r));
+    return v;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 v;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(v.r) : "l"(a.r), "l"(b.r));
+    return v;
+}
+
 // The normal distribution's upper tail Q(t) = erfc(t / sqrt 2) / 2, t >= 0, as
 // e * R(u) with e = exp(-t^2 / 2), u = 1 / (1 + 0.24 t) and R a polynomial
 // without constant term, the form of Hastings' approximations (Approximations
 // for Digital Computers, 1955).  The coefficients are a fit of this project's
 // own: iteratively reweighted least squares of R against Q e^(t^2/2) on
 // t in [0, 40], largest relative error 7.6e-7 evaluated in fp32.  `e` comes
-// back for the density.  15 instructions, two of them of the special function
-// unit, which keeps the elementwise kernels bound by memory.
-__device__ __forceinline__ float normal_tail(float t, float &e) {
-    e = ex2_approx(-0.72134752f * t * t);  // log2(e) / 2
-    const float u = rcp_approx(fmaf(0.24f, t, 1.f));
-    float r = fmaf(u, -0.0529928472f, 0.152797519f);
-    r = fmaf(u, r, -0.0657069748f);
-    r = fmaf(u, r, 0.118390834f);
-    r = fmaf(u, r, 0.0633970503f);
-    r = fmaf(u, r, 0.0928386496f);
-    r = fmaf(u, r, 0.0955221622f);
-    r = fmaf(u, r, 0.0957537928f);
-    return e * (u * r);
+// back for the density.
+__device__ __forceinline__ F2 normal_tail2(float2 t, F2 &e) {
+    const F2 tt = f2(t.x, t.y);
+    const float2 a = split(mul2(mul2(tt, f2(-0.72134752f)), tt));  // log2(e) / 2
+    const float2 d = split(fma2(f2(0.24f), tt, f2(1.f)));
+    e = f2(ex2_approx(a.x), ex2_approx(a.y));
+    const F2 u = f2(rcp_approx(d.x), rcp_approx(d.y));
+    F2 r = fma2(u, f2(-0.0529928472f), f2(0.152797519f));
+    r = fma2(u, r, f2(-0.0657069748f));
+    r = fma2(u, r, f2(0.118390834f));
+    r = fma2(u, r, f2(0.0633970503f));
+    r = fma2(u, r, f2(0.0928386496f));
+    r = fma2(u, r, f2(0.0955221622f));
+    r = fma2(u, r, f2(0.0957537928f));
+    return mul2(e, mul2(u, r));
+}
+// Phi(x) of two values.
+__device__ __forceinline__ F2 normal_cdf2(float2 x, F2 &e) {
+    const F2 q = normal_tail2(make_float2(fabsf(x.x), fabsf(x.y)), e);
+    const float2 lo = split(q), hi = split(fma2(q, f2(-1.f), f2(1.f)));
+    return f2(x.x < 0.f ? lo.x : hi.x, x.y < 0.f ? lo.y : hi.y);
+}
+__device__ __forceinline__ F2 sigmoid2(F2 x) {
+    const float2 a = split(mul2(x, f2(-1.44269504f)));
+    const float2 d = split(add2(f2(ex2_approx(a.x), ex2_approx(a.y)), f2(1.f)));
+    return f2(rcp_approx(d.x), rcp_approx(d.y));
 }
 
-template <int kAct>
-__device__ __forceinline__ float act(float x) {
-    if (kAct == FCAI_ACT_RELU) return x < 0.f ? 0.f : x;  // a NaN stays
-    if (kAct == FCAI_ACT_GELU) {
-        float e;
-        const float q = normal_tail(fabsf(x), e);
-        return x * (x < 0.f ? q : 1.f - q);
+// v = act(v) of kN values (a multiple of 2); `kind` is the same for the whole kernel.
+template <int kN>
+__device__ __forceinline__ void act_n(int kind, float (&v)[kN]) {
+    if (kind == FCAI_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // a NaN stays
+    } else if (kind == FCAI_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) {
+            F2 e;
+            const float2 x = make_float2(v[i], v[i + 1]);
+            const float2 y = split(mul2(f2(x.x, x.y), normal_cdf2(x, e)));
+            v[i] = y.x, v[i + 1] = y.y;
+        }
+    } else if (kind == FCAI_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) {
+            const F2 x = f2(v[i], v[i + 1]);
+            const float2 y = split(mul2(x, sigmoid2(x)));
+            v[i] = y.x, v[i + 1] = y.y;
+        }
     }
-    if (kAct == FCAI_ACT_SILU) return x * rcp_approx(1.f + ex2_approx(-1.44269504f * x));
-    return x;
 }
-template <int kAct>
-__device__ __forceinline__ float act_grad(float x) {
-    if (kAct == FCAI_ACT_RELU) return x > 0.f ? 1.f : 0.f;
-    if (kAct == FCAI_ACT_GELU) {
-        float e;
-        const float q = normal_tail(fabsf(x), e);
-        return fmaf(x * e, 0.398942280f, x < 0.f ? q : 1.f - q);  // Phi(x) + x phi(x)
+// g *= act'(x)
+template <int kN>
+__device__ __forceinline__ void act_grad_n(int kind, const float (&x)[kN], float (&g)[kN]) {
+    if (kind == FCAI_ACT_RELU) {
+#pragma unroll
+        for (int i = 0; i < kN; ++i) g[i] *= x[i] > 0.f ? 1.f : 0.f;
+    } else if (kind == FCAI_ACT_GELU) {
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) {
+            F2 e;
+            const float2 xx = make_float2(x[i], x[i + 1]);
+            const F2 cdf = normal_cdf2(xx, e);
+            const F2 d = fma2(mul2(f2(xx.x, xx.y), e), f2(0.398942280f), cdf);  // Phi(x) + x phi(x)
+            const float2 y = split(mul2(f2(g[i], g[i + 1]), d));
+            g[i] = y.x, g[i + 1] = y.y;
+        }
+    } else if (kind == FCAI_ACT_SILU) {
+#pragma unroll
+        for (int i = 0; i < kN; i += 2) {
+            const F2 xx = f2(x[i], x[i + 1]);
+            const F2 s = sigmoid2(xx);
+            const F2 d = mul2(s, fma2(xx, fma2(s, f2(-1.f), f2(1.f)), f2(1.f)));
+            const float2 y = split(mul2(f2(g[i], g[i + 1]), d));
+            g[i] = y.x, g[i + 1] = y.y;
+        }
     }
-    if (kAct == FCAI_ACT_SILU) {
-        const float s = rcp_approx(1.f + ex2_approx(-1.44269504f * x));
-        return s * fmaf(x, 1.f - s, 1.f);
-    }
-    return 1.f;
 }
-// The same with the activation chosen at run time (uniform over the kernel).
-__device__ __forceinline__ float act_rt(int kind, float x) {
-    switch (kind) {
-        case FCAI_ACT_RELU: return act<FCAI_ACT_RELU>(x);
-        case FCAI_ACT_GELU: return act<FCAI_ACT_GELU>(x);
-        case FCAI_ACT_SILU: return act<FCAI_ACT_SILU>(x);
-        default: return x;
-    }
+__device__ __forceinline__ float act_1(int kind, float x) {
+    float v[2] = {x, 0.f};
+    act_n(kind, v);
+    return v[0];
 }
 
 // ---- 8-bit blocks ---------------------------------------------------------------

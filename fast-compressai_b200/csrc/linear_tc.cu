@@ -67,12 +67,15 @@ struct Params {
     float *partial;                    // [splits][M][ldp], or NULL
 };
 
-template <int kBN>
+// A tile is kPair ? 256 : 128 rows by kBN columns.
+template <int kBN, bool kPair>
 struct Layout {
+    static constexpr int kNB = kPair ? kBN / 2 : kBN;  // rows of B this CTA stages
+    static constexpr int kTileM = kPair ? 2 * kBM : kBM;
     static constexpr int kA = kBM * kBK * 2;
-    static constexpr int kB = kBN * kBK * 2;
+    static constexpr int kB = kNB * kBK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = kBN == 64 ? 8 : 6;
+    static constexpr int kStages = kNB == 64 ? 8 : 6;
     static constexpr int offStaging = kStages * kStage;
     static constexpr int offBar = offStaging + kEpiWarps * kStagingWarp;
     static constexpr int kBars = 2 * kStages + 2 * 2 + 1;
@@ -81,15 +84,6 @@ struct Layout {
     static constexpr int kAlloc = kBytes + 1024;  // the base is rounded up to 1024
     static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
-
-__device__ __forceinline__ void tma_load_2d_w(void *dst, const CUtensorMap *map, uint64_t *bar, int c0, int c1) {
-    asm volatile(
-        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
-        "@e cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
-        "[%4];\n\t}" ::"r"(smem_u32(dst)),
-        "l"(reinterpret_cast<uint64_t>(map)), "r"(c0), "r"(c1), "r"(smem_u32(bar))
-        : "memory");
-}
 
 // Unit -> (row tile, column tile, split).  Tiles run through groups of group_m
 // row tiles, column by column, so that the CTAs of a wave share operand tiles
@@ -105,29 +99,55 @@ __device__ __forceinline__ void unit_coords(const Params &p, int unit, int &tm, 
     tm = g * p.group_m + rest - tn * gm;
 }
 
-// Epilogue of 8 neighbouring columns of one row.
-template <typename T>
-__device__ __forceinline__ void finish8(const Params &p, int64_t row, int col, float (&v)[8], const float (&bias)[8]) {
+// Epilogue of kR rows' 8 neighbouring columns from `col` on; rows at
+// `row + i * row_step`, those from M on left out.  All rows go through each
+// step together, so that their loads and arithmetic overlap.
+template <typename T, int kR>
+__device__ __forceinline__ void finish(const Params &p, int64_t row, int row_step, int col, float (&v)[kR * 8]) {
+    if (p.bias) {
+        float bias[8];
+        Vec8<T>::load(static_cast<const T *>(p.bias) + col, bias);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] += bias[i];
-    if (p.pre) Vec8<T>::store(static_cast<T *>(p.pre) + row * p.ldpre + col, v);
-    if (p.act != FCAI_ACT_NONE) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = act_rt(p.act, v[i]);
+        for (int i = 0; i < kR * 8; ++i) v[i] += bias[i & 7];
     }
+    if (p.pre) {
+#pragma unroll
+        for (int i = 0; i < kR; ++i)
+            if (row + i * row_step < p.M) {
+                float o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) o[e] = v[i * 8 + e];
+                Vec8<T>::store(static_cast<T *>(p.pre) + (row + i * row_step) * p.ldpre + col, o);
+            }
+    }
+    uint4 res[kR];
     if (p.residual) {
-        float r[8];
-        Vec8<T>::load(static_cast<const T *>(p.residual) + row * p.ldr + col, r);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] += r[i];
+        for (int i = 0; i < kR; ++i)
+            if (row + i * row_step < p.M)
+                res[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + (row + i * row_step) * p.ldr + col));
     }
-    Vec8<T>::store(static_cast<T *>(p.y) + row * p.ldy + col, v);
+    act_n(p.act, v);
+#pragma unroll
+    for (int i = 0; i < kR; ++i) {
+        if (row + i * row_step >= p.M) continue;
+        float o[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = v[i * 8 + e];
+        if (p.residual) {
+            float r[8];
+            Vec8<T>::unpack(res[i], r);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] += r[e];
+        }
+        Vec8<T>::store(static_cast<T *>(p.y) + (row + i * row_step) * p.ldy + col, o);
+    }
 }
 template <typename T>
 __device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, float v, float bias) {
     v += bias;
     if (p.pre) static_cast<T *>(p.pre)[row * p.ldpre + col] = from_f32<T>(v);
-    v = act_rt(p.act, v);
+    v = act_1(p.act, v);
     if (p.residual) v += to_f32(static_cast<const T *>(p.residual)[row * p.ldr + col]);
     static_cast<T *>(p.y)[row * p.ldy + col] = from_f32<T>(v);
 }
@@ -138,29 +158,36 @@ __device__ __forceinline__ void write_chunk(const Params &p, const unsigned char
                                             int lane) {
     if (col0 >= p.N) return;
     if (p.partial || p.vec) {
-        const int c = (lane & 3) * 8, col = col0 + c;
+        const int col = col0 + (lane & 3) * 8, r0 = lane >> 2;
         if (col >= (p.partial ? p.ldp : p.N)) return;  // both multiples of 8
-        float bias[8];
-        if (!p.partial) {
-            if (p.bias) Vec8<T>::load(static_cast<const T *>(p.bias) + col, bias);
-            else
-                for (int i = 0; i < 8; ++i) bias[i] = 0.f;
-        }
+        float v[32];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + (lane >> 2), row = row0 + r;
-            if (row >= p.M) continue;
+            const int r = i * 8 + r0;
             const float4 a = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3)) ^ (r & 7)) << 4));
             const float4 b = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3) + 1) ^ (r & 7)) << 4));
-            float v[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-            if (p.partial) Vec8<float>::store(p.partial + ((int64_t)sp * p.M + row) * p.ldp + col, v);
-            else finish8<T>(p, row, col, v, bias);
+            v[8 * i] = a.x, v[8 * i + 1] = a.y, v[8 * i + 2] = a.z, v[8 * i + 3] = a.w;
+            v[8 * i + 4] = b.x, v[8 * i + 5] = b.y, v[8 * i + 6] = b.z, v[8 * i + 7] = b.w;
+        }
+        if (p.partial) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = row0 + i * 8 + r0;
+                if (row >= p.M) break;
+                float4 *dst = reinterpret_cast<float4 *>(p.partial + ((int64_t)sp * p.M + row) * p.ldp + col);
+                dst[0] = make_float4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3]);
+                dst[1] = make_float4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]);
+            }
+        } else {
+            finish<T, 4>(p, row0 + r0, 8, col, v);
         }
     } else {
         const int col = col0 + lane;
         if (col >= p.N) return;
         const float bias = p.bias ? to_f32(static_cast<const T *>(p.bias)[col]) : 0.f;
-        for (int r = 0; r < 32 && row0 + r < p.M; ++r) {
+#pragma unroll 4
+        for (int r = 0; r < 32; ++r) {
+            if (row0 + r >= p.M) break;
             const float v = *reinterpret_cast<const float *>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
             finish1<T>(p, row0 + r, col, v, bias);
         }
@@ -168,24 +195,31 @@ __device__ __forceinline__ void write_chunk(const Params &p, const unsigned char
 }
 
 // kTA / kTB: the operand's rows run along K (its M / N axis is contiguous).
-template <typename T, int kBN, bool kTA, bool kTB>
+// kPair: clusters of two CTAs share each MMA (cta_group::2, M = 256): each CTA
+// stages its 128 rows of A and half the columns' rows of B and owns 128 rows
+// of the accumulator; the rank-0 CTA issues for both.
+template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
 __global__ void __launch_bounds__(kThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
-    using Lay = Layout<kBN>;
+    using Lay = Layout<kBN, kPair>;
     constexpr int kStages = Lay::kStages;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Lay::offBar);
+    uint64_t *full = reinterpret_cast<uint64_t *>(smem + Lay::offBar);  // pairs: rank 0's counts both CTAs' loads
     uint64_t *empty = full + kStages;
-    uint64_t *accf = empty + kStages;  // accumulator filled (by the MMA warp)
-    uint64_t *acce = accf + 2;         // accumulator read (one arrival per epilogue warp)
+    uint64_t *accf = empty + kStages;  // accumulator filled (by the MMA warp; pairs: in both CTAs)
+    uint64_t *acce = accf + 2;         // accumulator read: one arrival per epilogue warp (pairs: of both CTAs, at rank 0)
     uint64_t *dbar = acce + 2;         // abort path: this CTA's MMAs drained
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::offSlot);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + Lay::offSlot + 4);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
+    const uint32_t rank = kPair ? cluster_ctarank() : 0u;
+    const bool leader = rank == 0;
+    const int unit0 = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
+    const int unit_step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
     constexpr uint32_t kTmemCols = 2 * kBN;
 
     if (threadIdx.x == 0) {
@@ -195,18 +229,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], kEpiWarps);
+            mbar_init(&acce[b], kPair ? 2 * kEpiWarps : kEpiWarps);
         }
         mbar_init(dbar, 1);
         *abort = 0;
         fence_barrier_init();
     }
     if (warp == kEpiWarps + 1) {
-        tmem_alloc(tmem_slot, kTmemCols);
-        tmem_relinquish();
+        if (kPair) {
+            tmem_alloc_pair(tmem_slot, kTmemCols);
+            tmem_relinquish_pair();
+        } else {
+            tmem_alloc(tmem_slot, kTmemCols);
+            tmem_relinquish();
+        }
     }
     tc_fence_before();
     __syncthreads();
+    // pairs: both CTAs' barriers exist before any remote arrive or load names them
+    if (kPair) cluster_sync_all();
     tc_fence_after();
     const uint32_t tmem_base = *tmem_slot;
 
@@ -218,12 +259,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         __syncwarp();
         uint32_t it = 0;
-        int last_round[kStages];
-        for (int s = 0; s < kStages; ++s) last_round[s] = -1;
         bool stop = false;
-        for (int unit = blockIdx.x; unit < p.units && !stop; unit += gridDim.x) {
+        for (int unit = unit0; unit < p.units && !stop; unit += unit_step) {
             int tm, tn, sp;
             unit_coords(p, unit, tm, tn, sp);
+            const int m0 = tm * Lay::kTileM + (int)rank * kBM, n0 = tn * kBN + (int)rank * Lay::kNB;
             const int k1 = min((sp + 1) * p.ksteps_split, p.ksteps);
             for (int ks = sp * p.ksteps_split; ks < k1; ++ks, ++it) {
                 const int s = it % kStages;
@@ -234,69 +274,94 @@ __global__ void __launch_bounds__(kThreads, 1)
                     break;
                 }
                 unsigned char *st = smem + s * Lay::kStage;
-                mbar_arrive_expect_tx_w(&full[s], Lay::kStage);
-                if (kTA) {
-                    tma_load_2d_w(st, &tmA, &full[s], tm * kBM, ks * kBK);
-                    tma_load_2d_w(st + 8192, &tmA, &full[s], tm * kBM + 64, ks * kBK);
-                } else {
-                    tma_load_2d_w(st, &tmA, &full[s], ks * kBK, tm * kBM);
-                }
-                if (kTB) {
+                const int k0 = ks * kBK;
+                if constexpr (kPair) {
+                    const uint32_t fb = mapa_shared(smem_u32(&full[s]), 0);
+                    if (leader) mbar_arrive_expect_tx_w(&full[s], 2 * Lay::kStage);
+                    if (kTA) {
+                        tma_load_2d_pair_w(st, &tmA, fb, m0, k0);
+                        tma_load_2d_pair_w(st + 8192, &tmA, fb, m0 + 64, k0);
+                    } else {
+                        tma_load_2d_pair_w(st, &tmA, fb, k0, m0);
+                    }
+                    if (kTB) {
 #pragma unroll
-                    for (int n = 0; n < kBN; n += 64)
-                        tma_load_2d_w(st + Lay::kA + n * 128, &tmB, &full[s], tn * kBN + n, ks * kBK);
+                        for (int n = 0; n < Lay::kNB; n += 64)
+                            tma_load_2d_pair_w(st + Lay::kA + n * 128, &tmB, fb, n0 + n, k0);
+                    } else {
+                        tma_load_2d_pair_w(st + Lay::kA, &tmB, fb, k0, n0);
+                    }
                 } else {
-                    tma_load_2d_w(st + Lay::kA, &tmB, &full[s], ks * kBK, tn * kBN);
+                    mbar_arrive_expect_tx_w(&full[s], Lay::kStage);
+                    if (kTA) {
+                        tma_load_2d_w(st, &tmA, &full[s], m0, k0);
+                        tma_load_2d_w(st + 8192, &tmA, &full[s], m0 + 64, k0);
+                    } else {
+                        tma_load_2d_w(st, &tmA, &full[s], k0, m0);
+                    }
+                    if (kTB) {
+#pragma unroll
+                        for (int n = 0; n < Lay::kNB; n += 64)
+                            tma_load_2d_w(st + Lay::kA + n * 128, &tmB, &full[s], n0 + n, k0);
+                    } else {
+                        tma_load_2d_w(st + Lay::kA, &tmB, &full[s], k0, n0);
+                    }
                 }
-                last_round[s] = (int)r;
             }
         }
-        if (*abort) {
-            // the loads in flight land before the CTA exits
+        if (*abort && leader) {
+            // the loads in flight land before the CTA exits (pairs: rank 0's
+            // barriers also count the peer's loads): the last rounds issued
             for (int s = 0; s < kStages; ++s)
-                if (last_round[s] >= 0) mbar_wait(&full[s], (uint32_t)last_round[s] & 1, nullptr, kWaitNs / 10);
+                if (it > (uint32_t)s) mbar_wait(&full[s], ((it - 1 - s) / kStages) & 1, nullptr, kWaitNs / 10);
         }
         __syncwarp();
     } else if (warp == kEpiWarps + 1) {
         // ---------------------------------------------------------- MMA issuer
-        constexpr uint32_t idesc = idesc_f16kind<T>(kBM, kBN, kTA, kTB);
-        uint32_t it = 0;
-        int j = 0;
-        bool ok = true;
-        for (int unit = blockIdx.x; unit < p.units && ok; unit += gridDim.x, ++j) {
-            int tm, tn, sp;
-            unit_coords(p, unit, tm, tn, sp);
-            const int buf = j & 1;
-            if (!mbar_wait_warp(&acce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs)) {
-                *abort = 1;
-                break;
-            }
-            tc_fence_after();
-            const uint32_t d = tmem_base + buf * kBN;
-            const int k0 = sp * p.ksteps_split, k1 = min(k0 + p.ksteps_split, p.ksteps);
-            for (int ks = k0; ks < k1; ++ks, ++it) {
-                const int s = it % kStages;
-                if (!mbar_wait_warp(&full[s], (it / kStages) & 1, abort, kWaitNs)) {
+        if (leader) {
+            constexpr uint32_t idesc = idesc_f16kind<T>(Lay::kTileM, kBN, kTA, kTB);
+            uint32_t it = 0;
+            int j = 0;
+            bool ok = true;
+            for (int unit = unit0; unit < p.units && ok; unit += unit_step, ++j) {
+                int tm, tn, sp;
+                unit_coords(p, unit, tm, tn, sp);
+                const int buf = j & 1;
+                if (!mbar_wait_warp(&acce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs, kPair)) {
                     *abort = 1;
-                    ok = false;
                     break;
                 }
                 tc_fence_after();
-                const uint32_t a0 = smem_u32(smem + s * Lay::kStage), b0 = a0 + Lay::kA;
+                const uint32_t d = tmem_base + buf * kBN;
+                const int k0 = sp * p.ksteps_split, k1 = min(k0 + p.ksteps_split, p.ksteps);
+                for (int ks = k0; ks < k1; ++ks, ++it) {
+                    const int s = it % kStages;
+                    if (!mbar_wait_warp(&full[s], (it / kStages) & 1, abort, kWaitNs)) {
+                        *abort = 1;
+                        ok = false;
+                        break;
+                    }
+                    tc_fence_after();
+                    const uint32_t a0 = smem_u32(smem + s * Lay::kStage), b0 = a0 + Lay::kA;
 #pragma unroll
-                for (int kk = 0; kk < kBK / 16; ++kk) {
-                    // K-major tiles: 16 k are 32 bytes of the 128-byte row, row
-                    // groups of 8 are 1024 bytes apart.  MN-major tiles: 16 k
-                    // are two groups of 8 rows, 1024 bytes apart, and blocks
-                    // of 64 along M / N are 8192 bytes apart.
-                    const uint64_t ad = kTA ? smem_desc(a0 + kk * 2048, 8192, 1024, 2) : smem_desc(a0 + kk * 32, 16, 1024, 2);
-                    const uint64_t bd = kTB ? smem_desc(b0 + kk * 2048, 8192, 1024, 2) : smem_desc(b0 + kk * 32, 16, 1024, 2);
-                    mma_bf16_w(d, ad, bd, idesc, (ks > k0 || kk > 0) ? 1u : 0u);
+                    for (int kk = 0; kk < kBK / 16; ++kk) {
+                        // K-major tiles: 16 k are 32 bytes of the 128-byte row, row
+                        // groups of 8 are 1024 bytes apart.  MN-major tiles: 16 k
+                        // are two groups of 8 rows, 1024 bytes apart, and blocks
+                        // of 64 along M / N are 8192 bytes apart.
+                        const uint64_t ad = kTA ? smem_desc(a0 + kk * 2048, 8192, 1024, 2) : smem_desc(a0 + kk * 32, 16, 1024, 2);
+                        const uint64_t bd = kTB ? smem_desc(b0 + kk * 2048, 8192, 1024, 2) : smem_desc(b0 + kk * 32, 16, 1024, 2);
+                        const uint32_t acc = (ks > k0 || kk > 0) ? 1u : 0u;
+                        if (kPair) mma_bf16_pair_w(d, ad, bd, idesc, acc);
+                        else mma_bf16_w(d, ad, bd, idesc, acc);
+                    }
+                    if (kPair) mma_commit_pair_both_w(&empty[s], 3);
+                    else mma_commit_w(&empty[s]);
                 }
-                mma_commit_w(&empty[s]);
+                if (!ok) break;
+                if (kPair) mma_commit_pair_both_w(&accf[buf], 3);
+                else mma_commit_w(&accf[buf]);
             }
-            if (!ok) break;
-            mma_commit_w(&accf[buf]);
         }
         __syncwarp();
     } else {
@@ -304,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int q = warp & 3, half = warp >> 2;
         unsigned char *stg = smem + Lay::offStaging + warp * kStagingWarp;
         int j = 0;
-        for (int unit = blockIdx.x; unit < p.units; unit += gridDim.x, ++j) {
+        for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
             int tm, tn, sp;
             unit_coords(p, unit, tm, tn, sp);
             const int buf = j & 1;
@@ -313,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 break;
             }
             tc_fence_after();
-            const int row0 = tm * kBM + q * 32;
+            const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
             const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
             for (int c = half * (kBN / 2); c < (half + 1) * (kBN / 2); c += 32) {
@@ -323,7 +388,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (c + 32 == (half + 1) * (kBN / 2)) {  // this warp has read its part of the accumulator
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&acce[buf]);
+                    if (lane == 0) {
+                        if (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[buf]), 0));
+                        else mbar_arrive(&acce[buf]);
+                    }
                 }
                 if (row0 < p.M) {
 #pragma unroll
@@ -340,18 +408,25 @@ __global__ void __launch_bounds__(kThreads, 1)
 
     // ---------------------------------------------------------------- teardown
     __syncthreads();
-    if (*abort) {
+    if (*abort && leader) {
         // TMEM is freed only once every MMA issued has completed
         if (warp == kEpiWarps + 1) {
-            mma_commit_w(dbar);
-            mbar_wait(dbar, 0, nullptr, kWaitNs / 10);
+            if (lane == 0) {
+                if (kPair) mma_commit_pair(dbar);
+                else mma_commit(dbar);
+                mbar_wait(dbar, 0, nullptr, kWaitNs / 10);
+            }
+            __syncwarp();
         }
         __syncthreads();
     }
+    // pairs: no remote arrive, load or MMA reaches a CTA that has left
+    if (kPair) cluster_sync_all();
     if (warp == kEpiWarps + 1) {
         __syncwarp();
         tc_fence_after();
-        tmem_dealloc(tmem_base, kTmemCols);
+        if (kPair) tmem_dealloc_pair(tmem_base, kTmemCols);
+        else tmem_dealloc(tmem_base, kTmemCols);
     }
 }
 
@@ -373,11 +448,7 @@ __global__ void reduce_kernel(const Params p) {
             for (int e = 0; e < 8; ++e) v[e] += u[e];
         }
         if (p.vec) {
-            float bias[8];
-            if (p.bias) Vec8<T>::load(static_cast<const T *>(p.bias) + col, bias);
-            else
-                for (int e = 0; e < 8; ++e) bias[e] = 0.f;
-            finish8<T>(p, row, col, v, bias);
+            finish<T, 1>(p, row, 0, col, v);
         } else {
             for (int e = 0; e < 8 && col + e < p.N; ++e)
                 finish1<T>(p, row, col + e, v[e], p.bias ? to_f32(static_cast<const T *>(p.bias)[col + e]) : 0.f);
@@ -440,25 +511,51 @@ static int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t o
 static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 static int round8(int v) { return (v + 7) / 8 * 8; }
 
-// How a product of M x N x K runs.
+// How a product of M x N x K runs.  Three tile shapes; the estimate below (in
+// SM clocks) picks the one that ends first.
+//   pair 256 x 256: 64 KB of operands a K step for both CTAs, 512 clocks of MMA;
+//   128 x 128: 32 KB for 256 clocks of MMA, held to about 560 by the operand
+//     feed from L2 (measured: 1.01 PFLOP/s over 16384 x 8192 x 8192);
+//   128 x 64: 24 KB, about 400.
 struct Plan {
-    int bn, splits, ksteps, ksteps_split, tiles_m, tiles_n;
+    int bn, pair, splits, ksteps, ksteps_split, tiles_m, tiles_n;
     int64_t partial_bytes;
 };
 static Plan make_plan(int64_t M, int64_t N, int64_t K) {
-    Plan pl;
+    struct Shape {
+        int bn, pair;
+        double kstep, epilogue;  // clocks a K step; clocks of a tile's epilogue
+    };
+    static const Shape shapes[3] = {{256, 1, 540., 5000.}, {128, 0, 560., 2500.}, {64, 0, 400., 1300.}};
     const int sms = fcai::sm_count();
-    pl.bn = N <= 64 ? 64 : 128;
-    pl.tiles_m = (int)((M + kBM - 1) / kBM);
-    pl.tiles_n = (int)((N + pl.bn - 1) / pl.bn);
-    pl.ksteps = (int)((K + kBK - 1) / kBK);
-    const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n;
-    int splits = tiles >= sms ? 1 : (int)(sms / tiles);
-    splits = std::max(1, std::min(splits, pl.ksteps / 4));
-    pl.ksteps_split = (pl.ksteps + splits - 1) / splits;
-    pl.splits = (pl.ksteps + pl.ksteps_split - 1) / pl.ksteps_split;  // none is empty
-    pl.partial_bytes = pl.splits > 1 ? round256((int64_t)pl.splits * M * round8((int)N) * 4) : 0;
-    return pl;
+    Plan best{};
+    double best_time = 0.;
+    for (const Shape &sh : shapes) {
+        if (sh.bn > 64 && N <= sh.bn / 2) continue;
+        Plan pl{};
+        pl.bn = sh.bn;
+        pl.pair = sh.pair;
+        const int tile_m = sh.pair ? 256 : 128;
+        pl.tiles_m = (int)((M + tile_m - 1) / tile_m);
+        pl.tiles_n = (int)((N + pl.bn - 1) / pl.bn);
+        pl.ksteps = (int)((K + kBK - 1) / kBK);
+        const int64_t tiles = (int64_t)pl.tiles_m * pl.tiles_n;
+        const int64_t slots = sh.pair ? sms / 2 : sms;
+        int splits = tiles >= slots ? 1 : (int)(slots / tiles);
+        splits = std::max(1, std::min(splits, pl.ksteps / 4));
+        pl.ksteps_split = (pl.ksteps + splits - 1) / splits;
+        pl.splits = (pl.ksteps + pl.ksteps_split - 1) / pl.ksteps_split;  // none is empty
+        pl.partial_bytes = pl.splits > 1 ? round256((int64_t)pl.splits * M * round8((int)N) * 4) : 0;
+        const int64_t waves = (tiles * pl.splits + slots - 1) / slots;
+        // a tile's epilogue runs under the next tile's K steps
+        double time = waves * std::max(pl.ksteps_split * sh.kstep, sh.epilogue) + sh.epilogue;
+        if (pl.splits > 1) time += 5000. + 2. * pl.partial_bytes / 4000.;  // the second launch and the partial tiles
+        if (best.bn == 0 || time < best_time) {
+            best = pl;
+            best_time = time;
+        }
+    }
+    return best;
 }
 
 struct Operand {
@@ -487,19 +584,42 @@ static int prepare_operand(Operand &o, int dtype, unsigned char *&ws, cudaStream
     return FCAI_OK;
 }
 
-template <typename T, int kBN, bool kTA, bool kTB>
+template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
 static int launch(const CUtensorMap &a, const CUtensorMap &b, const Params &p, cudaStream_t stream) {
-    using Lay = Layout<kBN>;
-    auto kernel = linear_tc_kernel<T, kBN, kTA, kTB>;
-    static int configured[64] = {0};
+    using Lay = Layout<kBN, kPair>;
+    auto kernel = linear_tc_kernel<T, kBN, kPair, kTA, kTB>;
+    static int slots[64] = {0};  // CTAs (pairs) resident at once
     int dev = 0;
     FCAI_CUDA_TRY(cudaGetDevice(&dev));
     if (dev < 0 || dev >= 64) return fcai::fail(FCAI_ERR_CUDA, "device ordinal %d unsupported", dev);
-    if (!configured[dev]) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = 2;
+    attr.val.clusterDim.y = 1;
+    attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.dynamicSmemBytes = Lay::kAlloc;
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (!slots[dev]) {
         FCAI_CUDA_TRY(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Lay::kAlloc));
-        configured[dev] = 1;
+        int n = fcai::sm_count();
+        if (kPair) {
+            cfg.gridDim = dim3(2, 1, 1);
+            FCAI_CUDA_TRY(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+            if (n < 1) return fcai::fail(FCAI_ERR_CUDA, "no CTA pair of this product fits on the device");
+        }
+        slots[dev] = n;
     }
-    kernel<<<std::min(p.units, fcai::sm_count()), kThreads, Lay::kAlloc, stream>>>(a, b, p);
+    const int n = std::min(p.units, slots[dev]);
+    if (kPair) {
+        cfg.gridDim = dim3(2 * n, 1, 1);
+        FCAI_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, b, p));
+    } else {
+        kernel<<<n, kThreads, Lay::kAlloc, stream>>>(a, b, p);
+    }
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
@@ -530,8 +650,11 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     if ((rc = prepare_operand(B, dtype, ws, stream))) return rc;
     CUtensorMap ma, mb;
     if ((rc = make_map(&ma, A.ptr, A.cols, A.rows, A.ld, kTA ? kBK : kBM, dtype))) return rc;
-    if ((rc = make_map(&mb, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.bn, dtype))) return rc;
-    rc = pl.bn == 64 ? launch<T, 64, kTA, kTB>(ma, mb, p, stream) : launch<T, 128, kTA, kTB>(ma, mb, p, stream);
+    if ((rc = make_map(&mb, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.pair ? pl.bn / 2 : pl.bn, dtype)))
+        return rc;
+    rc = pl.pair        ? launch<T, 256, true, kTA, kTB>(ma, mb, p, stream)
+         : pl.bn == 128 ? launch<T, 128, false, kTA, kTB>(ma, mb, p, stream)
+                        : launch<T, 64, false, kTA, kTB>(ma, mb, p, stream);
     if (rc) return rc;
     if (pl.splits > 1) {
         reduce_kernel<T><<<elementwise_grid(M * (p.ldp / 8), 256), 256, 0, stream>>>(p);

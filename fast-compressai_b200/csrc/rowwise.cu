@@ -76,6 +76,44 @@ __device__ __forceinline__ void store_codes(uint8_t *row, const Cols<kV> &c, int
     }
 }
 
+// Eight elements as they lie in memory, 4 or 8 registers: what is in flight or waits for a sum.
+template <typename T, bool kV>
+struct Raw8 {
+    uint32_t w[sizeof(T) * 2];
+    __device__ __forceinline__ void load(const T *row, const Cols<kV> &c, int n, bool in) {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) * 2; ++i) w[i] = 0u;
+        if constexpr (kV) {
+            if (in && c.first < n) {
+#pragma unroll
+                for (int i = 0; i < (int)sizeof(T) / 2; ++i) {
+                    const uint4 q = __ldg(reinterpret_cast<const uint4 *>(row + c.first) + i);
+                    w[4 * i] = q.x, w[4 * i + 1] = q.y, w[4 * i + 2] = q.z, w[4 * i + 3] = q.w;
+                }
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (!in || c[i] >= n) continue;
+                if constexpr (sizeof(T) == 4) w[i] = __float_as_uint(__ldg(row + c[i]));
+                else w[i / 2] |= (uint32_t)__ldg(reinterpret_cast<const unsigned short *>(row) + c[i]) << (16 * (i & 1));
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 f = unpack2(w[i], T());
+                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+            }
+        }
+    }
+};
+
 // What a backward pass reads x from.
 struct Kept {
     const void *x;
@@ -96,7 +134,7 @@ __device__ __forceinline__ void decode8(int keep, uint2 q, float s, float (&v)[8
 // A kept value's bits as they are loaded, before they are decoded: loads of several rows go out together.
 template <typename T, bool kV, bool k8>
 struct KeptRaw {
-    float v[k8 ? 1 : 8];
+    Raw8<T, kV> x;
     uint2 q;
     float s;
     __device__ __forceinline__ void load(const Kept &k, int64_t row, const Cols<kV> &c, int n, int nblk, bool in) {
@@ -104,15 +142,14 @@ struct KeptRaw {
             q = load_codes(k.codes + row * n, c, n, in);
             s = in && c.first < n ? __ldg(k.scales + row * nblk + c.first / kBlock) : 0.f;
         } else {
-            load8(static_cast<const T *>(k.x) + row * k.ldx, c, n, in, v);
+            x.load(static_cast<const T *>(k.x) + row * k.ldx, c, n, in);
         }
     }
     __device__ __forceinline__ void get(const Kept &k, float (&o)[8]) const {
         if constexpr (k8) {
             decode8(k.keep, q, s, o);
         } else {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) o[i] = v[i];
+            x.get(o);
         }
     }
 };
@@ -142,67 +179,35 @@ __device__ __forceinline__ void keep_block(int keep, const float (&v)[8], uint8_
     if (in && c.first % kBlock == 0 && c.first < n) *scale = s;
 }
 
-__device__ __forceinline__ void act8(int kind, float (&y)[8]) {
-    switch (kind) {
-        case FCAI_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_RELU>(y[i]);
-            break;
-        case FCAI_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_GELU>(y[i]);
-            break;
-        case FCAI_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = act<FCAI_ACT_SILU>(y[i]);
-            break;
-        default: break;
-    }
-}
-__device__ __forceinline__ void act_grad8(int kind, const float (&x)[8], float (&g)[8]) {
-    switch (kind) {
-        case FCAI_ACT_RELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] *= act_grad<FCAI_ACT_RELU>(x[i]);
-            break;
-        case FCAI_ACT_GELU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] *= act_grad<FCAI_ACT_GELU>(x[i]);
-            break;
-        case FCAI_ACT_SILU:
-#pragma unroll
-            for (int i = 0; i < 8; ++i) g[i] *= act_grad<FCAI_ACT_SILU>(x[i]);
-            break;
-        default: break;
-    }
-}
-
 // ---- strips: activations, checkpoint load ------------------------------------
-// grid (row shares, strips): with the shares in x the launch has no limit of 65535 there.
+// grid (strips, row shares): the CTAs that run at the same time cover whole rows, which DRAM pages like.
 template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads)
     act_forward_kernel(const T *__restrict__ x, int64_t ldx, T *__restrict__ y, int64_t ldy, uint8_t *__restrict__ codes,
                        float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep) {
-    const int strip = blockIdx.y;
+    const int strip = blockIdx.x;
     const Cols<kV> c(strip * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.x * kRowsIter;
+    const int64_t step = (int64_t)gridDim.y * kRowsIter;
     const int sub = (threadIdx.x >> 4) & 1;
     // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
-    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 5) * 2; r0 < rows; r0 += step * kUnroll) {
-        float v[kUnroll][8];
+    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 5) * 2; r0 < rows; r0 += step * kUnroll) {
+        Raw8<T, kV> raw[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = r0 + u * step + sub;
-            load8(x + row * ldx, c, n, row < rows, v[u]);
+            raw[u].load(x + row * ldx, c, n, row < rows);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = r0 + u * step + sub;
             const bool in = row < rows;
-            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, v[u], codes + row * n, scales + row * nblk + strip, c, n, in);
+            if (r0 + u * step >= rows) break;
+            float v[8];
+            raw[u].get(v);
+            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, v, codes + row * n, scales + row * nblk + strip, c, n, in);
             if (y) {
-                act8(act, v[u]);
-                store8(y + row * ldy, c, n, in, v[u]);
+                act_n(act, v);
+                store8(y + row * ldy, c, n, in, v);
             }
         }
     }
@@ -211,14 +216,15 @@ __global__ void __launch_bounds__(kThreads)
 template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads)
     checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
-    const Cols<kV> c(blockIdx.y * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.x * kRowsIter;
-    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
+    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
+    const int64_t step = (int64_t)gridDim.y * kRowsIter;
+    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
         KeptRaw<T, kV, true> raw[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) raw[u].load(k, r0 + u * step, c, n, nblk, r0 + u * step < rows);
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
+            if (r0 + u * step >= rows) break;
             float v[8];
             raw[u].get(k, v);
             store8(out + (r0 + u * step) * ldo, c, n, r0 + u * step < rows, v);
@@ -252,34 +258,35 @@ __global__ void __launch_bounds__(kThreads)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
                         float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
     __shared__ float sh[kThreads * 8];
-    const Cols<kV> c(blockIdx.y * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.x * kRowsIter;
+    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
+    const int64_t step = (int64_t)gridDim.y * kRowsIter;
     float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    for (int64_t r0 = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
-        float g[kUnroll][8];
+    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
+        Raw8<T, kV> raw_g[kUnroll];
         KeptRaw<T, kV, k8> raw[kUnroll];
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = r0 + u * step;
-            load8(dy + row * lddy, c, n, row < rows, g[u]);
+            raw_g[u].load(dy + row * lddy, c, n, row < rows);
             if (act != FCAI_ACT_NONE) raw[u].load(k, row, c, n, nblk, row < rows);
         }
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = r0 + u * step;
+            if (row >= rows) break;
+            float g[8];
+            raw_g[u].get(g);
             if (act != FCAI_ACT_NONE) {
                 float x[8];
                 raw[u].get(k, x);
-                act_grad8(act, x, g[u]);
+                act_grad_n(act, x, g);
             }
-            if (dx) store8(dx + row * lddx, c, n, row < rows, g[u]);
-            if (row < rows) {
+            if (dx) store8(dx + row * lddx, c, n, true, g);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) acc[i] += g[u][i];
-            }
+            for (int i = 0; i < 8; ++i) acc[i] += g[i];
         }
     }
-    if (partial) group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.x * n, blockIdx.y * kBlock, n, sh);
+    if (partial) group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, sh);
 }
 
 // Column sums of partial[rows][stride], in a fixed order: columns [0, n0) to
@@ -321,22 +328,27 @@ struct Group {
     static constexpr int kGroups = kCta / kLanes;
     static constexpr int kWarpsRow = kLanes <= 32 ? 1 : kLanes / 32;
 };
-template <int kLanes>
-__device__ __forceinline__ float2 group_sum2(float a, float b, float2 (*sh)[16], int &turn) {
+// Sums of kN values over the group, exchanged together.
+template <int kLanes, int kN>
+__device__ __forceinline__ void group_sum(float (&v)[kN], float (*sh)[16][kN], int &turn) {
 #pragma unroll
-    for (int d = (kLanes < 32 ? kLanes : 32) / 2; d >= 1; d >>= 1) {
-        a += __shfl_xor_sync(0xffffffffu, a, d);
-        b += __shfl_xor_sync(0xffffffffu, b, d);
-    }
+    for (int d = (kLanes < 32 ? kLanes : 32) / 2; d >= 1; d >>= 1)
+#pragma unroll
+        for (int i = 0; i < kN; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
     if constexpr (kLanes > 32) {
-        if ((threadIdx.x & 31) == 0) sh[turn][threadIdx.x >> 5] = make_float2(a, b);
-        __syncthreads();
-        a = b = 0.f;
+        if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-        for (int w = 0; w < kLanes / 32; ++w) a += sh[turn][w].x, b += sh[turn][w].y;
+            for (int i = 0; i < kN; ++i) sh[turn][threadIdx.x >> 5][i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kN; ++i) {
+            v[i] = 0.f;
+#pragma unroll
+            for (int w = 0; w < kLanes / 32; ++w) v[i] += sh[turn][w][i];
+        }
         turn ^= 1;
     }
-    return make_float2(a, b);
 }
 template <int kLanes, bool kV>
 __device__ __forceinline__ Cols<kV> chunk_cols(int chunk) {
@@ -364,135 +376,189 @@ __device__ __forceinline__ void load_affine(const Affine &a, const void *p, cons
     }
 }
 
-// kRows rows a group and step.
-template <typename T, bool kV, int kLanes, int kChunks, int kRows>
-__global__ void __launch_bounds__(Group<kLanes>::kCta)
+// kRows rows a group and step, their sums exchanged together; whole-CTA groups
+// fetch the next step's rows before they sum this one's.
+template <typename T, bool kV, bool k8, int kLanes, int kChunks, int kRows>
+__global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunks == 1 ? 1024 / kLanes : 1)
     norm_forward_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
                         float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
                         float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
     using G = Group<kLanes>;
-    __shared__ float2 sh[2][16];
+    __shared__ float sh[2][16][kRows];
     int turn = 0;
     const float inv_n = 1.f / n;
     const int64_t step = (int64_t)gridDim.x * G::kGroups * kRows;
+    const int sub = threadIdx.x / kLanes;
     // the loop runs on the CTA's first row: shuffles and barriers need everyone
-    for (int64_t r0 = (int64_t)blockIdx.x * G::kGroups * kRows; r0 < rows; r0 += step) {
-        float v[kRows][kChunks][8];
+    int64_t r0 = (int64_t)blockIdx.x * G::kGroups * kRows;
+    Raw8<T, kV> next[kRows][kChunks];
+    auto fetch = [&](int64_t first) {
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            const int64_t row = r0 + u * G::kGroups + threadIdx.x / kLanes;
+            const int64_t row = first + u * G::kGroups + sub;
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j) load8(x + row * ldx, chunk_cols<kLanes, kV>(j), n, row < rows, v[u][j]);
+            for (int j = 0; j < kChunks; ++j) next[u][j].load(x + row * ldx, chunk_cols<kLanes, kV>(j), n, row < rows);
         }
+    };
+    fetch(r0);
+    float w[kChunks][8], b[kChunks][8];
+#pragma unroll
+    for (int j = 0; j < kChunks; ++j) {
+        load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
+        load_affine<T>(af, af.b, chunk_cols<kLanes, kV>(j), n, 0.f, b[j]);
+    }
+    for (; r0 < rows; r0 += step) {
+        Raw8<T, kV> raw[kRows][kChunks];
+#pragma unroll
+        for (int u = 0; u < kRows; ++u)
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) raw[u][j] = next[u][j];
+        if (r0 + step < rows) fetch(r0 + step);
+        float mean[kRows], rstd[kRows], v[8];
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            const int64_t row = r0 + u * G::kGroups + threadIdx.x / kLanes;
-            const bool in = row < rows;
-            float s = 0.f;
+            mean[u] = 0.f;
 #pragma unroll
-            for (int j = 0; j < kChunks; ++j)
+            for (int j = 0; j < kChunks; ++j) {
+                raw[u][j].get(v);
+                mean[u] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+            }
+        }
+        group_sum<kLanes>(mean, sh, turn);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) s += v[u][j][i];
-            const float mean = group_sum2<kLanes>(s, 0.f, sh, turn).x * inv_n;
-            s = 0.f;
+        for (int u = 0; u < kRows; ++u) {
+            mean[u] *= inv_n;
+            rstd[u] = 0.f;
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+                raw[u][j].get(v);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const float d = (kV ? c.first : c[i]) < n ? v[u][j][i] - mean : 0.f;
-                    s = fmaf(d, d, s);
+                    const float d = (kV ? c.first : c[i]) < n ? v[i] - mean[u] : 0.f;
+                    rstd[u] = fmaf(d, d, rstd[u]);
                 }
             }
-            const float rstd = 1.f / sqrtf(fmaf(group_sum2<kLanes>(s, 0.f, sh, turn).x, inv_n, eps));
+        }
+        group_sum<kLanes>(rstd, sh, turn);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t row = r0 + u * G::kGroups + sub;
+            const bool in = row < rows;
+            const float rs = 1.f / sqrtf(fmaf(rstd[u], inv_n, eps));
             if (mean_out && in && threadIdx.x % kLanes == 0) {
-                mean_out[row] = mean;
-                rstd_out[row] = rstd;
+                mean_out[row] = mean[u];
+                rstd_out[row] = rs;
             }
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 const Cols<kV> c = chunk_cols<kLanes, kV>(j);
-                if (keep >= FCAI_KEEP_INT8)
-                    keep_block<kLanes>(keep, v[u][j], codes + row * n, scales + row * nblk + c.first / kBlock, c, n, in);
-                float w[8], b[8];
-                load_affine<T>(af, af.w, c, n, 1.f, w);
-                load_affine<T>(af, af.b, c, n, 0.f, b);
+                raw[u][j].get(v);
+                if (k8)
+                    keep_block<kLanes>(keep, v, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, in);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[u][j][i] = fmaf((v[u][j][i] - mean) * rstd, w[i], b[i]);
-                store8(y + row * ldy, c, n, in, v[u][j]);
+                for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - mean[u]) * rs, w[j][i], b[j][i]);
+                store8(y + row * ldy, c, n, in, v);
             }
         }
     }
 }
 
 // dx, and the CTA's sums of dy xhat and dy over its rows in partial[CTA][2][n].
-// Each thread keeps its channels' sums in registers from row to row; the next
-// row's loads go out before this row's sums are exchanged.
-template <typename T, bool kV, bool k8, int kLanes, int kChunks>
-__global__ void __launch_bounds__(Group<kLanes>::kCta)
+// Each thread keeps its channels' sums in registers from row to row.  Rows wait
+// for their sums as they came from memory (4 registers per 8 16-bit values) and
+// are converted again after it: registers, which set how many rows are in
+// flight, are dearer here than instructions.
+template <typename T, bool kV, bool k8, int kLanes, int kChunks, int kRows>
+__global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 2 : kLanes * kChunks <= 512 ? 1024 / kLanes : 1)
     norm_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
                          const float *__restrict__ rstd, Affine af, T *__restrict__ dx, int64_t lddx,
                          float *__restrict__ partial, int64_t rows, int n, int nblk) {
     using G = Group<kLanes>;
-    __shared__ float2 sh[2][16];
+    constexpr bool kHoldWeight = kChunks <= 2;
+    __shared__ float sh[2][16][2 * kRows];
     __shared__ float sums[G::kGroups > 1 ? kThreads * 8 : 1];
     int turn = 0;
     const float inv_n = 1.f / n;
-    float aw[kChunks][8], ab[kChunks][8];
+    float aw[kChunks][8], ab[kChunks][8], w[kChunks][8];
 #pragma unroll
-    for (int j = 0; j < kChunks; ++j)
+    for (int j = 0; j < kChunks; ++j) {
+        if (kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
 #pragma unroll
         for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
-    const int64_t step = (int64_t)gridDim.x * G::kGroups;
+    }
+    const int64_t step = (int64_t)gridDim.x * G::kGroups * kRows;
     const int sub = threadIdx.x / kLanes;
-    int64_t r0 = (int64_t)blockIdx.x * G::kGroups;
-    float g[kChunks][8];
-    KeptRaw<T, kV, k8> raw[kChunks];
-    float mu = 0.f, rs = 0.f;
-    auto fetch = [&](int64_t row) {
-        const bool in = row < rows;
-        mu = in ? __ldg(mean + row) : 0.f;
-        rs = in ? __ldg(rstd + row) : 0.f;
+    int64_t r0 = (int64_t)blockIdx.x * G::kGroups * kRows;
+    Raw8<T, kV> next_g[kRows][kChunks];
+    KeptRaw<T, kV, k8> next_x[kRows][kChunks];
+    float next_mu[kRows], next_rs[kRows];
+    auto fetch = [&](int64_t first) {
 #pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            const Cols<kV> c = chunk_cols<kLanes, kV>(j);
-            load8(dy + row * lddy, c, n, in, g[j]);
-            raw[j].load(k, row, c, n, nblk, in);
-        }
-    };
-    fetch(r0 + sub);
-    for (; r0 < rows; r0 += step) {
-        const int64_t row = r0 + sub;
-        const bool in = row < rows;
-        const float rs0 = rs;
-        float t[kChunks][8], xh[kChunks][8];
-        float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-        for (int j = 0; j < kChunks; ++j) {
-            const Cols<kV> c = chunk_cols<kLanes, kV>(j);
-            float w[8];
-            load_affine<T>(af, af.w, c, n, 1.f, w);
-            raw[j].get(k, xh[j]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                // past the row's end dy is zero; xhat there is kept out of the sums by that
-                xh[j][i] = (xh[j][i] - mu) * rs0;
-                t[j][i] = g[j][i] * w[i];
-                s1 += t[j][i];
-                s2 = fmaf(t[j][i], xh[j][i], s2);
-                aw[j][i] = fmaf(g[j][i], xh[j][i], aw[j][i]);
-                ab[j][i] += g[j][i];
-            }
-        }
-        if (r0 + step < rows) fetch(row + step);
-        const float2 m = group_sum2<kLanes>(s1, s2, sh, turn);
-        if (dx) {
-            const float m1 = m.x * inv_n, m2 = m.y * inv_n;
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t row = first + u * G::kGroups + sub;
+            const bool in = row < rows;
+            next_mu[u] = in ? __ldg(mean + row) : 0.f;
+            next_rs[u] = in ? __ldg(rstd + row) : 0.f;
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
+                const Cols<kV> c = chunk_cols<kLanes, kV>(j);
+                next_g[u][j].load(dy + row * lddy, c, n, in);
+                next_x[u][j].load(k, row, c, n, nblk, in);
+            }
+        }
+    };
+    fetch(r0);
+    for (; r0 < rows; r0 += step) {
+        Raw8<T, kV> raw_g[kRows][kChunks];
+        KeptRaw<T, kV, k8> raw_x[kRows][kChunks];
+        float mu[kRows], rs[kRows], s[2 * kRows];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) t[j][i] = rs0 * (t[j][i] - m1 - xh[j][i] * m2);
-                store8(dx + row * lddx, chunk_cols<kLanes, kV>(j), n, in, t[j]);
+        for (int u = 0; u < kRows; ++u) {
+            mu[u] = next_mu[u], rs[u] = next_rs[u];
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) raw_g[u][j] = next_g[u][j], raw_x[u][j] = next_x[u][j];
+        }
+        if (r0 + step < rows) fetch(r0 + step);
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            s[2 * u] = s[2 * u + 1] = 0.f;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                float g[8], xh[8];
+                raw_g[u][j].get(g);
+                raw_x[u][j].get(k, xh);
+                if (!kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    // past the row's end dy is zero, which keeps xhat there out of every sum
+                    xh[i] = (xh[i] - mu[u]) * rs[u];
+                    const float t = g[i] * w[j][i];
+                    s[2 * u] += t;
+                    s[2 * u + 1] = fmaf(t, xh[i], s[2 * u + 1]);
+                    aw[j][i] = fmaf(g[i], xh[i], aw[j][i]);
+                    ab[j][i] += g[i];
+                }
+            }
+        }
+        group_sum<kLanes>(s, sh, turn);
+        if (!dx) continue;
+#pragma unroll
+        for (int u = 0; u < kRows; ++u) {
+            const int64_t row = r0 + u * G::kGroups + sub;
+            const float m1 = s[2 * u] * inv_n, m2 = s[2 * u + 1] * inv_n;
+#pragma unroll
+            for (int j = 0; j < kChunks; ++j) {
+                float g[8], xh[8];
+                raw_g[u][j].get(g);
+                raw_x[u][j].get(k, xh);
+                if (!kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float h = (xh[i] - mu[u]) * rs[u];
+                    g[i] = rs[u] * (g[i] * w[j][i] - m1 - h * m2);
+                }
+                store8(dx + row * lddx, chunk_cols<kLanes, kV>(j), n, row < rows, g);
             }
         }
     }
@@ -517,7 +583,7 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta)
 
 // Rows of more than kMaxHeld channels: a CTA per row that reads it again (from
 // cache) for each step.
-constexpr int kMaxHeld = 16384;
+constexpr int kMaxHeld = 8192;
 template <bool kV>
 __device__ __forceinline__ Cols<kV> wide_cols(int c0) {  // c0: a multiple of the CTA's 2048 channels
     return Cols<kV>(c0 + (threadIdx.x / 16) * kBlock, threadIdx.x & 15, 16);
@@ -527,28 +593,30 @@ __global__ void __launch_bounds__(kThreads)
     norm_forward_wide_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
                              float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
                              float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
-    __shared__ float2 sh[2][16];
+    __shared__ float sh[2][16][1];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const T *xr = x + row * ldx;
-        float s = 0.f, v[8];
+        float s[1] = {0.f}, v[8];
         for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
             load8(xr, wide_cols<kV>(c0), n, true, v);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) s += v[i];
+            for (int i = 0; i < 8; ++i) s[0] += v[i];
         }
-        const float mean = group_sum2<kThreads>(s, 0.f, sh, turn).x / n;
-        s = 0.f;
+        group_sum<kThreads>(s, sh, turn);
+        const float mean = s[0] / n;
+        s[0] = 0.f;
         for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
             const Cols<kV> c = wide_cols<kV>(c0);
             load8(xr, c, n, true, v);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float d = c[i] < n ? v[i] - mean : 0.f;
-                s = fmaf(d, d, s);
+                s[0] = fmaf(d, d, s[0]);
             }
         }
-        const float rstd = 1.f / sqrtf(group_sum2<kThreads>(s, 0.f, sh, turn).x / n + eps);
+        group_sum<kThreads>(s, sh, turn);
+        const float rstd = 1.f / sqrtf(s[0] / n + eps);
         if (threadIdx.x == 0 && mean_out) {
             mean_out[row] = mean;
             rstd_out[row] = rstd;
@@ -574,11 +642,11 @@ __global__ void __launch_bounds__(kThreads)
     norm_backward_stats_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
                                const float *__restrict__ rstd, Affine af, float2 *__restrict__ stats, int64_t rows, int n,
                                int nblk) {
-    __shared__ float2 sh[2][16];
+    __shared__ float sh[2][16][2];
     int turn = 0;
     for (int64_t row = blockIdx.x; row < rows; row += gridDim.x) {
         const float mu = mean[row], rs = rstd[row];
-        float s1 = 0.f, s2 = 0.f;
+        float s[2] = {0.f, 0.f};
         for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
             const Cols<kV> c = wide_cols<kV>(c0);
             float g[8], x[8], w[8];
@@ -590,12 +658,12 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float t = g[i] * w[i];  // zero past the row's end: g is
-                s1 += t;
-                s2 = fmaf(t, (x[i] - mu) * rs, s2);
+                s[0] += t;
+                s[1] = fmaf(t, (x[i] - mu) * rs, s[1]);
             }
         }
-        const float2 s = group_sum2<kThreads>(s1, s2, sh, turn);
-        if (threadIdx.x == 0) stats[row] = make_float2(s.x / n, s.y / n);
+        group_sum<kThreads>(s, sh, turn);
+        if (threadIdx.x == 0) stats[row] = make_float2(s[0] / n, s[1] / n);
     }
 }
 
@@ -605,11 +673,11 @@ __global__ void __launch_bounds__(kThreads)
                                const float *__restrict__ rstd, Affine af, const float2 *__restrict__ stats,
                                T *__restrict__ dx, int64_t lddx, float *__restrict__ partial, int64_t rows, int n, int nblk) {
     __shared__ float sh[kThreads * 8];
-    const int base = blockIdx.y * kBlock;
+    const int base = blockIdx.x * kBlock;
     const Cols<kV> c(base, threadIdx.x & 15, 16);
     float w[8], aw[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ab[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
     load_affine<T>(af, af.w, c, n, 1.f, w);
-    for (int64_t row = (int64_t)blockIdx.x * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.x * kRowsIter) {
+    for (int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.y * kRowsIter) {
         const float mu = mean[row], rs = rstd[row];
         const float2 m = stats[row];
         float g[8], x[8];
@@ -627,7 +695,7 @@ __global__ void __launch_bounds__(kThreads)
         if (dx) store8(dx + row * lddx, c, n, true, x);
     }
     if (partial) {
-        float *pr = partial + (int64_t)blockIdx.x * 2 * n;
+        float *pr = partial + (int64_t)blockIdx.y * 2 * n;
         group_sums<16, kThreads, kV>(aw, pr, base, n, sh);
         group_sums<16, kThreads, kV>(ab, pr + n, base, n, sh);
     }
@@ -647,8 +715,8 @@ static bool codes_vec(const void *codes, int n) { return !codes || ((reinterpret
 static int row_shares(int64_t rows, int strips, bool sums) {
     const int64_t steps = (rows + kRowsIter - 1) / kRowsIter;
     const int64_t fill = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 8 + strips - 1) / strips);
-    if (sums || steps <= fill) return (int)std::min(steps, fill);
-    return (int)std::max(fill, (steps + kUnroll - 1) / kUnroll);
+    if (sums || steps <= fill) return (int)std::min<int64_t>({steps, fill, 65535});
+    return (int)std::min<int64_t>(std::max(fill, (steps + kUnroll - 1) / kUnroll), 65535);
 }
 // How the layer norm runs rows of n channels: threads a row, 8-channel chunks a thread.
 struct Held {
@@ -662,13 +730,14 @@ static Held held(int n) {
     if (n <= 1024) return {128, 1};
     if (n <= 2048) return {256, 1};
     if (n <= 4096) return {512, 1};
-    if (n <= 8192) return {512, 2};
-    return {512, 4};
+    return {512, 2};
 }
+// Rows a group has in flight in the backward kernel.
+constexpr int backward_rows(int lanes, int chunks) { return lanes <= 32 ? 2 / chunks : 1; }
 static int norm_backward_grid(int64_t rows, int n) {
     const Held h = held(n);
-    const int groups = h.lanes <= 32 ? kThreads / h.lanes : 1;
-    const int per_sm = h.lanes <= 32 ? 4 : 1024 / h.lanes / h.chunks > 0 ? 1024 / h.lanes / h.chunks : 1;
+    const int groups = (h.lanes <= 32 ? kThreads / h.lanes : 1) * backward_rows(h.lanes, h.chunks);
+    const int per_sm = h.lanes <= 32 ? 3 : std::max(1, 1024 / h.lanes / h.chunks);
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
 }
 static int64_t act_workspace(int64_t rows, int n) {
@@ -727,7 +796,7 @@ static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *c
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
     const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
     const int strips = blocks_of(n);
-    const dim3 grid(row_shares(rows, strips, false), strips);
+    const dim3 grid(strips, row_shares(rows, strips, false));
     auto kernel = vec ? act_forward_kernel<T, true> : act_forward_kernel<T, false>;
     kernel<<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales,
                                       rows, n, strips, act, q ? keep : FCAI_KEEP_NONE);
@@ -743,7 +812,7 @@ static int act_backward(const void *dy, int64_t lddy, const Kept &k, void *dx, i
                      (act == FCAI_ACT_NONE || (k8 ? codes_vec(k.codes, n) : aligned16(k.x, k.ldx, dtype)));
     auto kernel = k8 ? (vec ? act_backward_kernel<T, true, true> : act_backward_kernel<T, false, true>)
                      : (vec ? act_backward_kernel<T, true, false> : act_backward_kernel<T, false, false>);
-    kernel<<<dim3(shares, strips), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
+    kernel<<<dim3(strips, shares), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
                                                       bias_grad ? ws : nullptr, rows, n, strips, act);
     FCAI_CUDA_TRY(cudaGetLastError());
     return bias_grad ? colsum(ws, shares, n, bias_grad, n, nullptr, 0, dtype, st) : FCAI_OK;
@@ -753,7 +822,7 @@ static int load_checkpoint(const Kept &k, void *out, int64_t ldo, int64_t rows, 
     const bool vec = n % 8 == 0 && aligned16(out, ldo, dtype) && codes_vec(k.codes, n);
     const int strips = blocks_of(n);
     auto kernel = vec ? checkpoint_load_kernel<T, true> : checkpoint_load_kernel<T, false>;
-    kernel<<<dim3(row_shares(rows, strips, false), strips), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
+    kernel<<<dim3(strips, row_shares(rows, strips, false)), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
@@ -767,14 +836,13 @@ struct NormForward {
     Affine af;
     cudaStream_t st;
 };
-template <typename T, bool kV, int kLanes, int kChunks>
+template <typename T, bool kV, bool k8, int kLanes, int kChunks>
 static int launch_norm_forward(const NormForward &a) {
-    // rows in flight: 4 x 8 values a thread, as far as one row leaves room
-    constexpr int kRows = kLanes > 32 ? 1 : 4 / kChunks;
+    constexpr int kRows = kLanes > 32 ? (kChunks == 1 ? 2 : 1) : 2 / kChunks;
     constexpr int64_t kPerCta = (int64_t)Group<kLanes>::kGroups * kRows;
     const int64_t want = (a.rows + kPerCta - 1) / kPerCta;
-    const int grid = (int)std::min<int64_t>(want, kLanes > 32 ? (int64_t)fcai::sm_count() * (2048 / kLanes) : 0x7FFFFFFF);
-    norm_forward_kernel<T, kV, kLanes, kChunks, kRows><<<grid, Group<kLanes>::kCta, 0, a.st>>>(
+    const int grid = (int)std::min<int64_t>(want, (int64_t)fcai::sm_count() * (kLanes > 32 ? std::max(1, 1024 / kLanes) : 6));
+    norm_forward_kernel<T, kV, k8, kLanes, kChunks, kRows><<<grid, Group<kLanes>::kCta, 0, a.st>>>(
         static_cast<const T *>(a.x), a.ldx, a.af, static_cast<T *>(a.y), a.ldy, a.mean, a.rstd, static_cast<uint8_t *>(a.codes),
         a.scales, a.rows, a.n, blocks_of(a.n), a.eps, a.keep);
     FCAI_CUDA_TRY(cudaGetLastError());
@@ -793,7 +861,7 @@ struct NormBackward {
 };
 template <typename T, bool kV, bool k8, int kLanes, int kChunks>
 static int launch_norm_backward(const NormBackward &a) {
-    norm_backward_kernel<T, kV, k8, kLanes, kChunks><<<norm_backward_grid(a.rows, a.n), Group<kLanes>::kCta, 0, a.st>>>(
+    norm_backward_kernel<T, kV, k8, kLanes, kChunks, backward_rows(kLanes, kChunks)><<<norm_backward_grid(a.rows, a.n), Group<kLanes>::kCta, 0, a.st>>>(
         static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, static_cast<T *>(a.dx), a.lddx, a.partial, a.rows, a.n,
         blocks_of(a.n));
     FCAI_CUDA_TRY(cudaGetLastError());
@@ -808,13 +876,12 @@ static int launch_norm_backward(const NormBackward &a) {
         case 128 * 8 + 1: return call(128, 1);                       \
         case 256 * 8 + 1: return call(256, 1);                       \
         case 512 * 8 + 1: return call(512, 1);                       \
-        case 512 * 8 + 2: return call(512, 2);                       \
-        default: return call(512, 4);                                \
+        default: return call(512, 2);                                \
     }
-template <typename T, bool kV>
+template <typename T, bool kV, bool k8>
 static int norm_forward_held(const NormForward &a) {
     const Held h = held(a.n);
-#define CALL(lanes, chunks) launch_norm_forward<T, kV, lanes, chunks>(a)
+#define CALL(lanes, chunks) launch_norm_forward<T, kV, k8, lanes, chunks>(a)
     RW_BY_HELD(CALL)
 #undef CALL
 }
@@ -834,7 +901,8 @@ static int norm_forward(const void *x, int64_t ldx, Affine af, int wdtype, void 
     af.vec = n % 8 == 0 && affine_vec(af.w, wdtype) && affine_vec(af.b, wdtype);
     if (n <= kMaxHeld) {
         const NormForward a{x, af.w, af.b, ldx, ldy, rows, y, codes, mean, rstd, scales, eps, n, keep, af, st};
-        return vec ? norm_forward_held<T, true>(a) : norm_forward_held<T, false>(a);
+        if (q) return vec ? norm_forward_held<T, true, true>(a) : norm_forward_held<T, false, true>(a);
+        return vec ? norm_forward_held<T, true, false>(a) : norm_forward_held<T, false, false>(a);
     }
     auto kernel = vec ? norm_forward_wide_kernel<T, true> : norm_forward_wide_kernel<T, false>;
     kernel<<<(int)std::min<int64_t>(rows, (int64_t)fcai::sm_count() * 8), kThreads, 0, st>>>(
@@ -850,7 +918,7 @@ static int norm_backward_any(const NormBackward &a, float2 *stats, int shares) {
     norm_backward_stats_kernel<T, kV, k8><<<(int)std::min<int64_t>(a.rows, (int64_t)fcai::sm_count() * 8), kThreads, 0, a.st>>>(
         static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, stats, a.rows, a.n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
-    norm_backward_strip_kernel<T, kV, k8><<<dim3(shares, strips), kThreads, 0, a.st>>>(
+    norm_backward_strip_kernel<T, kV, k8><<<dim3(strips, shares), kThreads, 0, a.st>>>(
         static_cast<const T *>(a.dy), a.lddy, a.k, a.mean, a.rstd, a.af, stats, static_cast<T *>(a.dx), a.lddx, a.partial, a.rows,
         a.n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
