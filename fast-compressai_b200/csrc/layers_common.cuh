@@ -38,34 +38,6 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
     return __half22float2(*reinterpret_cast<__half2 *>(&w));
 }
 
-// Eight consecutive elements from / to a 16-byte aligned address (f32: two
-// 16-byte accesses).
-template <typename T> struct Vec8 {
-    static __device__ __forceinline__ void load(const T *p, float (&v)[8]) {
-        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
-        unpack(q, v);
-    }
-    static __device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8]) {
-        const float2 a = unpack2(q.x, T()), b = unpack2(q.y, T()), c = unpack2(q.z, T()), d = unpack2(q.w, T());
-        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
-    }
-    static __device__ __forceinline__ void store(T *p, const float (&v)[8]) {
-        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
-                                                   pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
-    }
-};
-template <> struct Vec8<float> {
-    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
-        const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
-        const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-    static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
-        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
-        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
-    }
-};
-
 // ---- activations --------------------------------------------------------------
 __device__ __forceinline__ float ex2_approx(float x) {
     float y;
@@ -111,6 +83,54 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
     return v;
 }
 
+// Eight consecutive elements from / to a 16-byte aligned address (f32: two
+// 16-byte accesses).
+template <typename T> struct Vec8 {
+    static __device__ __forceinline__ void load(const T *p, float (&v)[8]) {
+        const uint4 q = __ldg(reinterpret_cast<const uint4 *>(p));
+        unpack(q, v);
+    }
+    static __device__ __forceinline__ void unpack(const uint4 &q, float (&v)[8]) {
+        const float2 a = unpack2(q.x, T()), b = unpack2(q.y, T()), c = unpack2(q.z, T()), d = unpack2(q.w, T());
+        v[0] = a.x, v[1] = a.y, v[2] = b.x, v[3] = b.y, v[4] = c.x, v[5] = c.y, v[6] = d.x, v[7] = d.y;
+    }
+    static __device__ __forceinline__ void store(T *p, const float (&v)[8]) {
+        *reinterpret_cast<uint4 *>(p) = make_uint4(pack2(v[0], v[1], T()), pack2(v[2], v[3], T()),
+                                                   pack2(v[4], v[5], T()), pack2(v[6], v[7], T()));
+    }
+};
+template <> struct Vec8<float> {
+    static __device__ __forceinline__ void load(const float *p, float (&v)[8]) {
+        const float4 a = __ldg(reinterpret_cast<const float4 *>(p));
+        const float4 b = __ldg(reinterpret_cast<const float4 *>(p) + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+    static __device__ __forceinline__ void store(float *p, const float (&v)[8]) {
+        reinterpret_cast<float4 *>(p)[0] = make_float4(v[0], v[1], v[2], v[3]);
+        reinterpret_cast<float4 *>(p)[1] = make_float4(v[4], v[5], v[6], v[7]);
+    }
+};
+
+// Eight values as pairs.
+struct V8 {
+    F2 p[4];
+    __device__ __forceinline__ void set(const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) p[i] = f2(v[2 * i], v[2 * i + 1]);
+    }
+    __device__ __forceinline__ void get(float (&v)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = split(p[i]);
+            v[2 * i] = f.x, v[2 * i + 1] = f.y;
+        }
+    }
+};
+__device__ __forceinline__ float hsum(F2 v) {
+    const float2 f = split(v);
+    return f.x + f.y;
+}
+
 // The normal distribution's upper tail Q(t) = erfc(t / sqrt 2) / 2, t >= 0, as
 // e * R(u) with e = exp(-t^2 / 2), u = 1 / (1 + 0.24 t) and R a polynomial
 // without constant term, the form of Hastings' approximations (Approximations
@@ -145,60 +165,54 @@ __device__ __forceinline__ F2 sigmoid2(F2 x) {
     return f2(rcp_approx(d.x), rcp_approx(d.y));
 }
 
-// v = act(v) of kN values (a multiple of 2); `kind` is the same for the whole kernel.
+// v = act(v) of kN pairs; `kind` is the same for the whole kernel.
 template <int kN>
-__device__ __forceinline__ void act_n(int kind, float (&v)[kN]) {
+__device__ __forceinline__ void act_n(int kind, F2 (&v)[kN]) {
     if (kind == FCAI_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = v[i] < 0.f ? 0.f : v[i];  // a NaN stays
+        for (int i = 0; i < kN; ++i) {
+            const float2 x = split(v[i]);
+            v[i] = f2(x.x < 0.f ? 0.f : x.x, x.y < 0.f ? 0.f : x.y);  // a NaN stays
+        }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 2) {
+        for (int i = 0; i < kN; ++i) {
             F2 e;
-            const float2 x = make_float2(v[i], v[i + 1]);
-            const float2 y = split(mul2(f2(x.x, x.y), normal_cdf2(x, e)));
-            v[i] = y.x, v[i + 1] = y.y;
+            v[i] = mul2(v[i], normal_cdf2(split(v[i]), e));
         }
     } else if (kind == FCAI_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 2) {
-            const F2 x = f2(v[i], v[i + 1]);
-            const float2 y = split(mul2(x, sigmoid2(x)));
-            v[i] = y.x, v[i + 1] = y.y;
-        }
+        for (int i = 0; i < kN; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));
     }
 }
 // g *= act'(x)
 template <int kN>
-__device__ __forceinline__ void act_grad_n(int kind, const float (&x)[kN], float (&g)[kN]) {
+__device__ __forceinline__ void act_grad_n(int kind, const F2 (&x)[kN], F2 (&g)[kN]) {
     if (kind == FCAI_ACT_RELU) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) g[i] *= x[i] > 0.f ? 1.f : 0.f;
+        for (int i = 0; i < kN; ++i) {
+            const float2 xx = split(x[i]);
+            g[i] = mul2(g[i], f2(xx.x > 0.f ? 1.f : 0.f, xx.y > 0.f ? 1.f : 0.f));
+        }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 2) {
+        for (int i = 0; i < kN; ++i) {
             F2 e;
-            const float2 xx = make_float2(x[i], x[i + 1]);
-            const F2 cdf = normal_cdf2(xx, e);
-            const F2 d = fma2(mul2(f2(xx.x, xx.y), e), f2(0.398942280f), cdf);  // Phi(x) + x phi(x)
-            const float2 y = split(mul2(f2(g[i], g[i + 1]), d));
-            g[i] = y.x, g[i + 1] = y.y;
+            const F2 cdf = normal_cdf2(split(x[i]), e);
+            g[i] = mul2(g[i], fma2(mul2(x[i], e), f2(0.398942280f), cdf));  // Phi(x) + x phi(x)
         }
     } else if (kind == FCAI_ACT_SILU) {
 #pragma unroll
-        for (int i = 0; i < kN; i += 2) {
-            const F2 xx = f2(x[i], x[i + 1]);
-            const F2 s = sigmoid2(xx);
-            const F2 d = mul2(s, fma2(xx, fma2(s, f2(-1.f), f2(1.f)), f2(1.f)));
-            const float2 y = split(mul2(f2(g[i], g[i + 1]), d));
-            g[i] = y.x, g[i + 1] = y.y;
+        for (int i = 0; i < kN; ++i) {
+            const F2 s = sigmoid2(x[i]);
+            g[i] = mul2(g[i], mul2(s, fma2(x[i], fma2(s, f2(-1.f), f2(1.f)), f2(1.f))));
         }
     }
 }
 __device__ __forceinline__ float act_1(int kind, float x) {
-    float v[2] = {x, 0.f};
+    F2 v[1] = {f2(x, 0.f)};
     act_n(kind, v);
-    return v[0];
+    return split(v[0]).x;
 }
 
 // ---- 8-bit blocks ---------------------------------------------------------------
@@ -216,35 +230,49 @@ __device__ __forceinline__ float max_nan(float a, float b) {
     asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(b));
     return y;
 }
+// Codes of four values times inv.  The products are rounded before they become
+// codes, as the definition says.  int8 without conversion instructions, which run at an
+// eighth of the rate: adding 1.5 * 2^23 leaves the integer, ties to even, in
+// the low bits; |x * inv| <= 127 (1 + 2^-22), so no code leaves its range, and
+// a NaN block's codes, whatever they are, read back as NaN.
 template <bool kE4m3>
-__device__ __forceinline__ uint32_t encode4(const float *v, float inv) {
+__device__ __forceinline__ uint32_t encode4(F2 a, F2 b, float inv) {
     if (kE4m3) {
-        const __nv_fp8x2_storage_t a = __nv_cvt_float2_to_fp8x2(make_float2(v[0] * inv, v[1] * inv), __NV_SATFINITE, __NV_E4M3);
-        const __nv_fp8x2_storage_t b = __nv_cvt_float2_to_fp8x2(make_float2(v[2] * inv, v[3] * inv), __NV_SATFINITE, __NV_E4M3);
-        return (uint32_t)a | ((uint32_t)b << 16);
+        a = mul2(a, f2(inv));
+        b = mul2(b, f2(inv));
+        const __nv_fp8x2_storage_t lo = __nv_cvt_float2_to_fp8x2(split(a), __NV_SATFINITE, __NV_E4M3);
+        const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(split(b), __NV_SATFINITE, __NV_E4M3);
+        return (uint32_t)lo | ((uint32_t)hi << 16);
     }
-    uint32_t w = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int q = max(-127, min(127, __float2int_rn(v[i] * inv)));  // a NaN converts to 0
-        w |= (uint32_t)(q & 0xFF) << (8 * i);
-    }
-    return w;
+    // one at a time: a packed product and sum can come out as one fused operation, which rounds once
+    auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); };
+    const float2 x = split(a), y = split(b);
+    const uint32_t lo = __byte_perm(code(x.x), code(x.y), 0x0040);
+    const uint32_t hi = __byte_perm(code(y.x), code(y.y), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
 }
 template <bool kE4m3>
-__device__ __forceinline__ void decode4(uint32_t w, float scale, float *v) {
+__device__ __forceinline__ uint2 encode8(const V8 &v, float inv) {
+    return make_uint2(encode4<kE4m3>(v.p[0], v.p[1], inv), encode4<kE4m3>(v.p[2], v.p[3], inv));
+}
+// Four codes times scale.  int8: the byte with its sign flipped becomes the low
+// bits of 2^23, and 2^23 + 128 is taken off again.
+template <bool kE4m3>
+__device__ __forceinline__ void decode4(uint32_t w, float scale, F2 &a, F2 &b) {
     if (kE4m3) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const __half2_raw r = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> (16 * h)), __NV_E4M3);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2 *>(&r));
-            v[2 * h] = f.x * scale;
-            v[2 * h + 1] = f.y * scale;
-        }
+        const __half2_raw lo = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w & 0xFFFFu), __NV_E4M3);
+        const __half2_raw hi = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(w >> 16), __NV_E4M3);
+        const float2 x = __half22float2(*reinterpret_cast<const __half2 *>(&lo));
+        const float2 y = __half22float2(*reinterpret_cast<const __half2 *>(&hi));
+        a = f2(x.x, x.y), b = f2(y.x, y.y);
     } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) v[i] = (float)(int8_t)(w >> (8 * i)) * scale;
+        w ^= 0x80808080u;
+        auto at = [&](uint32_t sel) { return __uint_as_float(__byte_perm(w, 0x4B000000u, sel)); };
+        a = add2(f2(at(0x7440), at(0x7441)), f2(-8388736.f));
+        b = add2(f2(at(0x7442), at(0x7443)), f2(-8388736.f));
     }
+    a = mul2(a, f2(scale));
+    b = mul2(b, f2(scale));
 }
 
 inline int dtype_size(int dtype) { return dtype == FCAI_DTYPE_F32 ? 4 : 2; }

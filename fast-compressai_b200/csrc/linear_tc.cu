@@ -127,7 +127,17 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int row_ste
             if (row + i * row_step < p.M)
                 res[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + (row + i * row_step) * p.ldr + col));
     }
-    act_n(p.act, v);
+    if (p.act != FCAI_ACT_NONE) {
+        F2 w[kR * 4];
+#pragma unroll
+        for (int i = 0; i < kR * 4; ++i) w[i] = f2(v[2 * i], v[2 * i + 1]);
+        act_n(p.act, w);
+#pragma unroll
+        for (int i = 0; i < kR * 4; ++i) {
+            const float2 o = split(w[i]);
+            v[2 * i] = o.x, v[2 * i + 1] = o.y;
+        }
+    }
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
         if (row + i * row_step >= p.M) continue;

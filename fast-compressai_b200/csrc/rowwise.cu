@@ -21,7 +21,7 @@ using namespace ly;
 constexpr int kThreads = 256;
 constexpr int kBlock = FCAI_KEEP_BLOCK;
 constexpr int kRowsIter = kThreads / 16;  // rows a strip CTA handles at a time
-constexpr int kUnroll = 4;                // rows a strip thread has in flight
+constexpr int kUnroll = 2;                // rows a strip thread has in flight
 
 // The eight channels a thread holds of its group's 8 * g: consecutive ones where
 // rows take 16-byte accesses (kV), else every g-th, so that neighbouring lanes
@@ -53,6 +53,12 @@ __device__ __forceinline__ void store8(T *row, const Cols<kV> &c, int n, bool in
             if (in && c[i] < n) row[c[i]] = from_f32<T>(v[i]);
     }
 }
+template <typename T, bool kV>
+__device__ __forceinline__ void store8(T *row, const Cols<kV> &c, int n, bool in, const V8 &v) {
+    float f[8];
+    v.get(f);
+    store8(row, c, n, in, f);
+}
 template <bool kV>
 __device__ __forceinline__ uint2 load_codes(const uint8_t *row, const Cols<kV> &c, int n, bool in) {
     uint2 q = make_uint2(0u, 0u);
@@ -76,6 +82,9 @@ __device__ __forceinline__ void store_codes(uint8_t *row, const Cols<kV> &c, int
     }
 }
 
+template <typename T> struct Pair;
+template <> struct Pair<__half> { using type = __half2; };
+template <> struct Pair<__nv_bfloat16> { using type = __nv_bfloat162; };
 // Eight elements as they lie in memory, 4 or 8 registers: what is in flight or waits for a sum.
 template <typename T, bool kV>
 struct Raw8 {
@@ -100,16 +109,34 @@ struct Raw8 {
             }
         }
     }
-    __device__ __forceinline__ void get(float (&v)[8]) const {
+    __device__ __forceinline__ V8 get() const {
+        V8 v;
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(w[i]);
+            for (int i = 0; i < 4; ++i) v.p[i] = f2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float2 f = unpack2(w[i], T());
-                v[2 * i] = f.x, v[2 * i + 1] = f.y;
+                v.p[i] = f2(f.x, f.y);
             }
+        }
+        return v;
+    }
+    // largest magnitude; NaN if there is one
+    __device__ __forceinline__ float amax() const {
+        if constexpr (sizeof(T) == 4) {
+            float m = fabsf(__uint_as_float(w[0]));
+#pragma unroll
+            for (int i = 1; i < 8; ++i) m = max_nan(m, fabsf(__uint_as_float(w[i])));
+            return m;
+        } else {
+            using T2 = typename Pair<T>::type;
+            T2 m = __habs2(*reinterpret_cast<const T2 *>(&w[0]));
+#pragma unroll
+            for (int i = 1; i < 4; ++i) m = __hmax2_nan(m, __habs2(*reinterpret_cast<const T2 *>(&w[i])));
+            const float2 f = unpack2(*reinterpret_cast<uint32_t *>(&m), T());
+            return max_nan(f.x, f.y);
         }
     }
 };
@@ -122,14 +149,16 @@ struct Kept {
     const float *scales;
     int keep;
 };
-__device__ __forceinline__ void decode8(int keep, uint2 q, float s, float (&v)[8]) {
+__device__ __forceinline__ V8 decode8(int keep, uint2 q, float s) {
+    V8 v;
     if (keep == FCAI_KEEP_E4M3) {
-        decode4<true>(q.x, s, v);
-        decode4<true>(q.y, s, v + 4);
+        decode4<true>(q.x, s, v.p[0], v.p[1]);
+        decode4<true>(q.y, s, v.p[2], v.p[3]);
     } else {
-        decode4<false>(q.x, s, v);
-        decode4<false>(q.y, s, v + 4);
+        decode4<false>(q.x, s, v.p[0], v.p[1]);
+        decode4<false>(q.y, s, v.p[2], v.p[3]);
     }
+    return v;
 }
 // A kept value's bits as they are loaded, before they are decoded: loads of several rows go out together.
 template <typename T, bool kV, bool k8>
@@ -145,35 +174,27 @@ struct KeptRaw {
             x.load(static_cast<const T *>(k.x) + row * k.ldx, c, n, in);
         }
     }
-    __device__ __forceinline__ void get(const Kept &k, float (&o)[8]) const {
-        if constexpr (k8) {
-            decode8(k.keep, q, s, o);
-        } else {
-            x.get(o);
-        }
+    __device__ __forceinline__ V8 get(const Kept &k) const {
+        if constexpr (k8) return decode8(k.keep, q, s);
+        else return x.get();
     }
 };
 
 // A block's codes and scale, from the kLanes (at most 16) lanes that hold its
-// channels, 8 each; the whole warp calls it.
+// channels, 8 each (amax: the lane's own); the whole warp calls it.
 template <int kLanes, bool kV>
-__device__ __forceinline__ void keep_block(int keep, const float (&v)[8], uint8_t *codes_row, float *scale, const Cols<kV> &c,
+__device__ __forceinline__ void keep_block(int keep, float amax, const V8 &v, uint8_t *codes_row, float *scale, const Cols<kV> &c,
                                            int n, bool in) {
-    float amax = fabsf(v[0]);
-#pragma unroll
-    for (int i = 1; i < 8; ++i) amax = max_nan(amax, fabsf(v[i]));
 #pragma unroll
     for (int d = (kLanes < 16 ? kLanes : 16) / 2; d >= 1; d >>= 1) amax = max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, d));
     uint2 q;
     float s;
     if (keep == FCAI_KEEP_E4M3) {
         s = block_scale<true>(amax);
-        const float inv = __frcp_rn(s);
-        q = make_uint2(encode4<true>(v, inv), encode4<true>(v + 4, inv));
+        q = encode8<true>(v, __frcp_rn(s));
     } else {
         s = block_scale<false>(amax);
-        const float inv = __frcp_rn(s);
-        q = make_uint2(encode4<false>(v, inv), encode4<false>(v + 4, inv));
+        q = encode8<false>(v, __frcp_rn(s));
     }
     store_codes(codes_row, c, n, in, q);
     if (in && c.first % kBlock == 0 && c.first < n) *scale = s;
@@ -182,7 +203,7 @@ __device__ __forceinline__ void keep_block(int keep, const float (&v)[8], uint8_
 // ---- strips: activations, checkpoint load ------------------------------------
 // grid (strips, row shares): the CTAs that run at the same time cover whole rows, which DRAM pages like.
 template <typename T, bool kV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
     act_forward_kernel(const T *__restrict__ x, int64_t ldx, T *__restrict__ y, int64_t ldy, uint8_t *__restrict__ codes,
                        float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep) {
     const int strip = blockIdx.x;
@@ -202,11 +223,10 @@ __global__ void __launch_bounds__(kThreads)
             const int64_t row = r0 + u * step + sub;
             const bool in = row < rows;
             if (r0 + u * step >= rows) break;
-            float v[8];
-            raw[u].get(v);
-            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, v, codes + row * n, scales + row * nblk + strip, c, n, in);
+            V8 v = raw[u].get();
+            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, raw[u].amax(), v, codes + row * n, scales + row * nblk + strip, c, n, in);
             if (y) {
-                act_n(act, v);
+                act_n(act, v.p);
                 store8(y + row * ldy, c, n, in, v);
             }
         }
@@ -214,7 +234,7 @@ __global__ void __launch_bounds__(kThreads)
 }
 
 template <typename T, bool kV>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, kV ? 6 : 4)
     checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
     const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.y * kRowsIter;
@@ -225,9 +245,7 @@ __global__ void __launch_bounds__(kThreads)
 #pragma unroll
         for (int u = 0; u < kUnroll; ++u) {
             if (r0 + u * step >= rows) break;
-            float v[8];
-            raw[u].get(k, v);
-            store8(out + (r0 + u * step) * ldo, c, n, r0 + u * step < rows, v);
+            store8(out + (r0 + u * step) * ldo, c, n, true, raw[u].get(k));
         }
     }
 }
@@ -235,11 +253,13 @@ __global__ void __launch_bounds__(kThreads)
 // Adds the sums of a CTA's groups of kLanes threads (8 * kLanes channels from
 // base on) and writes them to a partial row.
 template <int kLanes, int kCta, bool kV>
-__device__ __forceinline__ void group_sums(const float (&acc)[8], float *partial_row, int base, int n, float *sh) {
+__device__ __forceinline__ void group_sums(const V8 &sums, float *partial_row, int base, int n, float *sh) {
     constexpr int kSpan = kLanes * 8;
     const int g = threadIdx.x / kLanes, l = threadIdx.x % kLanes;
     const Cols<kV> c(0, l % 16 + (kV ? l / 16 * 16 : 0), kLanes < 16 ? kLanes : 16);
     const int blk = kV ? 0 : l / 16 * kBlock;
+    float acc[8];
+    sums.get(acc);
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) sh[g * kSpan + blk + c[i]] = acc[i];
@@ -254,13 +274,13 @@ __device__ __forceinline__ void group_sums(const float (&acc)[8], float *partial
 
 // dx = dy act'(x) and partial sums of it over the CTA's rows
 template <typename T, bool kV, bool k8>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
                         float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
     __shared__ float sh[kThreads * 8];
     const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.y * kRowsIter;
-    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+    V8 acc = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
     for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
         Raw8<T, kV> raw_g[kUnroll];
         KeptRaw<T, kV, k8> raw[kUnroll];
@@ -274,16 +294,14 @@ __global__ void __launch_bounds__(kThreads)
         for (int u = 0; u < kUnroll; ++u) {
             const int64_t row = r0 + u * step;
             if (row >= rows) break;
-            float g[8];
-            raw_g[u].get(g);
+            V8 g = raw_g[u].get();
             if (act != FCAI_ACT_NONE) {
-                float x[8];
-                raw[u].get(k, x);
-                act_grad_n(act, x, g);
+                const V8 x = raw[u].get(k);
+                act_grad_n(act, x.p, g.p);
             }
             if (dx) store8(dx + row * lddx, c, n, true, g);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] += g[i];
+            for (int i = 0; i < 4; ++i) acc.p[i] = add2(acc.p[i], g.p[i]);
         }
     }
     if (partial) group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, sh);
@@ -328,6 +346,13 @@ struct Group {
     static constexpr int kGroups = kCta / kLanes;
     static constexpr int kWarpsRow = kLanes <= 32 ? 1 : kLanes / 32;
 };
+// CTAs an SM is to hold of the norm kernels: 64 registers a thread for 16-bit
+// rows, 128 for f32 ones and two chunks.
+constexpr int norm_ctas(int lanes, int chunks, bool f32, int warp_groups) {
+    if (lanes <= 32) return f32 && chunks == 2 ? 1 : f32 ? 2 : warp_groups;
+    const int threads = f32 || chunks > 1 ? 512 : 1024;
+    return threads > lanes ? threads / lanes : 1;
+}
 // Sums of kN values over the group, exchanged together.
 template <int kLanes, int kN>
 __device__ __forceinline__ void group_sum(float (&v)[kN], float (*sh)[16][kN], int &turn) {
@@ -341,12 +366,13 @@ __device__ __forceinline__ void group_sum(float (&v)[kN], float (*sh)[16][kN], i
             for (int i = 0; i < kN; ++i) sh[turn][threadIdx.x >> 5][i] = v[i];
         }
         __syncthreads();
+        // every warp adds the warps' sums, a lane each
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            v[i] = 0.f;
+        for (int i = 0; i < kN; ++i) v[i] = sh[turn][threadIdx.x & (kLanes / 32 - 1)][i];
 #pragma unroll
-            for (int w = 0; w < kLanes / 32; ++w) v[i] += sh[turn][w][i];
-        }
+        for (int d = kLanes / 64; d >= 1; d >>= 1)
+#pragma unroll
+            for (int i = 0; i < kN; ++i) v[i] += __shfl_xor_sync(0xffffffffu, v[i], d);
         turn ^= 1;
     }
 }
@@ -362,7 +388,8 @@ struct Affine {
     int f32, vec;
 };
 template <typename T, bool kV>
-__device__ __forceinline__ void load_affine(const Affine &a, const void *p, const Cols<kV> &c, int n, float dflt, float (&v)[8]) {
+__device__ __forceinline__ V8 load_affine(const Affine &a, const void *p, const Cols<kV> &c, int n, float dflt) {
+    float v[8];
     if (!p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = dflt;
@@ -374,12 +401,15 @@ __device__ __forceinline__ void load_affine(const Affine &a, const void *p, cons
         for (int i = 0; i < 8; ++i)
             v[i] = c[i] >= n ? 0.f : a.f32 ? static_cast<const float *>(p)[c[i]] : to_f32(static_cast<const T *>(p)[c[i]]);
     }
+    V8 o;
+    o.set(v);
+    return o;
 }
 
 // kRows rows a group and step, their sums exchanged together; whole-CTA groups
 // fetch the next step's rows before they sum this one's.
 template <typename T, bool kV, bool k8, int kLanes, int kChunks, int kRows>
-__global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunks == 1 ? 1024 / kLanes : 1)
+__global__ void __launch_bounds__(Group<kLanes>::kCta, norm_ctas(kLanes, kChunks, sizeof(T) == 4, k8 || kChunks == 2 ? 2 : 3))
     norm_forward_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
                         float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
                         float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
@@ -401,11 +431,11 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunk
         }
     };
     fetch(r0);
-    float w[kChunks][8], b[kChunks][8];
+    V8 w[kChunks], b[kChunks];
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-        load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
-        load_affine<T>(af, af.b, chunk_cols<kLanes, kV>(j), n, 0.f, b[j]);
+        w[j] = load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f);
+        b[j] = load_affine<T>(af, af.b, chunk_cols<kLanes, kV>(j), n, 0.f);
     }
     for (; r0 < rows; r0 += step) {
         Raw8<T, kV> raw[kRows][kChunks];
@@ -414,31 +444,39 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunk
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) raw[u][j] = next[u][j];
         if (r0 + step < rows) fetch(r0 + step);
-        float mean[kRows], rstd[kRows], v[8];
+        float mean[kRows], rstd[kRows];
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            mean[u] = 0.f;
+            F2 s = f2(0.f);
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
-                raw[u][j].get(v);
-                mean[u] += ((v[0] + v[1]) + (v[2] + v[3])) + ((v[4] + v[5]) + (v[6] + v[7]));
+                const V8 v = raw[u][j].get();
+                s = add2(s, add2(add2(v.p[0], v.p[1]), add2(v.p[2], v.p[3])));
             }
+            mean[u] = hsum(s);
         }
         group_sum<kLanes>(mean, sh, turn);
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
             mean[u] *= inv_n;
-            rstd[u] = 0.f;
+            F2 s = f2(0.f);
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 const Cols<kV> c = chunk_cols<kLanes, kV>(j);
-                raw[u][j].get(v);
+                const V8 v = raw[u][j].get();
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float d = (kV ? c.first : c[i]) < n ? v[i] - mean[u] : 0.f;
-                    rstd[u] = fmaf(d, d, rstd[u]);
+                for (int i = 0; i < 4; ++i) {
+                    F2 d = add2(v.p[i], f2(-mean[u]));
+                    if (kV) {
+                        if (c.first >= n) d = f2(0.f);
+                    } else {
+                        const float2 e = split(d);
+                        d = f2(c[2 * i] < n ? e.x : 0.f, c[2 * i + 1] < n ? e.y : 0.f);
+                    }
+                    s = fma2(d, d, s);
                 }
             }
+            rstd[u] = hsum(s);
         }
         group_sum<kLanes>(rstd, sh, turn);
 #pragma unroll
@@ -453,11 +491,11 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunk
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
                 const Cols<kV> c = chunk_cols<kLanes, kV>(j);
-                raw[u][j].get(v);
+                V8 v = raw[u][j].get();
                 if (k8)
-                    keep_block<kLanes>(keep, v, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, in);
+                    keep_block<kLanes>(keep, raw[u][j].amax(), v, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, in);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - mean[u]) * rs, w[j][i], b[j][i]);
+                for (int i = 0; i < 4; ++i) v.p[i] = fma2(mul2(add2(v.p[i], f2(-mean[u])), f2(rs)), w[j].p[i], b[j].p[i]);
                 store8(y + row * ldy, c, n, in, v);
             }
         }
@@ -470,22 +508,20 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 3 : kChunk
 // are converted again after it: registers, which set how many rows are in
 // flight, are dearer here than instructions.
 template <typename T, bool kV, bool k8, int kLanes, int kChunks, int kRows>
-__global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 2 : kLanes * kChunks <= 512 ? 1024 / kLanes : 1)
+__global__ void __launch_bounds__(Group<kLanes>::kCta, norm_ctas(kLanes, kChunks, sizeof(T) == 4, 2))
     norm_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, const float *__restrict__ mean,
                          const float *__restrict__ rstd, Affine af, T *__restrict__ dx, int64_t lddx,
                          float *__restrict__ partial, int64_t rows, int n, int nblk) {
     using G = Group<kLanes>;
-    constexpr bool kHoldWeight = kChunks <= 2;
     __shared__ float sh[2][16][2 * kRows];
     __shared__ float sums[G::kGroups > 1 ? kThreads * 8 : 1];
     int turn = 0;
     const float inv_n = 1.f / n;
-    float aw[kChunks][8], ab[kChunks][8], w[kChunks][8];
+    V8 aw[kChunks], ab[kChunks], w[kChunks];
 #pragma unroll
     for (int j = 0; j < kChunks; ++j) {
-        if (kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) aw[j][i] = ab[j][i] = 0.f;
+        w[j] = load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f);
+        aw[j] = ab[j] = V8{f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
     }
     const int64_t step = (int64_t)gridDim.x * G::kGroups * kRows;
     const int sub = threadIdx.x / kLanes;
@@ -522,24 +558,23 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 2 : kLanes
         if (r0 + step < rows) fetch(r0 + step);
 #pragma unroll
         for (int u = 0; u < kRows; ++u) {
-            s[2 * u] = s[2 * u + 1] = 0.f;
+            F2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
-                float g[8], xh[8];
-                raw_g[u][j].get(g);
-                raw_x[u][j].get(k, xh);
-                if (!kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
+                const V8 g = raw_g[u][j].get(), x = raw_x[u][j].get(k);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
+                for (int i = 0; i < 4; ++i) {
                     // past the row's end dy is zero, which keeps xhat there out of every sum
-                    xh[i] = (xh[i] - mu[u]) * rs[u];
-                    const float t = g[i] * w[j][i];
-                    s[2 * u] += t;
-                    s[2 * u + 1] = fmaf(t, xh[i], s[2 * u + 1]);
-                    aw[j][i] = fmaf(g[i], xh[i], aw[j][i]);
-                    ab[j][i] += g[i];
+                    const F2 xh = mul2(add2(x.p[i], f2(-mu[u])), f2(rs[u]));
+                    const F2 t = mul2(g.p[i], w[j].p[i]);
+                    s1 = add2(s1, t);
+                    s2 = fma2(t, xh, s2);
+                    aw[j].p[i] = fma2(g.p[i], xh, aw[j].p[i]);
+                    ab[j].p[i] = add2(ab[j].p[i], g.p[i]);
                 }
             }
+            s[2 * u] = hsum(s1);
+            s[2 * u + 1] = hsum(s2);
         }
         group_sum<kLanes>(s, sh, turn);
         if (!dx) continue;
@@ -549,14 +584,12 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 2 : kLanes
             const float m1 = s[2 * u] * inv_n, m2 = s[2 * u + 1] * inv_n;
 #pragma unroll
             for (int j = 0; j < kChunks; ++j) {
-                float g[8], xh[8];
-                raw_g[u][j].get(g);
-                raw_x[u][j].get(k, xh);
-                if (!kHoldWeight) load_affine<T>(af, af.w, chunk_cols<kLanes, kV>(j), n, 1.f, w[j]);
+                V8 g = raw_g[u][j].get();
+                const V8 x = raw_x[u][j].get(k);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float h = (xh[i] - mu[u]) * rs[u];
-                    g[i] = rs[u] * (g[i] * w[j][i] - m1 - h * m2);
+                for (int i = 0; i < 4; ++i) {
+                    const F2 xh = mul2(add2(x.p[i], f2(-mu[u])), f2(rs[u]));
+                    g.p[i] = mul2(f2(rs[u]), fma2(xh, f2(-m2), fma2(g.p[i], w[j].p[i], f2(-m1))));
                 }
                 store8(dx + row * lddx, chunk_cols<kLanes, kV>(j), n, row < rows, g);
             }
@@ -571,11 +604,14 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, kLanes <= 32 ? 2 : kLanes
             group_sums<kLanes, kThreads, kV>(aw[j], pr, j * kLanes * 8, n, sums);
             group_sums<kLanes, kThreads, kV>(ab[j], pr + n, j * kLanes * 8, n, sums);
         } else {
+            float vw[8], vb[8];
+            aw[j].get(vw);
+            ab[j].get(vb);
 #pragma unroll
             for (int i = 0; i < 8; ++i)
                 if (c[i] < n) {
-                    pr[c[i]] = aw[j][i];
-                    pr[n + c[i]] = ab[j][i];
+                    pr[c[i]] = vw[i];
+                    pr[n + c[i]] = vb[i];
                 }
         }
     }
@@ -623,15 +659,15 @@ __global__ void __launch_bounds__(kThreads)
         }
         for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
             const Cols<kV> c = wide_cols<kV>(c0);
-            load8(xr, c, n, true, v);
+            Raw8<T, kV> raw;
+            raw.load(xr, c, n, true);
+            V8 o = raw.get();
             if (keep >= FCAI_KEEP_INT8)
-                keep_block<16>(keep, v, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, true);
-            float w[8], b[8];
-            load_affine<T>(af, af.w, c, n, 1.f, w);
-            load_affine<T>(af, af.b, c, n, 0.f, b);
+                keep_block<16>(keep, raw.amax(), o, codes + row * n, scales + row * nblk + c.first / kBlock, c, n, true);
+            const V8 w = load_affine<T>(af, af.w, c, n, 1.f), b = load_affine<T>(af, af.b, c, n, 0.f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = fmaf((v[i] - mean) * rstd, w[i], b[i]);
-            store8(y + row * ldy, c, n, true, v);
+            for (int i = 0; i < 4; ++i) o.p[i] = fma2(mul2(add2(o.p[i], f2(-mean)), f2(rstd)), w.p[i], b.p[i]);
+            store8(y + row * ldy, c, n, true, o);
         }
     }
 }
@@ -649,18 +685,20 @@ __global__ void __launch_bounds__(kThreads)
         float s[2] = {0.f, 0.f};
         for (int c0 = 0; c0 < n; c0 += kThreads * 8) {
             const Cols<kV> c = wide_cols<kV>(c0);
-            float g[8], x[8], w[8];
-            KeptRaw<T, kV, k8> raw;
-            load8(dy + row * lddy, c, n, true, g);
-            raw.load(k, row, c, n, nblk, true);
-            raw.get(k, x);
-            load_affine<T>(af, af.w, c, n, 1.f, w);
+            Raw8<T, kV> raw_g;
+            KeptRaw<T, kV, k8> raw_x;
+            raw_g.load(dy + row * lddy, c, n, true);
+            raw_x.load(k, row, c, n, nblk, true);
+            const V8 g = raw_g.get(), x = raw_x.get(k), w = load_affine<T>(af, af.w, c, n, 1.f);
+            F2 s1 = f2(0.f), s2 = f2(0.f);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float t = g[i] * w[i];  // zero past the row's end: g is
-                s[0] += t;
-                s[1] = fmaf(t, (x[i] - mu) * rs, s[1]);
+            for (int i = 0; i < 4; ++i) {
+                const F2 t = mul2(g.p[i], w.p[i]);  // zero past the row's end: g is
+                s1 = add2(s1, t);
+                s2 = fma2(t, mul2(add2(x.p[i], f2(-mu)), f2(rs)), s2);
             }
+            s[0] += hsum(s1);
+            s[1] += hsum(s2);
         }
         group_sum<kThreads>(s, sh, turn);
         if (threadIdx.x == 0) stats[row] = make_float2(s[0] / n, s[1] / n);
@@ -675,22 +713,23 @@ __global__ void __launch_bounds__(kThreads)
     __shared__ float sh[kThreads * 8];
     const int base = blockIdx.x * kBlock;
     const Cols<kV> c(base, threadIdx.x & 15, 16);
-    float w[8], aw[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f}, ab[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    load_affine<T>(af, af.w, c, n, 1.f, w);
+    V8 aw = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)}, ab = aw;
+    const V8 w = load_affine<T>(af, af.w, c, n, 1.f);
     for (int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); row < rows; row += (int64_t)gridDim.y * kRowsIter) {
         const float mu = mean[row], rs = rstd[row];
         const float2 m = stats[row];
-        float g[8], x[8];
-        KeptRaw<T, kV, k8> raw;
-        load8(dy + row * lddy, c, n, true, g);
-        raw.load(k, row, c, n, nblk, true);
-        raw.get(k, x);
+        Raw8<T, kV> raw_g;
+        KeptRaw<T, kV, k8> raw_x;
+        raw_g.load(dy + row * lddy, c, n, true);
+        raw_x.load(k, row, c, n, nblk, true);
+        const V8 g = raw_g.get();
+        V8 x = raw_x.get(k);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float xh = (x[i] - mu) * rs;
-            aw[i] = fmaf(g[i], xh, aw[i]);
-            ab[i] += g[i];
-            x[i] = rs * (g[i] * w[i] - m.x - xh * m.y);
+        for (int i = 0; i < 4; ++i) {
+            const F2 xh = mul2(add2(x.p[i], f2(-mu)), f2(rs));
+            aw.p[i] = fma2(g.p[i], xh, aw.p[i]);
+            ab.p[i] = add2(ab.p[i], g.p[i]);
+            x.p[i] = mul2(f2(rs), fma2(xh, f2(-m.y), fma2(g.p[i], w.p[i], f2(-m.x))));
         }
         if (dx) store8(dx + row * lddx, c, n, true, x);
     }
@@ -838,7 +877,7 @@ struct NormForward {
 };
 template <typename T, bool kV, bool k8, int kLanes, int kChunks>
 static int launch_norm_forward(const NormForward &a) {
-    constexpr int kRows = kLanes > 32 ? (kChunks == 1 ? 2 : 1) : 2 / kChunks;
+    constexpr int kRows = kLanes > 32 ? (kChunks == 1 && !k8 ? 2 : 1) : 2 / kChunks;
     constexpr int64_t kPerCta = (int64_t)Group<kLanes>::kGroups * kRows;
     const int64_t want = (a.rows + kPerCta - 1) / kPerCta;
     const int grid = (int)std::min<int64_t>(want, (int64_t)fcai::sm_count() * (kLanes > 32 ? std::max(1, 1024 / kLanes) : 6));
