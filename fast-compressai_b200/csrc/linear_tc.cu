@@ -13,20 +13,31 @@
 // row stride is not 16-byte aligned, which TMA cannot read, is copied once
 // into the workspace with a padded stride (repack_kernel).
 //
-// CTA organisation (persistent, one CTA per SM, 10 warps):
-//   warps 0-7  epilogue: TMEM -> registers -> a per-warp 32 x 32 fp32 staging
-//              tile (XOR-swizzled, so both directions are free of bank
-//              conflicts) -> bias, activation, residual and rounding in a
-//              layout where 4 lanes cover 32 columns of a row, 16 bytes each
-//   warp 8     TMA producer
-//   warp 9     MMA issuer; owns the TMEM allocation
+// CTA organisation (persistent, one CTA per SM, 18 warps; 10 with 64 columns):
+//   16 (8) warps  epilogue: TMEM -> registers -> a per-warp 32 x 32 fp32
+//                 staging tile (XOR-swizzled, so both directions are free of
+//                 bank conflicts) -> bias, activation, residual and rounding
+//                 in a layout where 4 lanes cover 32 columns of a row, 16
+//                 bytes each
+//   one warp      TMA producer
+//   one warp      MMA issuer; owns the TMEM allocation
 // Two TMEM accumulators let the epilogue of a tile overlap the next mainloop.
+// Layers with short contractions are bound by the epilogue's instructions, and
+// four epilogue warps a scheduler hide its latencies where two did not.
+//
+// A forward product that keeps the activation's input in 8 bits makes the
+// codes here: the warps that share 128 columns of a row exchange their largest
+// magnitudes through shared memory, and the codes leave beside y, so the
+// activation's input never exists in memory in more than 8 bits.
 //
 // Work units are (tile, split): when a product has fewer tiles than SMs (few
 // rows, or a weight gradient whose long axis is the contraction), K is split
 // and each unit writes an fp32 partial tile to the workspace; reduce_kernel
 // sums the splits in order (bitwise the same on every run) and applies the
 // epilogue.
+//
+// Up to 32 rows the forward product is a matter of reading w once:
+// few_rows_kernel does it with warp-level MMAs, w as their 16-row operand.
 #include <cuda_runtime.h>
 #include <cudaTypedefs.h>
 
@@ -48,23 +59,37 @@ using namespace ly;
 
 constexpr int kBM = 128;            // tile rows of one CTA
 constexpr int kBK = 64;             // K per ring stage: one 128-byte swizzled row
-constexpr int kEpiWarps = 8;
-constexpr int kThreads = (kEpiWarps + 2) * 32;
 constexpr int kStagingWarp = 32 * 32 * 4;
 constexpr uint64_t kWaitNs = 1000000000ull;
 
+// Division of n < 2^31 by a divisor known on the host (Granlund and Montgomery,
+// Division by Invariant Integers using Multiplication, 1994).
+struct FastDiv {
+    uint32_t d, mul, shift;
+};
+static FastDiv fast_div(uint32_t d) {
+    uint32_t l = 0;
+    while (l < 32 && (1ull << l) < d) ++l;
+    return {d, (uint32_t)((((1ull << l) - d) << 32) / d + 1), l};
+}
+__device__ __forceinline__ int divide(int n, const FastDiv &f) { return (int)((__umulhi((uint32_t)n, f.mul) + (uint32_t)n) >> f.shift); }
+
 struct Params {
     int M, N;
-    int tiles_m, tiles_n, group_m;
-    int splits, ksteps, ksteps_split;  // K steps in all and per split
+    int tiles_m, group_m;
+    FastDiv splits, group, gm, gm_last;  // group: tiles of a group; gm: row tiles of a full / the last group
+    int ksteps, ksteps_split;            // K steps in all and per split
     int units;
-    int ldp;                           // partial tiles: row stride (N rounded up to 8)
-    int vec;                           // y, residual, pre and bias take 16-byte accesses
+    int ldp;                             // partial tiles: row stride (N rounded up to 8)
+    int vec;                             // y, residual, pre, bias and codes take wide accesses
     int act;
     const void *bias, *residual;
     void *y, *pre;
     int64_t ldy, ldr, ldpre;
-    float *partial;                    // [splits][M][ldp], or NULL
+    float *partial;                      // [splits][M][ldp], or NULL
+    uint8_t *codes;                      // [M][N], or NULL
+    float *scales;                       // [M][nblk]
+    int nblk, keep;
 };
 
 // A tile is kPair ? 256 : 128 rows by kBN columns.
@@ -72,15 +97,19 @@ template <int kBN, bool kPair>
 struct Layout {
     static constexpr int kNB = kPair ? kBN / 2 : kBN;  // rows of B this CTA stages
     static constexpr int kTileM = kPair ? 2 * kBM : kBM;
+    static constexpr int kColWarps = kBN == 64 ? 2 : 4;  // epilogue warps side by side, 32 columns each
+    static constexpr int kEpiWarps = 4 * kColWarps;
+    static constexpr int kThreads = (kEpiWarps + 2) * 32;
     static constexpr int kA = kBM * kBK * 2;
     static constexpr int kB = kNB * kBK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = kNB == 64 ? 8 : 6;
+    static constexpr int kStages = kNB == 64 ? 8 : 5;
     static constexpr int offStaging = kStages * kStage;
     static constexpr int offBar = offStaging + kEpiWarps * kStagingWarp;
     static constexpr int kBars = 2 * kStages + 2 * 2 + 1;
     static constexpr int offSlot = offBar + kBars * 8;
-    static constexpr int kBytes = offSlot + 16;
+    static constexpr int offOk = offSlot + 16;  // per quarter and parity of the tile: a warp's wait ran out
+    static constexpr int kBytes = offOk + 32;
     static constexpr int kAlloc = kBytes + 1024;  // the base is rounded up to 1024
     static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
@@ -89,36 +118,64 @@ struct Layout {
 // row tiles, column by column, so that the CTAs of a wave share operand tiles
 // in L2; the splits of a tile are neighbours.
 __device__ __forceinline__ void unit_coords(const Params &p, int unit, int &tm, int &tn, int &sp) {
-    const int t = unit / p.splits;
-    sp = unit - t * p.splits;
-    const int per = p.group_m * p.tiles_n;
-    const int g = t / per;
-    const int rest = t - g * per;
-    const int gm = min(p.group_m, p.tiles_m - g * p.group_m);
-    tn = rest / gm;
-    tm = g * p.group_m + rest - tn * gm;
+    const int t = divide(unit, p.splits);
+    sp = unit - t * (int)p.splits.d;
+    const int g = divide(t, p.group);
+    const int rest = t - g * (int)p.group.d;
+    const int m0 = g * p.group_m;
+    const bool last = p.tiles_m - m0 < p.group_m;
+    tn = last ? divide(rest, p.gm_last) : divide(rest, p.gm);
+    tm = m0 + rest - tn * (int)(last ? p.gm_last.d : p.gm.d);
 }
 
-// Epilogue of kR rows' 8 neighbouring columns from `col` on; rows at
-// `row + i * row_step`, those from M on left out.  All rows go through each
-// step together, so that their loads and arithmetic overlap.
-template <typename T, int kR>
-__device__ __forceinline__ void finish(const Params &p, int64_t row, int row_step, int col, float (&v)[kR * 8]) {
-    if (p.bias) {
-        float bias[8];
-        Vec8<T>::load(static_cast<const T *>(p.bias) + col, bias);
+// A block's scale and the codes of kR rows' 8 columns (pairs v[4 * i ...]).
+__device__ __forceinline__ float keep_scale(int keep, float amax) {
+    return keep == FCAI_KEEP_E4M3 ? block_scale<true>(amax) : block_scale<false>(amax);
+}
+__device__ __forceinline__ uint2 keep_codes(int keep, const V8 &v, float scale) {
+    const float inv = __frcp_rn(scale);
+    return keep == FCAI_KEEP_E4M3 ? encode8<true>(v, inv) : encode8<false>(v, inv);
+}
+__device__ __forceinline__ float amax8(const F2 *v) {
+    float m = 0.f;
 #pragma unroll
-        for (int i = 0; i < kR * 8; ++i) v[i] += bias[i & 7];
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = split(v[i]);
+        m = max_nan(m, max_nan(fabsf(f.x), fabsf(f.y)));
     }
+    return m;
+}
+
+template <typename T>
+__device__ __forceinline__ uint4 pack8(const F2 *v) {
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = split(v[i]);
+        w[i] = pack2(f.x, f.y, T());
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+template <typename T>
+__device__ __forceinline__ void unpack8(const uint4 &q, F2 *v) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = unpack2(w[i], T());
+        v[i] = f2(f.x, f.y);
+    }
+}
+
+// Epilogue of kR rows' 8 neighbouring columns from `col` on, bias already
+// added; rows at `row + i * row_step`, those from M on left out.  All rows go
+// through each step together, so that their loads and arithmetic overlap.
+template <typename T, int kR>
+__device__ __forceinline__ void finish(const Params &p, int64_t row, int row_step, int col, F2 (&v)[kR * 4]) {
     if (p.pre) {
 #pragma unroll
         for (int i = 0; i < kR; ++i)
-            if (row + i * row_step < p.M) {
-                float o[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) o[e] = v[i * 8 + e];
-                Vec8<T>::store(static_cast<T *>(p.pre) + (row + i * row_step) * p.ldpre + col, o);
-            }
+            if (row + i * row_step < p.M)
+                *reinterpret_cast<uint4 *>(static_cast<T *>(p.pre) + (row + i * row_step) * p.ldpre + col) = pack8<T>(v + 4 * i);
     }
     uint4 res[kR];
     if (p.residual) {
@@ -127,70 +184,95 @@ __device__ __forceinline__ void finish(const Params &p, int64_t row, int row_ste
             if (row + i * row_step < p.M)
                 res[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + (row + i * row_step) * p.ldr + col));
     }
-    if (p.act != FCAI_ACT_NONE) {
-        F2 w[kR * 4];
-#pragma unroll
-        for (int i = 0; i < kR * 4; ++i) w[i] = f2(v[2 * i], v[2 * i + 1]);
-        act_n(p.act, w);
-#pragma unroll
-        for (int i = 0; i < kR * 4; ++i) {
-            const float2 o = split(w[i]);
-            v[2 * i] = o.x, v[2 * i + 1] = o.y;
-        }
-    }
+    act_n(p.act, v);
 #pragma unroll
     for (int i = 0; i < kR; ++i) {
         if (row + i * row_step >= p.M) continue;
-        float o[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = v[i * 8 + e];
         if (p.residual) {
-            float r[8];
-            Vec8<T>::unpack(res[i], r);
+            F2 r[4];
+            unpack8<T>(res[i], r);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) o[e] += r[e];
+            for (int e = 0; e < 4; ++e) v[4 * i + e] = add2(v[4 * i + e], r[e]);
         }
-        Vec8<T>::store(static_cast<T *>(p.y) + (row + i * row_step) * p.ldy + col, o);
+        *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + (row + i * row_step) * p.ldy + col) = pack8<T>(v + 4 * i);
     }
 }
 template <typename T>
-__device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, float v, float bias) {
-    v += bias;
+__device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, float v) {
     if (p.pre) static_cast<T *>(p.pre)[row * p.ldpre + col] = from_f32<T>(v);
     v = act_1(p.act, v);
     if (p.residual) v += to_f32(static_cast<const T *>(p.residual)[row * p.ldr + col]);
     static_cast<T *>(p.y)[row * p.ldy + col] = from_f32<T>(v);
 }
+template <typename T>
+__device__ __forceinline__ void add_bias8(const Params &p, int col, F2 *v, int rows) {
+    if (!p.bias) return;
+    F2 b[4];
+    unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.bias) + col)), b);
+#pragma unroll
+    for (int i = 0; i < rows * 4; ++i) v[i] = add2(v[i], b[i & 3]);
+}
 
 // One 32 x 32 chunk of a warp: rows [row0, row0 + 32) from the staging tile.
-template <typename T>
-__device__ __forceinline__ void write_chunk(const Params &p, const unsigned char *stg, int row0, int col0, int sp,
-                                            int lane) {
-    if (col0 >= p.N) return;
+// With codes the kColWarps warps of these rows all come here for each chunk
+// (whatever their columns), and meet at named barrier 1 + quarter.
+template <typename T, int kColWarps>
+__device__ __forceinline__ void write_chunk(const Params &p, unsigned char *staging, int quarter, int colwarp, int row0, int col0,
+                                            int sp, int lane) {
+    const unsigned char *stg = staging + (colwarp * 4 + quarter) * kStagingWarp;
     if (p.partial || p.vec) {
         const int col = col0 + (lane & 3) * 8, r0 = lane >> 2;
-        if (col >= (p.partial ? p.ldp : p.N)) return;  // both multiples of 8
-        float v[32];
+        const bool in = col < (p.partial ? p.ldp : p.N);  // both multiples of 8
+        F2 v[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int r = i * 8 + r0;
             const float4 a = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3)) ^ (r & 7)) << 4));
             const float4 b = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3) + 1) ^ (r & 7)) << 4));
-            v[8 * i] = a.x, v[8 * i + 1] = a.y, v[8 * i + 2] = a.z, v[8 * i + 3] = a.w;
-            v[8 * i + 4] = b.x, v[8 * i + 5] = b.y, v[8 * i + 6] = b.z, v[8 * i + 7] = b.w;
+            v[4 * i] = f2(a.x, a.y), v[4 * i + 1] = f2(a.z, a.w), v[4 * i + 2] = f2(b.x, b.y), v[4 * i + 3] = f2(b.z, b.w);
         }
         if (p.partial) {
+            if (!in) return;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const int row = row0 + i * 8 + r0;
                 if (row >= p.M) break;
                 float4 *dst = reinterpret_cast<float4 *>(p.partial + ((int64_t)sp * p.M + row) * p.ldp + col);
-                dst[0] = make_float4(v[8 * i], v[8 * i + 1], v[8 * i + 2], v[8 * i + 3]);
-                dst[1] = make_float4(v[8 * i + 4], v[8 * i + 5], v[8 * i + 6], v[8 * i + 7]);
+                const float2 a = split(v[4 * i]), b = split(v[4 * i + 1]), c = split(v[4 * i + 2]), d = split(v[4 * i + 3]);
+                dst[0] = make_float4(a.x, a.y, b.x, b.y);
+                dst[1] = make_float4(c.x, c.y, d.x, d.y);
             }
-        } else {
-            finish<T, 4>(p, row0 + r0, 8, col, v);
+            return;
         }
+        if (in) add_bias8<T>(p, col, v, 4);
+        if (p.codes) {
+            const int blk = col0 / FCAI_KEEP_BLOCK;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float m = in ? amax8(v + 4 * i) : 0.f;
+                m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
+                m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
+                // the staging tile is in registers by now: its first words take the rows' magnitudes
+                if (i == 0) __syncwarp();
+                if ((lane & 3) == 0) reinterpret_cast<float *>(staging + (colwarp * 4 + quarter) * kStagingWarp)[i * 8 + r0] = m;
+            }
+            named_barrier_sync(1 + quarter, kColWarps * 32);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float m = 0.f;
+#pragma unroll
+                for (int w = 0; w < kColWarps; ++w)
+                    m = max_nan(m, reinterpret_cast<const float *>(staging + (w * 4 + quarter) * kStagingWarp)[i * 8 + r0]);
+                const int row = row0 + i * 8 + r0;
+                if (!in || row >= p.M) continue;
+                const float s = keep_scale(p.keep, m);
+                const V8 x = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
+                *reinterpret_cast<uint2 *>(p.codes + (int64_t)row * p.N + col) = keep_codes(p.keep, x, s);
+                if (colwarp == 0 && (lane & 3) == 0) p.scales[(int64_t)row * p.nblk + blk] = s;
+            }
+            named_barrier_sync(1 + quarter, kColWarps * 32);  // the magnitudes have been read
+        }
+        if (in) finish<T, 4>(p, row0 + r0, 8, col, v);
     } else {
         const int col = col0 + lane;
         if (col >= p.N) return;
@@ -199,7 +281,7 @@ __device__ __forceinline__ void write_chunk(const Params &p, const unsigned char
         for (int r = 0; r < 32; ++r) {
             if (row0 + r >= p.M) break;
             const float v = *reinterpret_cast<const float *>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-            finish1<T>(p, row0 + r, col, v, bias);
+            finish1<T>(p, row0 + r, col, v + bias);
         }
     }
 }
@@ -209,10 +291,10 @@ __device__ __forceinline__ void write_chunk(const Params &p, const unsigned char
 // stages its 128 rows of A and half the columns' rows of B and owns 128 rows
 // of the accumulator; the rank-0 CTA issues for both.
 template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
     using Lay = Layout<kBN, kPair>;
-    constexpr int kStages = Lay::kStages;
+    constexpr int kStages = Lay::kStages, kEpiWarps = Lay::kEpiWarps;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -223,6 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     uint64_t *dbar = acce + 2;         // abort path: this CTA's MMAs drained
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::offSlot);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + Lay::offSlot + 4);
+    volatile int *failed = reinterpret_cast<volatile int *>(smem + Lay::offOk);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -243,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         mbar_init(dbar, 1);
         *abort = 0;
+        for (int i = 0; i < 8; ++i) failed[i] = 0;
         fence_barrier_init();
     }
     if (warp == kEpiWarps + 1) {
@@ -376,26 +460,32 @@ __global__ void __launch_bounds__(kThreads, 1)
         __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue
-        const int q = warp & 3, half = warp >> 2;
+        const int q = warp & 3, colwarp = warp >> 2;
         unsigned char *stg = smem + Lay::offStaging + warp * kStagingWarp;
         int j = 0;
         for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
             int tm, tn, sp;
             unit_coords(p, unit, tm, tn, sp);
             const int buf = j & 1;
-            if (!mbar_wait_warp(&accf[buf], (j >> 1) & 1, abort, kWaitNs)) {
-                *abort = 1;
-                break;
+            bool ok = mbar_wait_warp(&accf[buf], (j >> 1) & 1, abort, kWaitNs);
+            if (!ok) *abort = 1;
+            if (p.codes) {
+                // the warps that will meet inside the tile leave together: a flag
+                // per tile parity, since none gets two tiles ahead of another
+                if (!ok) failed[2 * q + buf] = 1;
+                named_barrier_sync(1 + q, Lay::kColWarps * 32);
+                ok = !failed[2 * q + buf];
             }
+            if (!ok) break;
             tc_fence_after();
             const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
             const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
-            for (int c = half * (kBN / 2); c < (half + 1) * (kBN / 2); c += 32) {
+            for (int c = colwarp * 32; c < kBN; c += Lay::kColWarps * 32) {
                 uint32_t v[32];
                 tmem_ld32(taddr + c, v);
                 tmem_wait_ld();
-                if (c + 32 == (half + 1) * (kBN / 2)) {  // this warp has read its part of the accumulator
+                if (c + Lay::kColWarps * 32 >= kBN) {  // this warp has read its part of the accumulator
                     tc_fence_before();
                     __syncwarp();
                     if (lane == 0) {
@@ -403,13 +493,15 @@ __global__ void __launch_bounds__(kThreads, 1)
                         else mbar_arrive(&acce[buf]);
                     }
                 }
-                if (row0 < p.M) {
+                const int col0 = tn * kBN + c;
+                // the warps of a quarter agree on this when they have to meet for codes
+                if (row0 < p.M && (col0 < p.N || (p.codes && tn * kBN + c / (Lay::kColWarps * 32) * (Lay::kColWarps * 32) < p.N))) {
 #pragma unroll
                     for (int e = 0; e < 8; ++e)
                         *reinterpret_cast<uint4 *>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
                             make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     __syncwarp();
-                    write_chunk<T>(p, stg, row0, tn * kBN + c, sp, lane);
+                    write_chunk<T, Lay::kColWarps>(p, smem + Lay::offStaging, q, colwarp, row0, col0, sp, lane);
                     __syncwarp();
                 }
             }
@@ -440,40 +532,182 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
 }
 
-// Sums the splits of 8 neighbouring columns in order and applies the epilogue.
+// Sums the splits in order and applies the epilogue: 16 lanes a row's 128
+// columns, 8 each, so that an 8-bit block is theirs.  Also the second half of a
+// product that keeps codes but whose rows do not take wide accesses.
 template <typename T>
-__global__ void reduce_kernel(const Params p) {
-    const int per_row = p.ldp / 8;
-    const int64_t n = (int64_t)p.M * per_row;
+__global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
+    const int col = blockIdx.x * FCAI_KEEP_BLOCK + (threadIdx.x & 15) * 8;
     const int64_t step = (int64_t)p.M * p.ldp;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / per_row;
-        const int col = (int)(i - row * per_row) * 8;
-        float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-        const float *src = p.partial + row * p.ldp + col;
-        for (int s = 0; s < p.splits; ++s, src += step) {
-            float u[8];
-            Vec8<float>::load(src, u);
+    // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
+    for (int64_t r0 = (int64_t)blockIdx.y * 16 + (threadIdx.x >> 5) * 2; r0 < p.M; r0 += (int64_t)gridDim.y * 16) {
+        const int64_t row = r0 + ((threadIdx.x >> 4) & 1);
+        const bool in = row < p.M && col < p.N;
+        F2 v[4] = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
+        if (in) {
+            const float *src = p.partial + row * p.ldp + col;
+#pragma unroll 4
+            for (int s = 0; s < (int)p.splits.d; ++s, src += step) {
+                const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
+                v[0] = add2(v[0], f2(a.x, a.y)), v[1] = add2(v[1], f2(a.z, a.w));
+                v[2] = add2(v[2], f2(b.x, b.y)), v[3] = add2(v[3], f2(b.z, b.w));
+            }
+            if (p.vec) {
+                add_bias8<T>(p, col, v, 1);
+            } else if (p.bias) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += u[e];
+                for (int e = 0; e < 4; ++e) {
+                    auto at = [&](int c) { return c < p.N ? to_f32(static_cast<const T *>(p.bias)[c]) : 0.f; };
+                    v[e] = add2(v[e], f2(at(col + 2 * e), at(col + 2 * e + 1)));
+                }
+            }
         }
+        if (p.codes) {
+            // columns from N on are zeros: their weights were, and no bias was added
+            float m = in ? amax8(v) : 0.f;
+#pragma unroll
+            for (int d = 8; d >= 1; d >>= 1) m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, d));
+            if (in) {
+                const float s = keep_scale(p.keep, m);
+                const uint2 q = keep_codes(p.keep, V8{v[0], v[1], v[2], v[3]}, s);
+                uint8_t *dst = p.codes + row * p.N + col;
+                if (p.vec) {
+                    *reinterpret_cast<uint2 *>(dst) = q;
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        if (col + e < p.N) dst[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
+                }
+                if ((threadIdx.x & 15) == 0) p.scales[row * p.nblk + blockIdx.x] = s;
+            }
+        }
+        if (!in) continue;
         if (p.vec) {
             finish<T, 1>(p, row, 0, col, v);
         } else {
-            for (int e = 0; e < 8 && col + e < p.N; ++e)
-                finish1<T>(p, row, col + e, v[e], p.bias ? to_f32(static_cast<const T *>(p.bias)[col + e]) : 0.f);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 f = split(v[e / 2]);
+                if (col + e < p.N) finish1<T>(p, row, col + e, e & 1 ? f.y : f.x);
+            }
         }
     }
 }
 
-// src[rows][cols] (row stride ld) -> dst[rows][ldd], for matrices TMA cannot read.
-__global__ void repack_kernel(const uint16_t *__restrict__ src, int64_t ld, uint16_t *__restrict__ dst, int64_t rows,
-                              int cols, int ldd) {
-    const int64_t n = rows * ldd;
-    for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) {
-        const int64_t row = i / ldd;
-        const int col = (int)(i - row * ldd);
-        dst[i] = col < cols ? __ldg(src + row * ld + col) : (uint16_t)0;
+// One or two matrices that TMA cannot read, [rows][cols] with row stride ld,
+// into dst[rows][ldd]: a warp a row.
+struct Repack {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t ld, rows;
+    int cols, ldd;
+};
+__global__ void __launch_bounds__(256) repack_kernel(const Repack a, const Repack b) {
+    const Repack &o = blockIdx.y ? b : a;
+    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < o.rows; row += (int64_t)gridDim.x * 8) {
+        const uint16_t *src = o.src + row * o.ld;
+        uint16_t *dst = o.dst + row * o.ldd;
+#pragma unroll 4
+        for (int c = threadIdx.x & 31; c < o.ldd; c += 32) dst[c] = c < o.cols ? __ldg(src + c) : (uint16_t)0;
+    }
+}
+
+// ---- few rows -----------------------------------------------------------------
+// y for up to 8 * kNB rows of x: every weight is read once, 16 bytes a lane, and
+// the sums run on warp-level MMAs (m16n8k16: 16 rows of w by 8 rows of x).
+// Lane (g, t) = (lane / 4, lane % 4) holds 8 consecutive k of w's rows g and g + 8
+// and of x's row g; an MMA takes k in any order as long as both operands agree,
+// so these 8 serve two MMAs as they were loaded.  A CTA owns 16 columns of y;
+// its warps take K in turns of 64, and their sums meet in shared memory in a
+// fixed order.  Bound by reading w; 16 warps times 4 loads of 512 bytes
+// in flight an SM cover the latency.
+template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
+template <>
+__device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+template <>
+__device__ __forceinline__ void mma16816<__half>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+struct FewRows {
+    const void *x, *w;
+    int64_t ldx, ldw;
+    int K;
+};
+// k .. k + 7 of a row (zeros past K, and everything for a row that is not there)
+template <bool kV>
+__device__ __forceinline__ uint4 load_k8(const uint16_t *row, int k, int K, bool in) {
+    uint4 q = make_uint4(0u, 0u, 0u, 0u);
+    if (kV) {
+        if (in && k < K) q = __ldg(reinterpret_cast<const uint4 *>(row + k));
+    } else {
+        uint32_t w[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (in && k + i < K) w[i / 2] |= (uint32_t)__ldg(row + k + i) << (16 * (i & 1));
+        q = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    return q;
+}
+template <typename T, int kNB, int kWarps, bool kV>
+__global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const FewRows f, const Params p) {
+    __shared__ float sums[kWarps][kNB * 128];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int n0 = blockIdx.x * 16;
+    const uint16_t *w0 = static_cast<const uint16_t *>(f.w) + (int64_t)(n0 + g) * f.ldw;
+    const uint16_t *w1 = w0 + 8 * f.ldw;
+    const bool in0 = n0 + g < p.N, in1 = n0 + g + 8 < p.N;
+    float d[kNB][4];
+#pragma unroll
+    for (int b = 0; b < kNB; ++b) d[b][0] = d[b][1] = d[b][2] = d[b][3] = 0.f;
+    constexpr int kUnroll = kNB == 4 ? 2 : 4;
+    for (int k0 = warp * 32; k0 < f.K; k0 += kWarps * 32 * kUnroll) {
+        uint4 a0[kUnroll], a1[kUnroll], x[kUnroll][kNB];
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const int k = k0 + u * kWarps * 32 + t * 8;
+            a0[u] = load_k8<kV>(w0, k, f.K, in0);
+            a1[u] = load_k8<kV>(w1, k, f.K, in1);
+#pragma unroll
+            for (int b = 0; b < kNB; ++b)
+                x[u][b] = load_k8<kV>(static_cast<const uint16_t *>(f.x) + (int64_t)(b * 8 + g) * f.ldx, k, f.K, b * 8 + g < p.M);
+        }
+#pragma unroll
+        for (int u = 0; u < kUnroll; ++u) {
+            const uint32_t lo[4] = {a0[u].x, a1[u].x, a0[u].y, a1[u].y}, hi[4] = {a0[u].z, a1[u].z, a0[u].w, a1[u].w};
+#pragma unroll
+            for (int b = 0; b < kNB; ++b) {
+                mma16816<T>(d[b], lo, x[u][b].x, x[u][b].y);
+                mma16816<T>(d[b], hi, x[u][b].z, x[u][b].w);
+            }
+        }
+    }
+    // d: rows g, g + 8 of w by rows 2 t, 2 t + 1 of x -> sums[warp][x row][w row]
+#pragma unroll
+    for (int b = 0; b < kNB; ++b) {
+        float *s = sums[warp] + (b * 8 + 2 * t) * 16 + g;
+        s[0] = d[b][0], s[16] = d[b][1], s[8] = d[b][2], s[24] = d[b][3];
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < kNB * 128; i += kWarps * 32) {
+        const int row = i >> 4, col = n0 + (i & 15);
+        if (row >= p.M || col >= (p.partial ? p.ldp : p.N)) continue;  // columns from N to ldp: zeros
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w) v += sums[w][i];
+        if (p.partial) {  // the epilogue follows in reduce_kernel, which sees whole 8-bit blocks
+            p.partial[(int64_t)row * p.ldp + col] = v;
+            continue;
+        }
+        if (p.bias) v += to_f32(static_cast<const T *>(p.bias)[col]);
+        finish1<T>(p, row, col, v);
     }
 }
 
@@ -531,17 +765,19 @@ struct Plan {
     int bn, pair, splits, ksteps, ksteps_split, tiles_m, tiles_n;
     int64_t partial_bytes;
 };
-static Plan make_plan(int64_t M, int64_t N, int64_t K) {
+// reduce: the epilogue runs in reduce_kernel even without splits; codes: tiles hold whole 8-bit blocks.
+static Plan make_plan(int64_t M, int64_t N, int64_t K, bool reduce = false, bool codes = false) {
     struct Shape {
         int bn, pair;
         double kstep, epilogue;  // clocks a K step; clocks of a tile's epilogue
     };
-    static const Shape shapes[3] = {{256, 1, 540., 5000.}, {128, 0, 560., 2500.}, {64, 0, 400., 1300.}};
+    static const Shape shapes[3] = {{256, 1, 540., 3000.}, {128, 0, 560., 1500.}, {64, 0, 400., 1300.}};
     const int sms = fcai::sm_count();
     Plan best{};
     double best_time = 0.;
     for (const Shape &sh : shapes) {
         if (sh.bn > 64 && N <= sh.bn / 2) continue;
+        if (codes && sh.bn < FCAI_KEEP_BLOCK && N > sh.bn) continue;
         Plan pl{};
         pl.bn = sh.bn;
         pl.pair = sh.pair;
@@ -555,7 +791,7 @@ static Plan make_plan(int64_t M, int64_t N, int64_t K) {
         splits = std::max(1, std::min(splits, pl.ksteps / 4));
         pl.ksteps_split = (pl.ksteps + splits - 1) / splits;
         pl.splits = (pl.ksteps + pl.ksteps_split - 1) / pl.ksteps_split;  // none is empty
-        pl.partial_bytes = pl.splits > 1 ? round256((int64_t)pl.splits * M * round8((int)N) * 4) : 0;
+        pl.partial_bytes = pl.splits > 1 || reduce ? round256((int64_t)pl.splits * M * round8((int)N) * 4) : 0;
         const int64_t waves = (tiles * pl.splits + slots - 1) / slots;
         // a tile's epilogue runs under the next tile's K steps
         double time = waves * std::max(pl.ksteps_split * sh.kstep, sh.epilogue) + sh.epilogue;
@@ -580,17 +816,24 @@ static int elementwise_grid(int64_t n, int threads) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((n + threads - 1) / threads, (int64_t)fcai::sm_count() * 8));
 }
 
-// Makes `o` readable by TMA, from the workspace if it has to be copied.
-static int prepare_operand(Operand &o, int dtype, unsigned char *&ws, cudaStream_t stream) {
-    if (aligned16(o.ptr, o.ld, dtype)) return FCAI_OK;
-    const int ldd = round8(o.cols);
-    repack_kernel<<<elementwise_grid(o.rows * ldd, 256), 256, 0, stream>>>(static_cast<const uint16_t *>(o.ptr), o.ld,
-                                                                         reinterpret_cast<uint16_t *>(ws), o.rows,
-                                                                         o.cols, ldd);
+// Makes both operands readable by TMA, from the workspace if they have to be copied.
+static int prepare_operands(Operand &a, Operand &b, int dtype, unsigned char *ws, cudaStream_t stream) {
+    Repack r[2];
+    int n = 0;
+    int64_t rows = 0;
+    for (Operand *o : {&a, &b}) {
+        if (aligned16(o->ptr, o->ld, dtype)) continue;
+        const int ldd = round8(o->cols);
+        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd};
+        rows = std::max(rows, o->rows);
+        o->ptr = ws;
+        o->ld = ldd;
+        ws += repack_bytes(o->rows, o->cols);
+    }
+    if (!n) return FCAI_OK;
+    const int grid = (int)std::min<int64_t>((rows + 7) / 8, (int64_t)fcai::sm_count() * 16);
+    repack_kernel<<<dim3(grid, n), 256, 0, stream>>>(r[0], r[n - 1]);
     FCAI_CUDA_TRY(cudaGetLastError());
-    o.ptr = ws;
-    o.ld = ldd;
-    ws += repack_bytes(o.rows, o.cols);
     return FCAI_OK;
 }
 
@@ -608,7 +851,7 @@ static int launch(const CUtensorMap &a, const CUtensorMap &b, const Params &p, c
     attr.val.clusterDim.y = 1;
     attr.val.clusterDim.z = 1;
     cudaLaunchConfig_t cfg{};
-    cfg.blockDim = dim3(kThreads, 1, 1);
+    cfg.blockDim = dim3(Lay::kThreads, 1, 1);
     cfg.dynamicSmemBytes = Lay::kAlloc;
     cfg.stream = stream;
     cfg.attrs = &attr;
@@ -628,36 +871,56 @@ static int launch(const CUtensorMap &a, const CUtensorMap &b, const Params &p, c
         cfg.gridDim = dim3(2 * n, 1, 1);
         FCAI_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, b, p));
     } else {
-        kernel<<<n, kThreads, Lay::kAlloc, stream>>>(a, b, p);
+        kernel<<<n, Lay::kThreads, Lay::kAlloc, stream>>>(a, b, p);
     }
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
 
+template <typename T>
+static int launch_reduce(const Params &p, cudaStream_t stream) {
+    const int shares = (int)std::min<int64_t>({((int64_t)p.M + 15) / 16, std::max<int64_t>(1, (int64_t)fcai::sm_count() * 8 / p.nblk), 65535});
+    reduce_kernel<T><<<dim3(p.nblk, shares), 256, 0, stream>>>(p);
+    FCAI_CUDA_TRY(cudaGetLastError());
+    return FCAI_OK;
+}
+
+// Whether the epilogue can use wide accesses; the codes are [M][N] bytes.
+static bool wide_outputs(const Params &p, int N, int dtype) {
+    return N % 8 == 0 && aligned16(p.y, p.ldy, dtype) && (!p.pre || aligned16(p.pre, p.ldpre, dtype)) &&
+           (!p.residual || aligned16(p.residual, p.ldr, dtype)) && (!p.bias || aligned16(p.bias, 0, dtype)) &&
+           (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
+}
+// A product with codes runs its epilogue in reduce_kernel when its rows do not
+// take wide accesses; whether they do may not change the workspace, so the size
+// is asked for as if they did not when N alone rules it out.
 template <typename T, bool kTA, bool kTB>
 static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Params p, unsigned char *ws,
                cudaStream_t stream) {
-    const Plan pl = make_plan(M, N, K);
+    p.vec = wide_outputs(p, N, dtype);
+    const bool reduce = p.codes && N % 8 != 0;
+    if (p.codes && !reduce && !p.vec) return fcai::fail(FCAI_ERR_INVALID, "linear: 8-bit codes need 16-byte aligned y, bias, residual rows, and 8-byte aligned codes");
+    const Plan pl = make_plan(M, N, K, reduce, p.codes != nullptr);
     p.M = (int)M;
     p.N = N;
     p.tiles_m = pl.tiles_m;
-    p.tiles_n = pl.tiles_n;
-    p.group_m = 8;
-    p.splits = pl.splits;
+    p.group_m = pl.pair ? 8 : 16;
+    p.splits = fast_div(pl.splits);
+    p.group = fast_div((uint32_t)p.group_m * pl.tiles_n);
+    p.gm = fast_div(p.group_m);
+    p.gm_last = fast_div(pl.tiles_m % p.group_m ? pl.tiles_m % p.group_m : p.group_m);
     p.ksteps = pl.ksteps;
     p.ksteps_split = pl.ksteps_split;
     p.units = pl.tiles_m * pl.tiles_n * pl.splits;
     p.ldp = round8(N);
-    p.vec = N % 8 == 0 && aligned16(p.y, p.ldy, dtype) && (!p.pre || aligned16(p.pre, p.ldpre, dtype)) &&
-            (!p.residual || aligned16(p.residual, p.ldr, dtype)) && (!p.bias || aligned16(p.bias, 0, dtype));
+    p.nblk = (N + FCAI_KEEP_BLOCK - 1) / FCAI_KEEP_BLOCK;
     p.partial = nullptr;
-    if (pl.splits > 1) {
+    if (pl.partial_bytes) {
         p.partial = reinterpret_cast<float *>(ws);
         ws += pl.partial_bytes;
     }
     int rc;
-    if ((rc = prepare_operand(A, dtype, ws, stream))) return rc;
-    if ((rc = prepare_operand(B, dtype, ws, stream))) return rc;
+    if ((rc = prepare_operands(A, B, dtype, ws, stream))) return rc;
     CUtensorMap ma, mb;
     if ((rc = make_map(&ma, A.ptr, A.cols, A.rows, A.ld, kTA ? kBK : kBM, dtype))) return rc;
     if ((rc = make_map(&mb, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.pair ? pl.bn / 2 : pl.bn, dtype)))
@@ -666,11 +929,38 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
          : pl.bn == 128 ? launch<T, 128, false, kTA, kTB>(ma, mb, p, stream)
                         : launch<T, 64, false, kTA, kTB>(ma, mb, p, stream);
     if (rc) return rc;
-    if (pl.splits > 1) {
-        reduce_kernel<T><<<elementwise_grid(M * (p.ldp / 8), 256), 256, 0, stream>>>(p);
-        FCAI_CUDA_TRY(cudaGetLastError());
-    }
+    return p.partial ? launch_reduce<T>(p, stream) : FCAI_OK;
+}
+
+// Up to this many rows the forward product runs without tiles.
+constexpr int kFewRows = 32;
+template <typename T, int kNB, bool kV>
+static int launch_few(const FewRows &f, const Params &p, cudaStream_t stream) {
+    // fewer column groups than SMs: more warps share a group's K
+    const int grid = (p.N + 15) / 16;
+    if (grid >= fcai::sm_count() || f.K < 2048) few_rows_kernel<T, kNB, 8, kV><<<grid, 256, 0, stream>>>(f, p);
+    else few_rows_kernel<T, kNB, 16, kV><<<grid, 512, 0, stream>>>(f, p);
+    FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
+}
+template <typename T, int kNB>
+static int launch_few(const FewRows &f, const Params &p, bool vec, cudaStream_t stream) {
+    return vec ? launch_few<T, kNB, true>(f, p, stream) : launch_few<T, kNB, false>(f, p, stream);
+}
+template <typename T>
+static int run_few(const FewRows &f, int rows, int N, int dtype, Params p, void *ws, cudaStream_t stream) {
+    p.M = rows;
+    p.N = N;
+    p.ldp = round8(N);
+    p.nblk = (N + FCAI_KEEP_BLOCK - 1) / FCAI_KEEP_BLOCK;
+    p.splits = fast_div(1);
+    p.vec = wide_outputs(p, N, dtype);
+    p.partial = p.codes ? static_cast<float *>(ws) : nullptr;
+    const bool vec = f.K % 8 == 0 && aligned16(f.x, f.ldx, dtype) && aligned16(f.w, f.ldw, dtype);
+    const int rc = rows <= 8    ? launch_few<T, 1>(f, p, vec, stream)
+                   : rows <= 16 ? launch_few<T, 2>(f, p, vec, stream)
+                                : launch_few<T, 4>(f, p, vec, stream);
+    return rc || !p.partial ? rc : launch_reduce<T>(p, stream);
 }
 
 // Checks shared by the three products.
@@ -688,13 +978,15 @@ static int check_common(int64_t rows, int cin, int cout, int dtype, const void *
     return FCAI_OK;
 }
 
-static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repack) {
+static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repack, int keep) {
     if (rows < 0 || rows > 0x7FFFFFFF - 256 || cin < 1 || cout < 1 || cin > (1 << 24) || cout > (1 << 24)) return -1;
     if (rows == 0) return 0;
     int64_t n;
     switch (op) {
         case FCAI_LINEAR_FORWARD:
-            n = make_plan(rows, cout, cin).partial_bytes;
+            if (rows <= kFewRows) return keep >= FCAI_KEEP_INT8 ? round256(rows * round8(cout) * 4) : 0;
+            if (keep >= FCAI_KEEP_INT8) n = make_plan(rows, cout, cin, cout % 8 != 0, true).partial_bytes;
+            else n = make_plan(rows, cout, cin).partial_bytes;
             if (repack & 1) n += repack_bytes(rows, cin);
             if (repack & 2) n += repack_bytes(cout, cin);
             return n;
@@ -713,9 +1005,9 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
     }
 }
 static int check_workspace(int op, int64_t rows, int cin, int cout, const void *a, int64_t lda, const void *b, int64_t ldb,
-                           int dtype, const void *ws, int64_t bytes) {
+                           int dtype, int keep, const void *ws, int64_t bytes) {
     const int repack = (aligned16(a, lda, dtype) ? 0 : 1) | (aligned16(b, ldb, dtype) ? 0 : 2);
-    const int64_t need = workspace_bytes(op, rows, cin, cout, repack);
+    const int64_t need = workspace_bytes(op, rows, cin, cout, repack, keep);
     if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
         return fcai::fail(FCAI_ERR_WORKSPACE, "linear: needs a 256-byte aligned workspace of %lld bytes", (long long)need);
     return FCAI_OK;
@@ -725,24 +1017,28 @@ static int check_workspace(int op, int64_t rows, int cin, int cout, const void *
 
 extern "C" {
 
-int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack) {
-    return ln::workspace_bytes(op, rows, cin, cout, repack);
+int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack, int32_t keep) {
+    return ln::workspace_bytes(op, rows, cin, cout, repack, keep);
 }
 
 int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                         const void *residual, int64_t ldr, void *y, int64_t ldy, void *pre, int64_t ldpre,
-                        int64_t rows, int32_t cin, int32_t cout, int32_t dtype, int32_t act, void *workspace,
-                        int64_t workspace_bytes, fcai_stream_t stream) {
+                        void *codes, float *scales, int64_t rows, int32_t cin, int32_t cout, int32_t dtype, int32_t act,
+                        int32_t keep, void *workspace, int64_t workspace_bytes, fcai_stream_t stream) {
     using namespace ln;
     fcai::clear_error();
     int rc = check_common(rows, cin, cout, dtype, x, ldx, cin, w, ldw, cin, y, ldy, cout);
     if (rc) return rc;
     if (act < FCAI_ACT_NONE || act > FCAI_ACT_SILU) return fcai::fail(FCAI_ERR_INVALID, "linear: unknown activation %d", act);
-    if ((residual && ldr < cout) || (pre && ldpre < cout))
+    if (keep < FCAI_KEEP_NONE || keep > FCAI_KEEP_E4M3) return fcai::fail(FCAI_ERR_INVALID, "linear: unknown keep %d", keep);
+    const bool k8 = keep >= FCAI_KEEP_INT8;
+    if ((rows && k8 && (!codes || !scales)) || (keep == FCAI_KEEP_FULL && rows && !pre) || (reinterpret_cast<uintptr_t>(scales) & 3))
+        return fcai::fail(FCAI_ERR_INVALID, "linear: the keep needs its output");
+    if ((residual && ldr < cout) || (keep == FCAI_KEEP_FULL && ldpre < cout))
         return fcai::fail(FCAI_ERR_INVALID, "linear: a row stride is smaller than its row");
     if (rows == 0) return FCAI_OK;
     if (!x || !w || !y) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
-    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, workspace, workspace_bytes)))
+    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, keep, workspace, workspace_bytes)))
         return rc;
     Params p{};
     p.act = act;
@@ -751,11 +1047,19 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     p.ldr = ldr;
     p.y = y;
     p.ldy = ldy;
-    p.pre = pre;
+    p.pre = keep == FCAI_KEEP_FULL ? pre : nullptr;
     p.ldpre = ldpre;
+    p.codes = k8 ? static_cast<uint8_t *>(codes) : nullptr;
+    p.scales = scales;
+    p.keep = keep;
     const Operand A{x, ldx, rows, cin}, B{w, ldw, cout, cin};
     auto *ws = static_cast<unsigned char *>(workspace);
     auto st = static_cast<cudaStream_t>(stream);
+    if (rows <= kFewRows) {
+        const FewRows f{x, w, ldx, ldw, cin};
+        return dtype == FCAI_DTYPE_BF16 ? run_few<__nv_bfloat16>(f, (int)rows, cout, dtype, p, ws, st)
+                                        : run_few<__half>(f, (int)rows, cout, dtype, p, ws, st);
+    }
     return dtype == FCAI_DTYPE_BF16 ? run<__nv_bfloat16, false, false>(A, B, rows, cout, cin, dtype, p, ws, st)
                                     : run<__half, false, false>(A, B, rows, cout, cin, dtype, p, ws, st);
 }
@@ -769,7 +1073,7 @@ int fcai_linear_backward_input(const void *dp, int64_t lddp, const void *w, int6
     if (rc) return rc;
     if (rows == 0) return FCAI_OK;
     if (!dp || !w || !dx) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dtype, workspace,
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dtype, 0, workspace,
                               workspace_bytes)))
         return rc;
     Params p{};
@@ -802,7 +1106,7 @@ int fcai_linear_backward_weight(const void *dp, int64_t lddp, const void *x, int
         FCAI_CUDA_TRY(cudaGetLastError());
         return FCAI_OK;
     }
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dtype, workspace,
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dtype, 0, workspace,
                               workspace_bytes)))
         return rc;
     const Operand A{dp, lddp, rows, cout}, B{x, ldx, rows, cin};

@@ -123,8 +123,8 @@ def _rows(t: torch.Tensor, n: int) -> tuple[torch.Tensor, int, int]:
 
 
 @lru_cache(maxsize=4096)
-def _linear_workspace(device_index: int, op: int, rows: int, cin: int, cout: int, repack: int) -> int:
-    return _native.lib().fcai_linear_workspace(op, rows, cin, cout, repack)
+def _linear_workspace(device_index: int, op: int, rows: int, cin: int, cout: int, repack: int, keep: int = 0) -> int:
+    return _native.lib().fcai_linear_workspace(op, rows, cin, cout, repack, keep)
 
 
 def _scratch(nbytes: int, device) -> tuple[torch.Tensor | None, int]:
@@ -277,14 +277,27 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         if residual is not None:
             residual, _, ldr = _rows(residual, cout)
             r = residual.data_ptr()
-        pre = torch.empty(out_shape, dtype=dtype, device=dev) if keep is not None and activation != "none" else None
+        pre = codes = scales = None
+        pk = 0 if activation == "none" else _KEEP[keep]  # what of the activation's input is kept
+        if pk == 1:
+            pre = torch.empty(out_shape, dtype=dtype, device=dev)
+        elif pk:
+            codes = torch.empty((rows, cout), dtype=torch.uint8, device=dev)
+            scales = torch.empty((rows, -(-cout // BLOCK)), dtype=torch.float32, device=dev)
+            if cout % 8 == 0:  # the codes leave with y's rows, in wide accesses
+                if bias is not None and bias.data_ptr() & 15:
+                    bias = bias.clone()
+                if residual is not None and (r | 2 * ldr) & 15:
+                    residual = residual.reshape(-1, cout).clone(memory_format=torch.contiguous_format)
+                    r, ldr = residual.data_ptr(), cout
         xp, wp = m.data_ptr(), w.data_ptr()
         repack = (1 if (xp | 2 * ldx) & 15 else 0) | (2 if (wp | 2 * ldw) & 15 else 0)
-        nbytes = _linear_workspace(dev.index, _FORWARD, rows, cin, cout, repack)
+        nbytes = _linear_workspace(dev.index, _FORWARD, rows, cin, cout, repack, pk)
         ws, wsp = _scratch(nbytes, dev)
         _check(_native.lib().fcai_linear_forward(
             xp, ldx, wp, ldw, 0 if bias is None else bias.data_ptr(), r, ldr, y.data_ptr(), cout,
-            0 if pre is None else pre.data_ptr(), cout, rows, cin, cout, _DTYPE[dtype], _ACT[activation], wsp, nbytes,
+            0 if pre is None else pre.data_ptr(), cout, 0 if codes is None else codes.data_ptr(),
+            0 if codes is None else scales.data_ptr(), rows, cin, cout, _DTYPE[dtype], _ACT[activation], pk, wsp, nbytes,
             _native.stream_handle(dev)))
         _native.count_launches(1)
         if keep is None:
@@ -292,8 +305,8 @@ def linear_forward(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | N
         kept = x
         if keep != "full":
             kept = _keep8(m, rows, cin, ldx, x.shape, keep)
-            if pre is not None:
-                pre = _keep8(pre, rows, cout, cout, out_shape, keep)
+            if pk:
+                pre = Checkpoint8(codes, scales, out_shape, dtype, keep)
     return y, Saved("linear", kept, out_shape, dtype, pre=pre, activation=activation, bias=bias is not None)
 
 

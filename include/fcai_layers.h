@@ -50,18 +50,22 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
 
 /* ---- matrix product -------------------------------------------------------
  * y[rows][cout] = act(x[rows][cin] * w[cout][cin]^T + bias) + residual; bf16
- * or f16, one type for all tensors.  bias, residual and pre may be NULL; pre
- * receives x * w^T + bias, rounded to the type.  Addresses and strides need
- * only the elements' alignment; 16-byte aligned addresses and strides (8
- * elements) are read without a copy. */
+ * or f16, one type for all tensors; bias and residual may be NULL.  `keep` says
+ * what of p = x * w^T + bias, the activation's input, stays for the backward
+ * pass: NONE; FULL, p rounded to the type in pre; INT8 or E4M3, p (before any
+ * rounding) as codes and scales.  Addresses and strides need only the elements'
+ * alignment; 16-byte aligned addresses and strides (8 elements) are read
+ * without a copy.  With an 8-bit keep and cout a multiple of 8, the addresses
+ * and strides of y, bias and residual are 16-byte aligned and codes 8-byte. */
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
 /* `repack`: bit 0 / bit 1 set when the call's first / second matrix is not
- * 16-byte aligned in address and row stride (x, w; dp, w; dp, x). */
-int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack);
+ * 16-byte aligned in address and row stride (x, w; dp, w; dp, x); `keep`: the
+ * forward call's (0 for the others). */
+int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack, int32_t keep);
 int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                         const void *residual, int64_t ldr, void *y, int64_t ldy, void *pre, int64_t ldpre,
-                        int64_t rows, int32_t cin, int32_t cout, int32_t dtype, int32_t act, void *workspace,
-                        int64_t workspace_bytes, fcai_stream_t stream);
+                        void *codes, float *scales, int64_t rows, int32_t cin, int32_t cout, int32_t dtype, int32_t act,
+                        int32_t keep, void *workspace, int64_t workspace_bytes, fcai_stream_t stream);
 /* dx[rows][cin] = dp[rows][cout] * w[cout][cin] */
 int fcai_linear_backward_input(const void *dp, int64_t lddp, const void *w, int64_t ldw, void *dx, int64_t lddx,
                                int64_t rows, int32_t cin, int32_t cout, int32_t dtype, void *workspace,

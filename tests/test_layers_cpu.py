@@ -50,16 +50,17 @@ def _code(name, *args):
 P = 1 << 20  # stands for a device address; no refused call reads it
 
 
-def _forward(x=P, ldx=64, w=P, ldw=64, bias=None, res=None, ldr=0, y=P, ldy=32, pre=None, ldpre=0, rows=8, cin=64, cout=32,
-             dtype=BF16, act=0, ws=None, wsb=0):
-    return _code("fcai_linear_forward", x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldpre, rows, cin, cout, dtype, act,
-                 ws, wsb, None)
+def _forward(x=P, ldx=64, w=P, ldw=64, bias=None, res=None, ldr=0, y=P, ldy=32, pre=None, ldpre=0, codes=None,
+             scales=None, rows=8, cin=64, cout=32, dtype=BF16, act=0, keep=0, ws=None, wsb=0):
+    return _code("fcai_linear_forward", x, ldx, w, ldw, bias, res, ldr, y, ldy, pre, ldpre, codes, scales, rows, cin, cout,
+                 dtype, act, keep, ws, wsb, None)
 
 
 @pytest.mark.parametrize("bad", [
     dict(dtype=F32), dict(dtype=3), dict(rows=-1), dict(rows=2 ** 31), dict(cin=0), dict(cout=0), dict(ldx=63), dict(ldw=10),
     dict(ldy=31), dict(act=4), dict(act=-1), dict(x=None), dict(w=None), dict(y=None), dict(x=P + 1), dict(res=P, ldr=8),
-    dict(pre=P, ldpre=31),
+    dict(pre=P, ldpre=31, keep=1), dict(keep=1), dict(keep=2, codes=P), dict(keep=3, scales=P), dict(keep=4),
+    dict(keep=2, codes=P, scales=P + 2), dict(keep=2, codes=P + 4, scales=P), dict(keep=2, codes=P, scales=P, y=P + 2),
 ])
 def test_linear_refusals(bad):
     assert _forward(**bad) == _native.FCAI_ERR_INVALID
@@ -68,14 +69,14 @@ def test_linear_refusals(bad):
 
 def test_linear_asks_for_its_workspace():
     # a row stride of 65 elements is not 16-byte aligned: x is repacked
-    need = _code("fcai_linear_workspace", 0, 8, 64, 32, 1)
-    assert need >= 8 * 64 * 2
-    assert _forward(ldx=65, ws=None, wsb=0) == _native.FCAI_ERR_WORKSPACE
-    assert _forward(ldx=65, ws=P, wsb=need - 1) == _native.FCAI_ERR_WORKSPACE
-    assert _forward(ldx=65, ws=P + 8, wsb=need + 8) == _native.FCAI_ERR_WORKSPACE
-    assert _code("fcai_linear_workspace", 3, 8, 64, 32, 0) == -1
-    assert _code("fcai_linear_workspace", 0, -1, 64, 32, 0) == -1
-    assert _code("fcai_linear_workspace", 2, 0, 64, 32, 0) == 0
+    need = _code("fcai_linear_workspace", 0, 80, 64, 32, 1, 0)
+    assert need >= 80 * 64 * 2
+    assert _forward(rows=80, ldx=65, ws=None, wsb=0) == _native.FCAI_ERR_WORKSPACE
+    assert _forward(rows=80, ldx=65, ws=P, wsb=need - 1) == _native.FCAI_ERR_WORKSPACE
+    assert _forward(rows=80, ldx=65, ws=P + 8, wsb=need + 8) == _native.FCAI_ERR_WORKSPACE
+    assert _code("fcai_linear_workspace", 3, 8, 64, 32, 0, 0) == -1
+    assert _code("fcai_linear_workspace", 0, -1, 64, 32, 0, 0) == -1
+    assert _code("fcai_linear_workspace", 2, 0, 64, 32, 0, 0) == 0
 
 
 def test_no_rows_need_no_device():
