@@ -106,7 +106,7 @@ struct Layout {
     static constexpr int kStages = kNB == 64 ? 8 : 5;
     static constexpr int offStaging = kStages * kStage;
     static constexpr int offBar = offStaging + kEpiWarps * kStagingWarp;
-    static constexpr int kBars = 2 * kStages + 2 * 2 + 1;
+    static constexpr int kBars = 2 * kStages + 3 * 2 + 1;
     static constexpr int offSlot = offBar + kBars * 8;
     static constexpr int offOk = offSlot + 16;  // per quarter and parity of the tile: a warp's wait ran out
     static constexpr int kBytes = offOk + 32;
@@ -167,35 +167,39 @@ __device__ __forceinline__ void unpack8(const uint4 &q, F2 *v) {
 }
 
 // Epilogue of kR rows' 8 neighbouring columns from `col` on, bias already
-// added; rows at `row + i * row_step`, those from M on left out.  All rows go
-// through each step together, so that their loads and arithmetic overlap.
+// added: rows row, row + 8, ..., those from M on left out; `res` holds the
+// residual's values if there is one.  All rows go through each step together,
+// so that their arithmetic overlaps.
 template <typename T, int kR>
-__device__ __forceinline__ void finish(const Params &p, int64_t row, int row_step, int col, F2 (&v)[kR * 4]) {
+__device__ __forceinline__ void load_residual(const Params &p, int row, int col, uint4 (&res)[kR]) {
+    if (!p.residual || col >= p.N) return;
+    const T *r = static_cast<const T *>(p.residual) + row * p.ldr + col;
+#pragma unroll
+    for (int i = 0; i < kR; ++i)
+        if (row + i * 8 < p.M) res[i] = __ldg(reinterpret_cast<const uint4 *>(r + i * 8 * p.ldr));
+}
+template <typename T, int kR>
+__device__ __forceinline__ void finish(const Params &p, int row, int col, F2 (&v)[kR * 4], const uint4 (&res)[kR]) {
     if (p.pre) {
+        T *o = static_cast<T *>(p.pre) + row * p.ldpre + col;
 #pragma unroll
         for (int i = 0; i < kR; ++i)
-            if (row + i * row_step < p.M)
-                *reinterpret_cast<uint4 *>(static_cast<T *>(p.pre) + (row + i * row_step) * p.ldpre + col) = pack8<T>(v + 4 * i);
-    }
-    uint4 res[kR];
-    if (p.residual) {
-#pragma unroll
-        for (int i = 0; i < kR; ++i)
-            if (row + i * row_step < p.M)
-                res[i] = __ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + (row + i * row_step) * p.ldr + col));
+            if (row + i * 8 < p.M) *reinterpret_cast<uint4 *>(o + i * 8 * p.ldpre) = pack8<T>(v + 4 * i);
     }
     act_n(p.act, v);
+    if (p.residual) {
 #pragma unroll
-    for (int i = 0; i < kR; ++i) {
-        if (row + i * row_step >= p.M) continue;
-        if (p.residual) {
+        for (int i = 0; i < kR; ++i) {
             F2 r[4];
             unpack8<T>(res[i], r);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[4 * i + e] = add2(v[4 * i + e], r[e]);
         }
-        *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + (row + i * row_step) * p.ldy + col) = pack8<T>(v + 4 * i);
     }
+    T *o = static_cast<T *>(p.y) + row * p.ldy + col;
+#pragma unroll
+    for (int i = 0; i < kR; ++i)
+        if (row + i * 8 < p.M) *reinterpret_cast<uint4 *>(o + i * 8 * p.ldy) = pack8<T>(v + 4 * i);
 }
 template <typename T>
 __device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, float v) {
@@ -213,66 +217,81 @@ __device__ __forceinline__ void add_bias8(const Params &p, int col, F2 *v, int r
     for (int i = 0; i < rows * 4; ++i) v[i] = add2(v[i], b[i & 3]);
 }
 
+// Shared memory by its 32-bit address: through a pointer computed from a
+// rounded base the compiler would use generic accesses.
+__device__ __forceinline__ void sts128(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+__device__ __forceinline__ float4 lds128(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ float lds32(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+
 // One 32 x 32 chunk of a warp: rows [row0, row0 + 32) from the staging tile.
 // With codes the kColWarps warps of these rows all come here for each chunk
 // (whatever their columns), and meet at named barrier 1 + quarter.
 template <typename T, int kColWarps>
-__device__ __forceinline__ void write_chunk(const Params &p, unsigned char *staging, int quarter, int colwarp, int row0, int col0,
-                                            int sp, int lane) {
-    const unsigned char *stg = staging + (colwarp * 4 + quarter) * kStagingWarp;
+__device__ __forceinline__ void write_chunk(const Params &p, uint32_t staging, int quarter, int colwarp, int row0, int col0,
+                                            int sp, int lane, const uint4 (&res)[4]) {
+    const uint32_t stg = staging + (colwarp * 4 + quarter) * kStagingWarp;
     if (p.partial || p.vec) {
         const int col = col0 + (lane & 3) * 8, r0 = lane >> 2;
         const bool in = col < (p.partial ? p.ldp : p.N);  // both multiples of 8
+        const uint32_t src = stg + r0 * 128;
+        const uint32_t c0 = ((2 * (lane & 3)) ^ r0) << 4;  // r0 < 8: the rows' swizzle
         F2 v[16];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int r = i * 8 + r0;
-            const float4 a = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3)) ^ (r & 7)) << 4));
-            const float4 b = *reinterpret_cast<const float4 *>(stg + r * 128 + (((2 * (lane & 3) + 1) ^ (r & 7)) << 4));
+            const float4 a = lds128(src + i * 1024 + c0), b = lds128(src + i * 1024 + (c0 ^ 16));
             v[4 * i] = f2(a.x, a.y), v[4 * i + 1] = f2(a.z, a.w), v[4 * i + 2] = f2(b.x, b.y), v[4 * i + 3] = f2(b.z, b.w);
         }
+        const int row = row0 + r0;
         if (p.partial) {
             if (!in) return;
+            float *dst = p.partial + ((int64_t)sp * p.M + row) * p.ldp + col;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const int row = row0 + i * 8 + r0;
-                if (row >= p.M) break;
-                float4 *dst = reinterpret_cast<float4 *>(p.partial + ((int64_t)sp * p.M + row) * p.ldp + col);
+                if (row + i * 8 >= p.M) break;
                 const float2 a = split(v[4 * i]), b = split(v[4 * i + 1]), c = split(v[4 * i + 2]), d = split(v[4 * i + 3]);
-                dst[0] = make_float4(a.x, a.y, b.x, b.y);
-                dst[1] = make_float4(c.x, c.y, d.x, d.y);
+                reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[0] = make_float4(a.x, a.y, b.x, b.y);
+                reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[1] = make_float4(c.x, c.y, d.x, d.y);
             }
             return;
         }
         if (in) add_bias8<T>(p, col, v, 4);
         if (p.codes) {
-            const int blk = col0 / FCAI_KEEP_BLOCK;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float m = in ? amax8(v + 4 * i) : 0.f;
                 m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
                 m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                // the staging tile is in registers by now: its first words take the rows' magnitudes
-                if (i == 0) __syncwarp();
-                if ((lane & 3) == 0) reinterpret_cast<float *>(staging + (colwarp * 4 + quarter) * kStagingWarp)[i * 8 + r0] = m;
+                // the staging tile is in registers by now (every lane's: the
+                // shuffles); its first words take the rows' magnitudes
+                if ((lane & 3) == 0) sts32(stg + (i * 8 + r0) * 4, m);
             }
             named_barrier_sync(1 + quarter, kColWarps * 32);
+            uint8_t *codes = p.codes + (int64_t)row * p.N + col;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 float m = 0.f;
 #pragma unroll
-                for (int w = 0; w < kColWarps; ++w)
-                    m = max_nan(m, reinterpret_cast<const float *>(staging + (w * 4 + quarter) * kStagingWarp)[i * 8 + r0]);
-                const int row = row0 + i * 8 + r0;
-                if (!in || row >= p.M) continue;
+                for (int w = 0; w < kColWarps; ++w) m = max_nan(m, lds32(staging + (w * 4 + quarter) * kStagingWarp + (i * 8 + r0) * 4));
+                if (!in || row + i * 8 >= p.M) continue;
                 const float s = keep_scale(p.keep, m);
                 const V8 x = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-                *reinterpret_cast<uint2 *>(p.codes + (int64_t)row * p.N + col) = keep_codes(p.keep, x, s);
-                if (colwarp == 0 && (lane & 3) == 0) p.scales[(int64_t)row * p.nblk + blk] = s;
+                *reinterpret_cast<uint2 *>(codes + (int64_t)i * 8 * p.N) = keep_codes(p.keep, x, s);
+                if (colwarp == 0 && (lane & 3) == 0) p.scales[(int64_t)(row + i * 8) * p.nblk + col0 / FCAI_KEEP_BLOCK] = s;
             }
             named_barrier_sync(1 + quarter, kColWarps * 32);  // the magnitudes have been read
         }
-        if (in) finish<T, 4>(p, row0 + r0, 8, col, v);
+        if (in) finish<T, 4>(p, row, col, v, res);
     } else {
         const int col = col0 + lane;
         if (col >= p.N) return;
@@ -280,8 +299,7 @@ __device__ __forceinline__ void write_chunk(const Params &p, unsigned char *stag
 #pragma unroll 4
         for (int r = 0; r < 32; ++r) {
             if (row0 + r >= p.M) break;
-            const float v = *reinterpret_cast<const float *>(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4);
-            finish1<T>(p, row0 + r, col, v + bias);
+            finish1<T>(p, row0 + r, col, lds32(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) + bias);
         }
     }
 }
@@ -301,8 +319,9 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + Lay::offBar);  // pairs: rank 0's counts both CTAs' loads
     uint64_t *empty = full + kStages;
     uint64_t *accf = empty + kStages;  // accumulator filled (by the MMA warp; pairs: in both CTAs)
-    uint64_t *acce = accf + 2;         // accumulator read: one arrival per epilogue warp (pairs: of both CTAs, at rank 0)
-    uint64_t *dbar = acce + 2;         // abort path: this CTA's MMAs drained
+    uint64_t *acce = accf + 2;         // accumulator read: one arrival per epilogue warp of this CTA
+    uint64_t *pacce = acce + 2;        // pairs, rank 0: the peer's accumulator read
+    uint64_t *dbar = pacce + 2;        // abort path: this CTA's MMAs drained
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::offSlot);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + Lay::offSlot + 4);
     volatile int *failed = reinterpret_cast<volatile int *>(smem + Lay::offOk);
@@ -322,7 +341,8 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
         }
         for (int b = 0; b < 2; ++b) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], kPair ? 2 * kEpiWarps : kEpiWarps);
+            mbar_init(&acce[b], kEpiWarps);
+            mbar_init(&pacce[b], 1);
         }
         mbar_init(dbar, 1);
         *abort = 0;
@@ -421,7 +441,8 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
                 int tm, tn, sp;
                 unit_coords(p, unit, tm, tn, sp);
                 const int buf = j & 1;
-                if (!mbar_wait_warp(&acce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs, kPair)) {
+                if (!mbar_wait_warp(&acce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs) ||
+                    (kPair && !mbar_wait_warp(&pacce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs, true))) {
                     *abort = 1;
                     break;
                 }
@@ -456,17 +477,34 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
                 if (kPair) mma_commit_pair_both_w(&accf[buf], 3);
                 else mma_commit_w(&accf[buf]);
             }
+        } else {
+            // The peer's accumulators are free: passed on by this warp, since an
+            // arrival in another CTA waits until the arriving thread's earlier
+            // stores have been seen, and the epilogue's lanes always have some.
+            int j = 0;
+            for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
+                if (!mbar_wait_warp(&acce[j & 1], (j >> 1) & 1, abort, kWaitNs)) {
+                    *abort = 1;
+                    break;
+                }
+                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&pacce[j & 1]), 0));
+            }
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue
         const int q = warp & 3, colwarp = warp >> 2;
-        unsigned char *stg = smem + Lay::offStaging + warp * kStagingWarp;
+        const uint32_t staging = smem_u32(smem + Lay::offStaging);
+        const uint32_t stg = staging + warp * kStagingWarp + lane * 128 + ((lane & 7) << 4);  // this row's chunk 0
         int j = 0;
         for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
             int tm, tn, sp;
             unit_coords(p, unit, tm, tn, sp);
             const int buf = j & 1;
+            const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
+            const bool wide_res = p.vec && p.residual && !p.partial;
+            uint4 res[4];  // the residual's rows: on their way while the accumulator fills
+            if (wide_res) load_residual<T, 4>(p, row0 + (lane >> 2), tn * kBN + colwarp * 32 + (lane & 3) * 8, res);
             bool ok = mbar_wait_warp(&accf[buf], (j >> 1) & 1, abort, kWaitNs);
             if (!ok) *abort = 1;
             if (p.codes) {
@@ -478,7 +516,6 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             }
             if (!ok) break;
             tc_fence_after();
-            const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
             const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
 #pragma unroll 1
             for (int c = colwarp * 32; c < kBN; c += Lay::kColWarps * 32) {
@@ -488,21 +525,18 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
                 if (c + Lay::kColWarps * 32 >= kBN) {  // this warp has read its part of the accumulator
                     tc_fence_before();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (kPair) mbar_arrive_cluster(mapa_shared(smem_u32(&acce[buf]), 0));
-                        else mbar_arrive(&acce[buf]);
-                    }
+                    if (lane == 0) mbar_arrive(&acce[buf]);
                 }
                 const int col0 = tn * kBN + c;
                 // the warps of a quarter agree on this when they have to meet for codes
                 if (row0 < p.M && (col0 < p.N || (p.codes && tn * kBN + c / (Lay::kColWarps * 32) * (Lay::kColWarps * 32) < p.N))) {
 #pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        *reinterpret_cast<uint4 *>(stg + lane * 128 + ((e ^ (lane & 7)) << 4)) =
-                            make_uint4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                    for (int e = 0; e < 8; ++e) sts128(stg ^ (e << 4), v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
                     __syncwarp();
-                    write_chunk<T, Lay::kColWarps>(p, smem + Lay::offStaging, q, colwarp, row0, col0, sp, lane);
+                    write_chunk<T, Lay::kColWarps>(p, staging, q, colwarp, row0, col0, sp, lane, res);
                     __syncwarp();
+                    if (wide_res && c + Lay::kColWarps * 32 < kBN)
+                        load_residual<T, 4>(p, row0 + (lane >> 2), col0 + Lay::kColWarps * 32 + (lane & 3) * 8, res);
                 }
             }
         }
@@ -583,7 +617,9 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
         }
         if (!in) continue;
         if (p.vec) {
-            finish<T, 1>(p, row, 0, col, v);
+            uint4 res[1];
+            load_residual<T, 1>(p, (int)row, col, res);
+            finish<T, 1>(p, (int)row, col, v, res);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
