@@ -138,12 +138,13 @@ __device__ __forceinline__ float hsum(F2 v) {
 // own: iteratively reweighted least squares of R against Q e^(t^2/2) on
 // t in [0, 40], largest relative error 7.6e-7 evaluated in fp32.  `e` comes
 // back for the density.
-__device__ __forceinline__ F2 normal_tail2(float2 t, F2 &e) {
-    const F2 tt = f2(t.x, t.y);
-    const float2 a = split(mul2(mul2(tt, f2(-0.72134752f)), tt));  // log2(e) / 2
-    const float2 d = split(fma2(f2(0.24f), tt, f2(1.f)));
+// One reciprocal serves the pair (1 / a = b / (a b)): the special function
+// unit, not the arithmetic, bounds GELU.  t <= 30, where Q is zero in fp32.
+__device__ __forceinline__ F2 normal_tail2(F2 t, F2 &e) {
+    const float2 a = split(mul2(mul2(t, f2(-0.72134752f)), t));  // log2(e) / 2
+    const float2 d = split(fma2(f2(0.24f), t, f2(1.f)));
     e = f2(ex2_approx(a.x), ex2_approx(a.y));
-    const F2 u = f2(rcp_approx(d.x), rcp_approx(d.y));
+    const F2 u = mul2(f2(d.y, d.x), f2(rcp_approx(d.x * d.y)));
     F2 r = fma2(u, f2(-0.0529928472f), f2(0.152797519f));
     r = fma2(u, r, f2(-0.0657069748f));
     r = fma2(u, r, f2(0.118390834f));
@@ -153,11 +154,34 @@ __device__ __forceinline__ F2 normal_tail2(float2 t, F2 &e) {
     r = fma2(u, r, f2(0.0957537928f));
     return mul2(e, mul2(u, r));
 }
-// Phi(x) of two values.
-__device__ __forceinline__ F2 normal_cdf2(float2 x, F2 &e) {
-    const F2 q = normal_tail2(make_float2(fabsf(x.x), fabsf(x.y)), e);
+// min(|x|, 30), 30 for a NaN: the pair's shared reciprocal must not carry one
+// value's NaN into the other.
+__device__ __forceinline__ F2 tail_arg(float2 x) { return f2(fminf(fabsf(x.x), 30.f), fminf(fabsf(x.y), 30.f)); }
+__device__ __forceinline__ float relu_nan(float x) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(0.f));
+    return y;
+}
+__device__ __forceinline__ float clamp_nan(float x) {  // to +-30; a NaN stays
+    float y;
+    asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(y) : "f"(x), "f"(30.f), "f"(-30.f));
+    return y;
+}
+// x Phi(x) = max(x, 0) - |x| Q(|x|)
+__device__ __forceinline__ F2 gelu2(F2 v) {
+    const float2 x = split(v);
+    F2 e;
+    const F2 t = tail_arg(x);
+    return fma2(mul2(t, f2(-1.f)), normal_tail2(t, e), f2(relu_nan(x.x), relu_nan(x.y)));
+}
+// its derivative, Phi(x) + x phi(x)
+__device__ __forceinline__ F2 gelu_grad2(F2 v) {
+    const float2 x = split(v);
+    F2 e;
+    const F2 q = normal_tail2(tail_arg(x), e);
     const float2 lo = split(q), hi = split(fma2(q, f2(-1.f), f2(1.f)));
-    return f2(x.x < 0.f ? lo.x : hi.x, x.y < 0.f ? lo.y : hi.y);
+    const F2 cdf = f2(x.x < 0.f ? lo.x : hi.x, x.y < 0.f ? lo.y : hi.y);
+    return fma2(mul2(f2(clamp_nan(x.x), clamp_nan(x.y)), e), f2(0.398942280f), cdf);
 }
 __device__ __forceinline__ F2 sigmoid2(F2 x) {
     const float2 a = split(mul2(x, f2(-1.44269504f)));
@@ -176,10 +200,7 @@ __device__ __forceinline__ void act_n(int kind, F2 (&v)[kN]) {
         }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            F2 e;
-            v[i] = mul2(v[i], normal_cdf2(split(v[i]), e));
-        }
+        for (int i = 0; i < kN; ++i) v[i] = gelu2(v[i]);
     } else if (kind == FCAI_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));
@@ -196,11 +217,7 @@ __device__ __forceinline__ void act_grad_n(int kind, const F2 (&x)[kN], F2 (&g)[
         }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) {
-            F2 e;
-            const F2 cdf = normal_cdf2(split(x[i]), e);
-            g[i] = mul2(g[i], fma2(mul2(x[i], e), f2(0.398942280f), cdf));  // Phi(x) + x phi(x)
-        }
+        for (int i = 0; i < kN; ++i) g[i] = mul2(g[i], gelu_grad2(x[i]));
     } else if (kind == FCAI_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
@@ -244,11 +261,12 @@ __device__ __forceinline__ uint32_t encode4(F2 a, F2 b, float inv) {
         const __nv_fp8x2_storage_t hi = __nv_cvt_float2_to_fp8x2(split(b), __NV_SATFINITE, __NV_E4M3);
         return (uint32_t)lo | ((uint32_t)hi << 16);
     }
-    // one at a time: a packed product and sum can come out as one fused operation, which rounds once
-    auto code = [&](float v) { return __float_as_uint(__fadd_rn(__fmul_rn(v, inv), 12582912.f)); };
-    const float2 x = split(a), y = split(b);
-    const uint32_t lo = __byte_perm(code(x.x), code(x.y), 0x0040);
-    const uint32_t hi = __byte_perm(code(y.x), code(y.y), 0x0040);
+    // The sum is written as a product with 1: a packed product and sum can come
+    // out as one fused operation, which would round once.
+    const float2 x = split(fma2(mul2(a, f2(inv)), f2(1.f), f2(12582912.f)));
+    const float2 y = split(fma2(mul2(b, f2(inv)), f2(1.f), f2(12582912.f)));
+    const uint32_t lo = __byte_perm(__float_as_uint(x.x), __float_as_uint(x.y), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(y.x), __float_as_uint(y.y), 0x0040);
     return __byte_perm(lo, hi, 0x5410);
 }
 template <bool kE4m3>

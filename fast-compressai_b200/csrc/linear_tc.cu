@@ -13,22 +13,25 @@
 // row stride is not 16-byte aligned, which TMA cannot read, is copied once
 // into the workspace with a padded stride (repack_kernel).
 //
-// CTA organisation (persistent, one CTA per SM, 18 warps; 10 with 64 columns):
-//   16 (8) warps  epilogue: TMEM -> registers -> a per-warp 32 x 32 fp32
+// CTA organisation (persistent, one CTA per SM, 18 warps):
+//   16 warps      epilogue: TMEM -> registers -> a per-warp 32 x 32 fp32
 //                 staging tile (XOR-swizzled, so both directions are free of
 //                 bank conflicts) -> bias, activation, residual and rounding
 //                 in a layout where 4 lanes cover 32 columns of a row, 16
 //                 bytes each
 //   one warp      TMA producer
 //   one warp      MMA issuer; owns the TMEM allocation
-// Two TMEM accumulators let the epilogue of a tile overlap the next mainloop.
-// Layers with short contractions are bound by the epilogue's instructions, and
-// four epilogue warps a scheduler hide its latencies where two did not.
+// Two or four TMEM accumulators let the epilogue of a tile overlap the next
+// mainloops.  Layers with short contractions are bound by the epilogue, so its
+// warps form as many groups as there are accumulators, each with every n-th
+// tile of its own: the groups are in different steps at any time, which hides
+// the latencies of one group behind the arithmetic of another.  A CTA with one
+// or two tiles in all lets every warp work on each tile instead.
 //
 // A forward product that keeps the activation's input in 8 bits makes the
-// codes here: the warps that share 128 columns of a row exchange their largest
-// magnitudes through shared memory, and the codes leave beside y, so the
-// activation's input never exists in memory in more than 8 bits.
+// codes here: a warp has whole 128-column blocks of its rows, takes their
+// largest magnitudes in a first pass over the accumulator, and the codes leave
+// beside y, so the activation's input never exists in memory in more than 8 bits.
 //
 // Work units are (tile, split): when a product has fewer tiles than SMs (few
 // rows, or a weight gradient whose long axis is the contraction), K is split
@@ -81,6 +84,7 @@ struct Params {
     int ksteps, ksteps_split;            // K steps in all and per split
     int units;
     int ldp;                             // partial tiles: row stride (N rounded up to 8)
+    int coop;                            // all epilogue warps on each tile
     int vec;                             // y, residual, pre, bias and codes take wide accesses
     int act;
     const void *bias, *residual;
@@ -97,19 +101,20 @@ template <int kBN, bool kPair>
 struct Layout {
     static constexpr int kNB = kPair ? kBN / 2 : kBN;  // rows of B this CTA stages
     static constexpr int kTileM = kPair ? 2 * kBM : kBM;
-    static constexpr int kColWarps = kBN == 64 ? 2 : 4;  // epilogue warps side by side, 32 columns each
-    static constexpr int kEpiWarps = 4 * kColWarps;
+    static constexpr int kEpiWarps = 16;
+    static constexpr int kBufs = kBN == 256 ? 2 : 4;     // accumulators, and groups of epilogue warps
+    static constexpr int kGroupWarps = kEpiWarps / kBufs;
+    static constexpr int kSpan = kBN < 128 ? kBN : 128;  // columns of a warp in a group
     static constexpr int kThreads = (kEpiWarps + 2) * 32;
     static constexpr int kA = kBM * kBK * 2;
     static constexpr int kB = kNB * kBK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = kNB == 64 ? 8 : 5;
+    static constexpr int kStages = kNB == 64 ? 6 : 5;
     static constexpr int offStaging = kStages * kStage;
     static constexpr int offBar = offStaging + kEpiWarps * kStagingWarp;
-    static constexpr int kBars = 2 * kStages + 3 * 2 + 1;
+    static constexpr int kBars = 2 * kStages + 3 * kBufs + 1;
     static constexpr int offSlot = offBar + kBars * 8;
-    static constexpr int offOk = offSlot + 16;  // per quarter and parity of the tile: a warp's wait ran out
-    static constexpr int kBytes = offOk + 32;
+    static constexpr int kBytes = offSlot + 16;
     static constexpr int kAlloc = kBytes + 1024;  // the base is rounded up to 1024
     static_assert(kAlloc <= 227 * 1024, "shared memory");
 };
@@ -235,12 +240,10 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
 }
 
 // One 32 x 32 chunk of a warp: rows [row0, row0 + 32) from the staging tile.
-// With codes the kColWarps warps of these rows all come here for each chunk
-// (whatever their columns), and meet at named barrier 1 + quarter.
-template <typename T, int kColWarps>
-__device__ __forceinline__ void write_chunk(const Params &p, uint32_t staging, int quarter, int colwarp, int row0, int col0,
-                                            int sp, int lane, const uint4 (&res)[4]) {
-    const uint32_t stg = staging + (colwarp * 4 + quarter) * kStagingWarp;
+// inv: 1 / scale of the lane's rows, for codes.
+template <typename T>
+__device__ __forceinline__ void write_chunk(const Params &p, uint32_t stg, int row0, int col0, int sp, int lane,
+                                            const uint4 (&res)[4], const float (&inv)[4]) {
     if (p.partial || p.vec) {
         const int col = col0 + (lane & 3) * 8, r0 = lane >> 2;
         const bool in = col < (p.partial ? p.ldp : p.N);  // both multiples of 8
@@ -266,30 +269,15 @@ __device__ __forceinline__ void write_chunk(const Params &p, uint32_t staging, i
             return;
         }
         if (in) add_bias8<T>(p, col, v, 4);
-        if (p.codes) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float m = in ? amax8(v + 4 * i) : 0.f;
-                m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 1));
-                m = max_nan(m, __shfl_xor_sync(0xffffffffu, m, 2));
-                // the staging tile is in registers by now (every lane's: the
-                // shuffles); its first words take the rows' magnitudes
-                if ((lane & 3) == 0) sts32(stg + (i * 8 + r0) * 4, m);
-            }
-            named_barrier_sync(1 + quarter, kColWarps * 32);
+        if (p.codes && in) {
             uint8_t *codes = p.codes + (int64_t)row * p.N + col;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                float m = 0.f;
-#pragma unroll
-                for (int w = 0; w < kColWarps; ++w) m = max_nan(m, lds32(staging + (w * 4 + quarter) * kStagingWarp + (i * 8 + r0) * 4));
-                if (!in || row + i * 8 >= p.M) continue;
-                const float s = keep_scale(p.keep, m);
+                if (row + i * 8 >= p.M) break;
                 const V8 x = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-                *reinterpret_cast<uint2 *>(codes + (int64_t)i * 8 * p.N) = keep_codes(p.keep, x, s);
-                if (colwarp == 0 && (lane & 3) == 0) p.scales[(int64_t)(row + i * 8) * p.nblk + col0 / FCAI_KEEP_BLOCK] = s;
+                *reinterpret_cast<uint2 *>(codes + (int64_t)i * 8 * p.N) =
+                    p.keep == FCAI_KEEP_E4M3 ? encode8<true>(x, inv[i]) : encode8<false>(x, inv[i]);
             }
-            named_barrier_sync(1 + quarter, kColWarps * 32);  // the magnitudes have been read
         }
         if (in) finish<T, 4>(p, row, col, v, res);
     } else {
@@ -312,19 +300,18 @@ template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
 __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
     linear_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
     using Lay = Layout<kBN, kPair>;
-    constexpr int kStages = Lay::kStages, kEpiWarps = Lay::kEpiWarps;
+    constexpr int kStages = Lay::kStages, kEpiWarps = Lay::kEpiWarps, kBufs = Lay::kBufs;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem =
         reinterpret_cast<unsigned char *>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t *full = reinterpret_cast<uint64_t *>(smem + Lay::offBar);  // pairs: rank 0's counts both CTAs' loads
     uint64_t *empty = full + kStages;
     uint64_t *accf = empty + kStages;  // accumulator filled (by the MMA warp; pairs: in both CTAs)
-    uint64_t *acce = accf + 2;         // accumulator read: one arrival per epilogue warp of this CTA
-    uint64_t *pacce = acce + 2;        // pairs, rank 0: the peer's accumulator read
-    uint64_t *dbar = pacce + 2;        // abort path: this CTA's MMAs drained
+    uint64_t *acce = accf + kBufs;     // accumulator read: one arrival per epilogue warp of this CTA that reads it
+    uint64_t *pacce = acce + kBufs;    // pairs, rank 0: the peer's accumulator read
+    uint64_t *dbar = pacce + kBufs;        // abort path: this CTA's MMAs drained
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::offSlot);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + Lay::offSlot + 4);
-    volatile int *failed = reinterpret_cast<volatile int *>(smem + Lay::offOk);
 
     const int warp = threadIdx.x >> 5;
     const int lane = threadIdx.x & 31;
@@ -332,21 +319,20 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
     const bool leader = rank == 0;
     const int unit0 = kPair ? (int)(blockIdx.x >> 1) : (int)blockIdx.x;
     const int unit_step = kPair ? (int)(gridDim.x >> 1) : (int)gridDim.x;
-    constexpr uint32_t kTmemCols = 2 * kBN;
+    constexpr uint32_t kTmemCols = kBufs * kBN;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
             mbar_init(&full[s], 1);
             mbar_init(&empty[s], 1);
         }
-        for (int b = 0; b < 2; ++b) {
+        for (int b = 0; b < kBufs; ++b) {
             mbar_init(&accf[b], 1);
-            mbar_init(&acce[b], kEpiWarps);
+            mbar_init(&acce[b], p.coop ? (kBN < 128 ? kBN / 32 * 4 : kEpiWarps) : Lay::kGroupWarps);
             mbar_init(&pacce[b], 1);
         }
         mbar_init(dbar, 1);
         *abort = 0;
-        for (int i = 0; i < 8; ++i) failed[i] = 0;
         fence_barrier_init();
     }
     if (warp == kEpiWarps + 1) {
@@ -440,9 +426,10 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             for (int unit = unit0; unit < p.units && ok; unit += unit_step, ++j) {
                 int tm, tn, sp;
                 unit_coords(p, unit, tm, tn, sp);
-                const int buf = j & 1;
-                if (!mbar_wait_warp(&acce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs) ||
-                    (kPair && !mbar_wait_warp(&pacce[buf], ((j >> 1) & 1) ^ 1, abort, kWaitNs, true))) {
+                const int buf = j % kBufs;
+                const uint32_t parity = ((j / kBufs) & 1) ^ 1;
+                if (!mbar_wait_warp(&acce[buf], parity, abort, kWaitNs) ||
+                    (kPair && !mbar_wait_warp(&pacce[buf], parity, abort, kWaitNs, true))) {
                     *abort = 1;
                     break;
                 }
@@ -483,63 +470,94 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             // stores have been seen, and the epilogue's lanes always have some.
             int j = 0;
             for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
-                if (!mbar_wait_warp(&acce[j & 1], (j >> 1) & 1, abort, kWaitNs)) {
+                if (!mbar_wait_warp(&acce[j % kBufs], (j / kBufs) & 1, abort, kWaitNs)) {
                     *abort = 1;
                     break;
                 }
-                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&pacce[j & 1]), 0));
+                if (lane == 0) mbar_arrive_cluster(mapa_shared(smem_u32(&pacce[j % kBufs]), 0));
             }
         }
         __syncwarp();
     } else {
         // ------------------------------------------------------------ epilogue
-        const int q = warp & 3, colwarp = warp >> 2;
-        const uint32_t staging = smem_u32(smem + Lay::offStaging);
-        const uint32_t stg = staging + warp * kStagingWarp + lane * 128 + ((lane & 7) << 4);  // this row's chunk 0
-        int j = 0;
-        for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
-            int tm, tn, sp;
-            unit_coords(p, unit, tm, tn, sp);
-            const int buf = j & 1;
-            const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
-            const bool wide_res = p.vec && p.residual && !p.partial;
-            uint4 res[4];  // the residual's rows: on their way while the accumulator fills
-            if (wide_res) load_residual<T, 4>(p, row0 + (lane >> 2), tn * kBN + colwarp * 32 + (lane & 3) * 8, res);
-            bool ok = mbar_wait_warp(&accf[buf], (j >> 1) & 1, abort, kWaitNs);
-            if (!ok) *abort = 1;
-            if (p.codes) {
-                // the warps that will meet inside the tile leave together: a flag
-                // per tile parity, since none gets two tiles ahead of another
-                if (!ok) failed[2 * q + buf] = 1;
-                named_barrier_sync(1 + q, Lay::kColWarps * 32);
-                ok = !failed[2 * q + buf];
-            }
-            if (!ok) break;
-            tc_fence_after();
-            const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
+        const int q = warp & 3;
+        // the warp's tiles (every jstep-th from j0 on) and its columns of each
+        const int j0 = p.coop ? 0 : warp / Lay::kGroupWarps, jstep = p.coop ? 1 : kBufs;
+        const int cbegin = p.coop ? (warp >> 2) * 32 : (warp % Lay::kGroupWarps) / 4 * 128;
+        const int cstep = p.coop ? 128 : 32, cend = p.coop ? kBN : cbegin + Lay::kSpan;
+        const uint32_t staging = smem_u32(smem + Lay::offStaging) + warp * kStagingWarp;
+        const uint32_t stg = staging + lane * 128 + ((lane & 7) << 4);  // this row's chunk 0
+        const bool wide_res = p.vec && p.residual && !p.partial;
+        if (cbegin < kBN)
+            for (int j = j0, unit = unit0 + j0 * unit_step; unit < p.units; j += jstep, unit += jstep * unit_step) {
+                int tm, tn, sp;
+                unit_coords(p, unit, tm, tn, sp);
+                const int buf = j % kBufs;
+                const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
+                const int ctile = tn * kBN;
+                uint4 res[4];  // the residual's rows: on their way while the accumulator fills
+                if (wide_res) load_residual<T, 4>(p, row0 + (lane >> 2), ctile + cbegin + (lane & 3) * 8, res);
+                if (!mbar_wait_warp(&accf[buf], (j / kBufs) & 1, abort, kWaitNs)) {
+                    *abort = 1;
+                    break;
+                }
+                tc_fence_after();
+                const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
+                float inv[4];  // codes: 1 / scale of this lane's four rows
+                if (p.codes && !p.partial && ctile + cbegin < p.N) {
+                    // first pass, a row a lane: the largest magnitude of the block;
+                    // the bias comes from the staging tile, 4 columns a load
+                    const int cb = ctile + cbegin + lane * 4;
+                    F2 b[2] = {f2(0.f), f2(0.f)};
+                    if (p.bias && lane * 4 < Lay::kSpan && cb < p.N) {
+                        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(p.bias) + cb));
+                        const float2 lo = unpack2(w.x, T()), hi = unpack2(w.y, T());
+                        b[0] = f2(lo.x, lo.y), b[1] = f2(hi.x, hi.y);
+                    }
+                    const float2 b0 = split(b[0]), b1 = split(b[1]);
+                    sts128(staging + lane * 16, __float_as_uint(b0.x), __float_as_uint(b0.y), __float_as_uint(b1.x), __float_as_uint(b1.y));
+                    __syncwarp();
+                    float m = 0.f;
 #pragma unroll 1
-            for (int c = colwarp * 32; c < kBN; c += Lay::kColWarps * 32) {
-                uint32_t v[32];
-                tmem_ld32(taddr + c, v);
-                tmem_wait_ld();
-                if (c + Lay::kColWarps * 32 >= kBN) {  // this warp has read its part of the accumulator
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&acce[buf]);
-                }
-                const int col0 = tn * kBN + c;
-                // the warps of a quarter agree on this when they have to meet for codes
-                if (row0 < p.M && (col0 < p.N || (p.codes && tn * kBN + c / (Lay::kColWarps * 32) * (Lay::kColWarps * 32) < p.N))) {
+                    for (int c = 0; c < Lay::kSpan; c += 32) {
+                        uint32_t v[32];
+                        tmem_ld32(taddr + cbegin + c, v);
+                        tmem_wait_ld();
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) sts128(stg ^ (e << 4), v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
-                    __syncwarp();
-                    write_chunk<T, Lay::kColWarps>(p, staging, q, colwarp, row0, col0, sp, lane, res);
-                    __syncwarp();
-                    if (wide_res && c + Lay::kColWarps * 32 < kBN)
-                        load_residual<T, 4>(p, row0 + (lane >> 2), col0 + Lay::kColWarps * 32 + (lane & 3) * 8, res);
+                        for (int e = 0; e < 8; ++e) {
+                            const float4 bb = lds128(staging + c * 4 + e * 16);
+                            const float2 x = split(add2(f2(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), f2(bb.x, bb.y)));
+                            const float2 y = split(add2(f2(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), f2(bb.z, bb.w)));
+                            m = max_nan(m, max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y))));
+                        }
+                    }
+                    const float s = keep_scale(p.keep, m);
+                    if (row0 + lane < p.M) p.scales[(int64_t)(row0 + lane) * p.nblk + (ctile + cbegin) / FCAI_KEEP_BLOCK] = s;
+                    const float r = __frcp_rn(s);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) inv[i] = __shfl_sync(0xffffffffu, r, i * 8 + (lane >> 2));
+                }
+#pragma unroll 1
+                for (int c = cbegin; c < cend; c += cstep) {
+                    uint32_t v[32];
+                    tmem_ld32(taddr + c, v);
+                    tmem_wait_ld();
+                    if (c + cstep >= cend) {  // this warp has read its part of the accumulator
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&acce[buf]);
+                    }
+                    if (row0 < p.M && ctile + c < p.N) {
+#pragma unroll
+                        for (int e = 0; e < 8; ++e) sts128(stg ^ (e << 4), v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        __syncwarp();
+                        write_chunk<T>(p, staging, row0, ctile + c, sp, lane, res, inv);
+                        __syncwarp();
+                        if (wide_res && c + cstep < cend)
+                            load_residual<T, 4>(p, row0 + (lane >> 2), ctile + c + cstep + (lane & 3) * 8, res);
+                    }
                 }
             }
-        }
     }
 
     // ---------------------------------------------------------------- teardown
@@ -950,6 +968,7 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     p.units = pl.tiles_m * pl.tiles_n * pl.splits;
     p.ldp = round8(N);
     p.nblk = (N + FCAI_KEEP_BLOCK - 1) / FCAI_KEEP_BLOCK;
+    p.coop = !p.codes && p.units <= 2 * (pl.pair ? fcai::sm_count() / 2 : fcai::sm_count());
     p.partial = nullptr;
     if (pl.partial_bytes) {
         p.partial = reinterpret_cast<float *>(ws);
