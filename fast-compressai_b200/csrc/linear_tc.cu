@@ -368,7 +368,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             for (int ks = sp * p.ksteps_split; ks < k1; ++ks, ++it) {
                 const int s = it % kStages;
                 const uint32_t r = it / kStages;
-                if (!mbar_wait_warp(&empty[s], (r & 1) ^ 1, abort, kWaitNs)) {
+                if (!mbar_wait_warp_idle(&empty[s], (r & 1) ^ 1, abort, kWaitNs)) {
                     *abort = 1;
                     stop = true;
                     break;
@@ -470,7 +470,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             // stores have been seen, and the epilogue's lanes always have some.
             int j = 0;
             for (int unit = unit0; unit < p.units; unit += unit_step, ++j) {
-                if (!mbar_wait_warp(&acce[j % kBufs], (j / kBufs) & 1, abort, kWaitNs)) {
+                if (!mbar_wait_warp_idle(&acce[j % kBufs], (j / kBufs) & 1, abort, kWaitNs)) {
                     *abort = 1;
                     break;
                 }
@@ -497,7 +497,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
                 const int ctile = tn * kBN;
                 uint4 res[4];  // the residual's rows: on their way while the accumulator fills
                 if (wide_res) load_residual<T, 4>(p, row0 + (lane >> 2), ctile + cbegin + (lane & 3) * 8, res);
-                if (!mbar_wait_warp(&accf[buf], (j / kBufs) & 1, abort, kWaitNs)) {
+                if (!mbar_wait_warp_idle(&accf[buf], (j / kBufs) & 1, abort, kWaitNs)) {
                     *abort = 1;
                     break;
                 }

@@ -432,6 +432,32 @@ __device__ __forceinline__ bool mbar_wait_warp(uint64_t *bar, uint32_t parity, v
     return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort, limit_ns, cluster_scope));
 }
 
+// The same for waits that are usually long (an accumulator that fills while its
+// readers idle): try_wait may suspend the thread for up to 20 us a time, so
+// that waiting warps take neither issue slots nor power from the running ones.
+__device__ __forceinline__ bool mbar_wait_warp_idle(uint64_t *bar, uint32_t parity, volatile int *abort, uint64_t limit_ns) {
+    auto test = [&]() {
+        uint32_t ok;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity), "r"(20000u)
+            : "memory");
+        return ok != 0;
+    };
+    bool ok = test();
+    if (!__all_sync(0xffffffffu, ok)) {
+        const uint64_t t0 = globaltimer();
+        for (uint32_t it = 0; !ok && it < (1u << 30); ++it) {
+            ok = test();
+            if (!ok && ((abort && *abort) || globaltimer() - t0 > limit_ns)) break;
+        }
+    }
+    return __all_sync(0xffffffffu, ok);
+}
+
 // Shared-memory matrix descriptor.  layout: 0 = no swizzle (core matrices of
 // 8 rows x 16 bytes), 2 = 128-byte swizzle.  Offsets in bytes.
 __device__ __forceinline__ uint64_t smem_desc(uint32_t saddr, uint32_t lbo, uint32_t sbo, uint32_t layout) {
