@@ -3,7 +3,9 @@
     python fast-compressai_b200/build_native.py [--force]
 
 Produces fast_compressai/_lib/libfcai_b200.so in-tree with nvcc
-(``-gencode arch=compute_100a,code=sm_100a``).  No GPU is needed to build.
+(``-gencode arch=compute_100a,code=sm_100a``) and, beside it with the host
+compiler, _layers_host.so, the module that takes the pointwise layers' calls
+from tensors to that library.  No GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -20,6 +22,8 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB_DIR = ROOT / "fast_compressai" / "_lib"
 LIB = LIB_DIR / "libfcai_b200.so"
+HOST = LIB_DIR / "_layers_host.so"
+HOST_SOURCE = "layers_host.cpp"
 
 SOURCES = [
     "warp_div.cu",
@@ -52,28 +56,67 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _inputs())
 
 
+def _host_up_to_date() -> bool:
+    if not HOST.exists():
+        return False
+    t = HOST.stat().st_mtime
+    return all(p.stat().st_mtime <= t for p in [CSRC / HOST_SOURCE, INCLUDE / "fcai_layers.h", INCLUDE / "fcai_warp_div.h"])
+
+
+def _build_host(verbose: bool) -> None:
+    """_layers_host.so, against the running interpreter and its torch."""
+    import sysconfig
+
+    import torch
+
+    root = Path(torch.__file__).resolve().parent
+    cuda = Path(_nvcc()).resolve().parents[1]
+    tmp = HOST.with_suffix(f".so.{os.getpid()}.tmp")
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+    for inc in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
+                Path(sysconfig.get_paths()["include"])):
+        cmd += ["-isystem", str(inc)]
+    cmd += [str(CSRC / HOST_SOURCE), "-o", str(tmp), "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
+            "-lc10", "-lc10_cuda", "-L", str(LIB_DIR), "-lfcai_b200", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    subprocess.run(cmd, check=True)
+    os.replace(tmp, HOST)
+
+
 def build(force: bool = False, verbose: bool = False) -> Path:
-    if not force and up_to_date():
-        return LIB
+    if force or not up_to_date():
+        _build_lib(verbose)
+    if force or not _host_up_to_date():
+        _build_host(verbose)
+    return LIB
+
+
+def _build_lib(verbose: bool) -> None:
     LIB_DIR.mkdir(parents=True, exist_ok=True)
     nvcc = _nvcc()
     objdir = ROOT / "_build"
     objdir.mkdir(exist_ok=True)
-    objs = []
-    for src in SOURCES:
+    objs, running = [], []
+    for src in SOURCES:  # the sources compile side by side
         obj = objdir / (Path(src).stem + ".o")
         cmd = [nvcc, *ARCH, *FLAGS, "-I", str(INCLUDE), "-c", str(CSRC / src), "-o", str(obj)]
         if verbose:
             print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        running.append((cmd, subprocess.Popen(cmd)))
         objs.append(str(obj))
+    for cmd, proc in running:
+        proc.wait()
+    for cmd, proc in running:
+        if proc.returncode:
+            raise subprocess.CalledProcessError(proc.returncode, cmd)
     tmp = LIB.with_suffix(f".so.{os.getpid()}.tmp")
     cmd = [nvcc, *ARCH, "-shared", "-cudart", "static", "-o", str(tmp), *objs]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
     os.replace(tmp, LIB)
-    return LIB
 
 
 def main(argv=None) -> int:

@@ -945,15 +945,14 @@ static bool wide_outputs(const Params &p, int N, int dtype) {
            (!p.residual || aligned16(p.residual, p.ldr, dtype)) && (!p.bias || aligned16(p.bias, 0, dtype)) &&
            (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
 }
-// A product with codes runs its epilogue in reduce_kernel when its rows do not
-// take wide accesses; whether they do may not change the workspace, so the size
-// is asked for as if they did not when N alone rules it out.
+// A product with codes runs its epilogue in reduce_kernel when N alone rules
+// wide accesses out (the workspace is asked for by sizes); otherwise its outputs
+// take them, which the entry point has checked.
 template <typename T, bool kTA, bool kTB>
 static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Params p, unsigned char *ws,
                cudaStream_t stream) {
     p.vec = wide_outputs(p, N, dtype);
     const bool reduce = p.codes && N % 8 != 0;
-    if (p.codes && !reduce && !p.vec) return fcai::fail(FCAI_ERR_INVALID, "linear: 8-bit codes need 16-byte aligned y, bias, residual rows, and 8-byte aligned codes");
     const Plan pl = make_plan(M, N, K, reduce, p.codes != nullptr);
     p.M = (int)M;
     p.N = N;
@@ -1093,8 +1092,6 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
         return fcai::fail(FCAI_ERR_INVALID, "linear: a row stride is smaller than its row");
     if (rows == 0) return FCAI_OK;
     if (!x || !w || !y) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
-    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, keep, workspace, workspace_bytes)))
-        return rc;
     Params p{};
     p.act = act;
     p.bias = bias;
@@ -1107,6 +1104,10 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     p.codes = k8 ? static_cast<uint8_t *>(codes) : nullptr;
     p.scales = scales;
     p.keep = keep;
+    if (k8 && rows > kFewRows && cout % 8 == 0 && !wide_outputs(p, cout, dtype))
+        return fcai::fail(FCAI_ERR_INVALID, "linear: codes need 16-byte aligned y, bias and residual rows, and 8-byte aligned codes");
+    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, keep, workspace, workspace_bytes)))
+        return rc;
     const Operand A{x, ldx, rows, cin}, B{w, ldw, cout, cin};
     auto *ws = static_cast<unsigned char *>(workspace);
     auto st = static_cast<cudaStream_t>(stream);

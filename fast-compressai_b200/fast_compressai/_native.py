@@ -7,6 +7,7 @@ fallback: if it cannot be loaded, callers get ``NativeLibraryError``.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import threading
 from pathlib import Path
 
@@ -216,6 +217,28 @@ def lib() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = handle
     return _lib
+
+
+_host = None
+
+
+def layers_host():
+    """Load (once) and return the module that takes the pointwise layers'
+    calls from tensors to the native library; the module's own name, beside it."""
+    global _host
+    if _host is None:
+        lib()  # the module links against it
+        path = LIB_PATH.with_name("_layers_host.so")
+        if not path.exists():
+            raise NativeLibraryError(f"{path} is not built; run fast-compressai_b200/build_native.py")
+        spec = importlib.util.spec_from_file_location("_layers_host", path)
+        try:
+            module = importlib.util.module_from_spec(spec)
+            spec.loader.exec_module(module)
+        except ImportError as exc:
+            raise NativeLibraryError(f"cannot load {path}: {exc}") from exc
+        _host = module
+    return _host
 
 
 def check(code: int) -> None:

@@ -60,7 +60,8 @@ def _forward(x=P, ldx=64, w=P, ldw=64, bias=None, res=None, ldr=0, y=P, ldy=32, 
     dict(dtype=F32), dict(dtype=3), dict(rows=-1), dict(rows=2 ** 31), dict(cin=0), dict(cout=0), dict(ldx=63), dict(ldw=10),
     dict(ldy=31), dict(act=4), dict(act=-1), dict(x=None), dict(w=None), dict(y=None), dict(x=P + 1), dict(res=P, ldr=8),
     dict(pre=P, ldpre=31, keep=1), dict(keep=1), dict(keep=2, codes=P), dict(keep=3, scales=P), dict(keep=4),
-    dict(keep=2, codes=P, scales=P + 2), dict(keep=2, codes=P + 4, scales=P), dict(keep=2, codes=P, scales=P, y=P + 2),
+    dict(keep=2, codes=P, scales=P + 2), dict(rows=80, keep=2, codes=P + 4, scales=P),
+    dict(rows=80, keep=2, codes=P, scales=P, y=P + 2),
 ])
 def test_linear_refusals(bad):
     assert _forward(**bad) == _native.FCAI_ERR_INVALID
