@@ -78,7 +78,7 @@ def _build_host(verbose: bool) -> None:
                 Path(sysconfig.get_paths()["include"])):
         cmd += ["-isystem", str(inc)]
     cmd += [str(CSRC / HOST_SOURCE), "-o", str(tmp), "-L", str(root / "lib"), "-ltorch_python", "-ltorch", "-ltorch_cpu",
-            "-lc10", "-lc10_cuda", "-L", str(LIB_DIR), "-lfcai_b200", "-Wl,-rpath,$ORIGIN"]
+            "-ltorch_cuda", "-lc10", "-lc10_cuda", "-L", str(LIB_DIR), "-lfcai_b200", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)

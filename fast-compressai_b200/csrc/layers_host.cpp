@@ -8,6 +8,8 @@
 // Plain CPython functions over torch's C++ tensors; every C++ exception ends in
 // a Python one.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
+#include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -82,9 +84,20 @@ bool unaligned(const void *p, int64_t ld) { return ((reinterpret_cast<uintptr_t>
 
 fcai_stream_t stream_of(const at::Tensor &t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
-at::Tensor scratch(int64_t bytes, const at::Tensor &like) {
+// A contiguous tensor on like's device, straight from the allocator (the
+// dispatcher costs as much again); the device is current.
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &like, at::ScalarType type) {
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
+}
+at::Tensor fresh(at::IntArrayRef sizes, const at::Tensor &like) { return fresh(sizes, like, like.scalar_type()); }
+// Memory for one call's kernels; back to the current stream's pool when it goes out of scope.
+struct Scratch {
+    c10::DataPtr p;
+    void *get() const { return p.get(); }
+};
+Scratch scratch(int64_t bytes) {
     if (bytes < 0) refuse("sizes out of range");
-    return bytes ? at::empty({bytes}, like.options().dtype(at::kByte)) : at::Tensor();
+    return {bytes ? c10::cuda::CUDACachingAllocator::get()->allocate((size_t)bytes) : c10::DataPtr()};
 }
 void *ptr(const at::Tensor &t) { return t.defined() ? t.data_ptr() : nullptr; }
 
@@ -92,8 +105,8 @@ struct Codes {
     at::Tensor codes, scales;
 };
 Codes new_codes(const at::Tensor &like, int64_t rows, int64_t n) {
-    return {at::empty({rows, n}, like.options().dtype(at::kByte)),
-            at::empty({rows, (n + FCAI_KEEP_BLOCK - 1) / FCAI_KEEP_BLOCK}, like.options().dtype(at::kFloat))};
+    return {fresh({rows, n}, like, at::kByte),
+            fresh({rows, (n + FCAI_KEEP_BLOCK - 1) / FCAI_KEEP_BLOCK}, like, at::kFloat)};
 }
 Codes save8(const at::Tensor &like, const Rows &m, int64_t n, int keep, void *y = nullptr, int act = 0) {
     Codes c = new_codes(like, m.rows, n);
@@ -230,7 +243,7 @@ PyObject *py_load8(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (total != codes.numel() || shape.empty() || shape.back() != c) refuse("the shape does not fit the codes");
         const at::ScalarType types[3] = {at::kBFloat16, at::kHalf, at::kFloat};
         if (dtype < 0 || dtype > 2) refuse("unknown dtype");
-        at::Tensor out = at::empty(shape, codes.options().dtype(types[dtype]));
+        at::Tensor out = fresh(shape, codes, types[dtype]);
         status(fcai_checkpoint_load(k.codes, k.scales, out.data_ptr(), c, k.m.rows, (int)c, dtype, keep, stream_of(codes)));
         return wrap(out);
     });
@@ -244,7 +257,7 @@ PyObject *py_activation_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t c = channels(x, "an activation");
         const c10::cuda::CUDAGuard guard(x.device());
         const Rows m = rows_of(x, c);
-        at::Tensor y = at::empty(x.sizes(), x.options());
+        at::Tensor y = fresh(x.sizes(), x);
         if (keep >= FCAI_KEEP_INT8) {
             const Codes k = save8(x, m, c, keep, y.data_ptr(), act);
             return wrap_all(y, k.codes, k.scales);
@@ -257,14 +270,14 @@ PyObject *py_activation_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
 
 // dx = g * act'(kept) and its column sums (either may be undefined)
 void act_backward(const at::Tensor &like, const Rows &g, int64_t n, const Kept &k, int act, const at::Tensor &dx, const at::Tensor &sums) {
-    at::Tensor ws;
+    Scratch ws;
     int64_t bytes = 0;
     if (sums.defined()) {
         bytes = fcai_activation_workspace(g.rows, (int)n);
-        ws = scratch(bytes, like);
+        ws = scratch(bytes);
     }
     status(fcai_activation_backward(g.p, g.ld, k.m.p, k.m.ld, k.codes, k.scales, ptr(dx), n, ptr(sums), g.rows, (int)n,
-                                    dtype_code(like, "an activation"), act, k.keep, ptr(ws), bytes, stream_of(like)));
+                                    dtype_code(like, "an activation"), act, k.keep, ws.get(), bytes, stream_of(like)));
 }
 
 // activation_backward(grad, kept or codes, scales, keep, act) -> dx
@@ -278,7 +291,7 @@ PyObject *py_activation_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Kept k = kept_of(a[1], a[2], keep, c);
         if (k.m.rows != g.rows) refuse("grad does not fit what was kept");
         if (keep < FCAI_KEEP_INT8) same(grad, "grad", THPVariable_Unpack(a[1]));
-        at::Tensor dx = at::empty(grad.sizes(), grad.options());
+        at::Tensor dx = fresh(grad.sizes(), grad);
         act_backward(grad, g, c, k, act, dx, at::Tensor());
         return wrap(dx);
     });
@@ -321,10 +334,10 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
             r = rows_of(res, cout);
         }
         const Rows m = rows_of(x, cin), wm = rows_of(w, cin);
-        at::Tensor y = at::empty(shape, x.options()), pre;
+        at::Tensor y = fresh(shape, x), pre;
         Codes k;
         const int kp = act == FCAI_ACT_NONE ? FCAI_KEEP_NONE : keep;  // what of the activation's input is kept
-        if (kp == FCAI_KEEP_FULL) pre = at::empty(shape, x.options());
+        if (kp == FCAI_KEEP_FULL) pre = fresh(shape, x);
         if (kp >= FCAI_KEEP_INT8) {
             k = new_codes(x, m.rows, cout);
             if (cout % 8 == 0) {  // the codes leave with y's rows, in wide accesses
@@ -338,10 +351,10 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         }
         const int repack = (unaligned(m.p, m.ld) ? 1 : 0) | (unaligned(wm.p, wm.ld) ? 2 : 0);
         const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_FORWARD, m.rows, (int)cin, (int)cout, repack, kp);
-        const at::Tensor ws = scratch(bytes, x);
+        const Scratch ws = scratch(bytes);
         status(fcai_linear_forward(m.p, m.ld, wm.p, wm.ld, ptr(bias), r.p, r.ld, y.data_ptr(), cout, ptr(pre), cout, ptr(k.codes),
                                    static_cast<float *>(ptr(k.scales)), m.rows, (int)cin, (int)cout, dtype_code(x, "linear"), act, kp,
-                                   ptr(ws), bytes, stream_of(x)));
+                                   ws.get(), bytes, stream_of(x)));
         if (keep == FCAI_KEEP_NONE) return wrap(y);
         if (keep == FCAI_KEEP_FULL) return wrap_all(y, pre);
         const Codes kx = save8(x, m, cin, keep);
@@ -365,11 +378,11 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const Kept x = kept_of(a[2], a[3], keep, cin);
         if (x.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
         at::Tensor dx, dw, db, dp;
-        if (needs & 4) db = at::empty({cout}, grad.options());
+        if (needs & 4) db = fresh({cout}, grad);
         if (act != FCAI_ACT_NONE) {
             const Kept p = kept_of(a[4], a[5], keep, cout);
             if (p.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
-            dp = at::empty({g.rows, cout}, grad.options());
+            dp = fresh({g.rows, cout}, grad);
             act_backward(grad, g, cout, p, act, dp, db);
             g = Rows{dp, dp.data_ptr(), cout, g.rows};
         } else if (needs & 4) {
@@ -379,19 +392,19 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (needs & 1) {
             at::DimVector shape(grad.sizes().begin(), grad.sizes().end());
             shape.back() = cin;
-            dx = at::empty(shape, grad.options());
+            dx = fresh(shape, grad);
             const Rows wm = rows_of(w, cin);
             const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_BACKWARD_INPUT, g.rows, (int)cin, (int)cout,
                                                         gpack | (unaligned(wm.p, wm.ld) ? 2 : 0), 0);
-            const at::Tensor ws = scratch(bytes, grad);
-            status(fcai_linear_backward_input(g.p, g.ld, wm.p, wm.ld, dx.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ptr(ws),
+            const Scratch ws = scratch(bytes);
+            status(fcai_linear_backward_input(g.p, g.ld, wm.p, wm.ld, dx.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ws.get(),
                                               bytes, st));
         }
         if (needs & 2) {
-            dw = at::empty({cout, cin}, grad.options());
+            dw = fresh({cout, cin}, grad);
             Rows m = x.m;
             if (keep >= FCAI_KEEP_INT8) {
-                at::Tensor v = at::empty({x.m.rows, cin}, grad.options());
+                at::Tensor v = fresh({x.m.rows, cin}, grad);
                 status(fcai_checkpoint_load(x.codes, x.scales, v.data_ptr(), cin, x.m.rows, (int)cin, dtype, keep, st));
                 const void *p = v.data_ptr();
                 m = Rows{std::move(v), p, cin, x.m.rows};
@@ -400,8 +413,8 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
             }
             const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, g.rows, (int)cin, (int)cout,
                                                         gpack | (unaligned(m.p, m.ld) ? 2 : 0), 0);
-            const at::Tensor ws = scratch(bytes, grad);
-            status(fcai_linear_backward_weight(g.p, g.ld, m.p, m.ld, dw.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ptr(ws),
+            const Scratch ws = scratch(bytes);
+            status(fcai_linear_backward_weight(g.p, g.ld, m.p, m.ld, dw.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ws.get(),
                                                bytes, st));
         }
         return wrap_all(dx, dw, db);
@@ -436,11 +449,11 @@ PyObject *py_layer_norm_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const at::Tensor &any = w.defined() ? w : b;
         const int wdtype = any.defined() ? dtype_code(any, "layer_norm") : dtype;
         const Rows m = rows_of(x, c);
-        at::Tensor y = at::empty(x.sizes(), x.options()), stats;
+        at::Tensor y = fresh(x.sizes(), x), stats;
         Codes k;
         float *mean = nullptr, *rstd = nullptr;
         if (keep != FCAI_KEEP_NONE) {
-            stats = at::empty({2, m.rows}, x.options().dtype(at::kFloat));
+            stats = fresh({2, m.rows}, x, at::kFloat);
             mean = stats.data_ptr<float>();
             rstd = mean + m.rows;
         }
@@ -470,17 +483,17 @@ PyObject *py_layer_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (keep < FCAI_KEEP_INT8) same(grad, "grad", THPVariable_Unpack(a[1]));
         const at::Tensor w = affine(a[4], "weight", grad, c);
         if (w.defined() && dtype_code(w, "layer_norm") != wdtype) refuse("layer_norm: weight has another dtype than in the forward call");
-        const auto wopt = grad.options().dtype(wdtype == FCAI_DTYPE_F32 ? at::kFloat : grad.scalar_type());
+        const at::ScalarType wt = wdtype == FCAI_DTYPE_F32 ? at::kFloat : grad.scalar_type();
         at::Tensor dx, dw, db;
-        if (needs & 1) dx = at::empty(grad.sizes(), grad.options());
-        if (needs & 2) dw = at::empty({c}, wopt);
-        if (needs & 4) db = at::empty({c}, wopt);
+        if (needs & 1) dx = fresh(grad.sizes(), grad);
+        if (needs & 2) dw = fresh({c}, grad, wt);
+        if (needs & 4) db = fresh({c}, grad, wt);
         if (needs & 7) {
             const int64_t bytes = fcai_layer_norm_workspace(g.rows, (int)c);
-            const at::Tensor ws = scratch(bytes, grad);
+            const Scratch ws = scratch(bytes);
             const float *mean = stats.data_ptr<float>();
             status(fcai_layer_norm_backward(g.p, g.ld, x.m.p, x.m.ld, x.codes, x.scales, mean, mean + g.rows, ptr(w), wdtype, ptr(dx), c,
-                                            ptr(dw), ptr(db), g.rows, (int)c, dtype, x.keep, ptr(ws), bytes, stream_of(grad)));
+                                            ptr(dw), ptr(db), g.rows, (int)c, dtype, x.keep, ws.get(), bytes, stream_of(grad)));
         }
         return wrap_all(dx, dw, db);
     });

@@ -284,10 +284,29 @@ __device__ __forceinline__ void write_chunk(const Params &p, uint32_t stg, int r
         const int col = col0 + lane;
         if (col >= p.N) return;
         const float bias = p.bias ? to_f32(static_cast<const T *>(p.bias)[col]) : 0.f;
-#pragma unroll 4
-        for (int r = 0; r < 32; ++r) {
-            if (row0 + r >= p.M) break;
-            finish1<T>(p, row0 + r, col, lds32(stg + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) + (lane & 3) * 4) + bias);
+        // eight rows' residuals at a time are on their way before the first is used
+#pragma unroll 1
+        for (int r = 0; r < 32 && row0 + r < p.M; r += 8) {
+            const int left = p.M - row0 - r;
+            float res[8], v[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                res[e] = p.residual && e < left ? to_f32(static_cast<const T *>(p.residual)[(row0 + r + e) * p.ldr + col]) : 0.f;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+                v[e] = lds32(stg + (r + e) * 128 + (((lane >> 2) ^ e) << 4) + (lane & 3) * 4) + bias;
+            if (p.pre) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (e < left) static_cast<T *>(p.pre)[(row0 + r + e) * p.ldpre + col] = from_f32<T>(v[e]);
+            }
+            F2 w[4] = {f2(v[0], v[1]), f2(v[2], v[3]), f2(v[4], v[5]), f2(v[6], v[7])};
+            act_n(p.act, w);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float2 f = split(w[e / 2]);
+                if (e < left) static_cast<T *>(p.y)[(row0 + r + e) * p.ldy + col] = from_f32<T>((e & 1 ? f.y : f.x) + res[e]);
+            }
         }
     }
 }
@@ -990,9 +1009,9 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
 constexpr int kFewRows = 32;
 template <typename T, int kNB, bool kV>
 static int launch_few(const FewRows &f, const Params &p, cudaStream_t stream) {
-    // fewer column groups than SMs: more warps share a group's K
+    // long rows: more warps share a group's K, so that about all of w is in flight at once
     const int grid = (p.N + 15) / 16;
-    if (grid >= fcai::sm_count() || f.K < 2048) few_rows_kernel<T, kNB, 8, kV><<<grid, 256, 0, stream>>>(f, p);
+    if (f.K < 2048) few_rows_kernel<T, kNB, 8, kV><<<grid, 256, 0, stream>>>(f, p);
     else few_rows_kernel<T, kNB, 16, kV><<<grid, 512, 0, stream>>>(f, p);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;

@@ -8,6 +8,13 @@
 //     in registers, meet in shared memory, and leave as one partial row per
 //     CTA, which colsum_kernel adds in a fixed order (the same bits every run);
 //   * rows: a CTA takes whole rows, for sums over channels.
+//
+// Both read through a ring of shared memory that cp.async fills, every thread
+// its own 16 bytes a row, several rows ahead of the one it works on: what is in
+// flight costs no registers, needs no barrier, and never drains while a row is
+// worked on (with the next rows in registers instead, too few bytes were in
+// flight: 3.3 to 4.7 TB/s).  Rows that do not take 16-byte accesses keep the
+// next row in registers.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -21,7 +28,6 @@ using namespace ly;
 constexpr int kThreads = 256;
 constexpr int kBlock = FCAI_KEEP_BLOCK;
 constexpr int kRowsIter = kThreads / 16;  // rows a strip CTA handles at a time
-constexpr int kUnroll = 2;                // rows a strip thread has in flight
 
 // The eight channels a thread holds of its group's 8 * g: consecutive ones where
 // rows take 16-byte accesses (kV), else every g-th, so that neighbouring lanes
@@ -180,6 +186,88 @@ struct KeptRaw {
     }
 };
 
+// ---- rows in flight ----------------------------------------------------------
+template <int kBytes>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void *src, bool in) {
+    const uint64_t g = __cvta_generic_to_global(src);
+    if constexpr (kBytes == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(g), "r"(in ? 16 : 0) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2, %3;" ::"r"(dst), "l"(g), "n"(kBytes), "r"(in ? kBytes : 0) : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int kPending>
+__device__ __forceinline__ void cp_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kPending) : "memory");
+}
+constexpr int kRingBytes = 32768;  // a CTA's ring at most
+
+// kCta threads, kPer chunks of 8 values a thread and step; kAsync: through the
+// ring at `base`, else the next step waits in registers.
+template <typename T, bool kV, bool kAsync, int kCta, int kPer>
+struct RowFeed {
+    static constexpr int kPieces = sizeof(T) / 2;
+    static constexpr int kStep = kPer * kPieces * kCta * 16;  // ring bytes a step
+    Raw8<T, kV> reg[kAsync ? 1 : kPer];
+    __device__ __forceinline__ void issue(uint32_t base, int i, const T *m, int64_t offset, const Cols<kV> &c, int n, bool in) {
+        if constexpr (kAsync) {
+            const bool ok = in && c.first < n;
+            const T *src = ok ? m + offset + c.first : m;
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+                cp_async<16>(base + ((i * kPieces + q) * kCta + threadIdx.x) * 16, src + (ok ? q * (16 / (int)sizeof(T)) : 0), ok);
+        } else {
+            reg[i].load(m + offset, c, n, in);
+        }
+    }
+    __device__ __forceinline__ Raw8<T, kV> get(uint32_t base, int i) const {
+        if constexpr (kAsync) {
+            Raw8<T, kV> r;
+#pragma unroll
+            for (int q = 0; q < kPieces; ++q)
+                asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(r.w[4 * q]), "=r"(r.w[4 * q + 1]), "=r"(r.w[4 * q + 2]), "=r"(r.w[4 * q + 3])
+                             : "r"(base + ((i * kPieces + q) * kCta + threadIdx.x) * 16)
+                             : "memory");
+            return r;
+        } else {
+            return reg[i];
+        }
+    }
+};
+template <typename T, bool kV, bool k8, bool kAsync, int kCta, int kPer>
+struct KeptFeed {
+    using Values = RowFeed<T, kV, kAsync, kCta, kPer>;
+    static constexpr int kStep = k8 ? kPer * kCta * 12 : Values::kStep;
+    Values x;
+    KeptRaw<T, kV, true> reg[kAsync || !k8 ? 1 : kPer];
+    __device__ __forceinline__ void issue(uint32_t base, int i, const Kept &k, int64_t row, const Cols<kV> &c, int n, int nblk, bool in) {
+        if constexpr (!k8) {
+            x.issue(base, i, static_cast<const T *>(k.x), row * k.ldx, c, n, in);
+        } else if constexpr (kAsync) {
+            const bool ok = in && c.first < n;
+            cp_async<8>(base + (i * kCta + threadIdx.x) * 8, ok ? k.codes + row * n + c.first : k.codes, ok);
+            cp_async<4>(base + kPer * kCta * 8 + (i * kCta + threadIdx.x) * 4, ok ? k.scales + row * nblk + c.first / kBlock : k.scales, ok);
+        } else {
+            reg[i].load(k, row, c, n, nblk, in);
+        }
+    }
+    __device__ __forceinline__ KeptRaw<T, kV, k8> get(uint32_t base, int i) const {
+        KeptRaw<T, kV, k8> r;
+        if constexpr (!k8) {
+            r.x = x.get(base, i);
+        } else if constexpr (kAsync) {
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(r.q.x), "=r"(r.q.y) : "r"(base + (i * kCta + threadIdx.x) * 8) : "memory");
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(r.s) : "r"(base + kPer * kCta * 8 + (i * kCta + threadIdx.x) * 4) : "memory");
+        } else {
+            r = reg[i];
+        }
+        return r;
+    }
+};
+// Steps in flight: as many as the ring holds, at most four.
+constexpr int ring_depth(int step_bytes) { return step_bytes * 4 <= kRingBytes ? 4 : step_bytes * 2 <= kRingBytes ? kRingBytes / step_bytes : 1; }
+
 // A block's codes and scale, from the kLanes (at most 16) lanes that hold its
 // channels, 8 each (amax: the lane's own); the whole warp calls it.
 template <int kLanes, bool kV>
@@ -206,44 +294,51 @@ template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
     act_forward_kernel(const T *__restrict__ x, int64_t ldx, T *__restrict__ y, int64_t ldy, uint8_t *__restrict__ codes,
                        float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep) {
+    using Feed = RowFeed<T, kV, kV, kThreads, 1>;
+    constexpr int kD = kV ? ring_depth(Feed::kStep) : 1;
+    __shared__ __align__(16) unsigned char ring[kV ? kD * Feed::kStep : 16];
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring);
     const int strip = blockIdx.x;
     const Cols<kV> c(strip * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.y * kRowsIter;
     const int sub = (threadIdx.x >> 4) & 1;
     // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
-    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 5) * 2; r0 < rows; r0 += step * kUnroll) {
-        Raw8<T, kV> raw[kUnroll];
+    int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 5) * 2;
+    Feed feed;
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t row = r0 + u * step + sub;
-            raw[u].load(x + row * ldx, c, n, row < rows);
-        }
-#pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t row = r0 + u * step + sub;
-            const bool in = row < rows;
-            if (r0 + u * step >= rows) break;
-            V8 v = raw[u].get();
-            if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, raw[u].amax(), v, codes + row * n, scales + row * nblk + strip, c, n, in);
-            if (y) {
-                act_n(act, v.p);
-                store8(y + row * ldy, c, n, in, v);
-            }
+    for (int d = 0; d < kD; ++d) {
+        feed.issue(base + d * Feed::kStep, 0, x, (r0 + d * step + sub) * ldx, c, n, r0 + d * step + sub < rows);
+        cp_commit();
+    }
+    for (int slot = 0; r0 < rows; r0 += step, slot = slot + 1 == kD ? 0 : slot + 1) {
+        cp_wait<kD - 1>();
+        const Raw8<T, kV> raw = feed.get(base + slot * Feed::kStep, 0);
+        V8 v = raw.get();
+        const int64_t row = r0 + sub;
+        const bool in = row < rows;
+        if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, raw.amax(), v, codes + row * n, scales + row * nblk + strip, c, n, in);
+        feed.issue(base + slot * Feed::kStep, 0, x, (row + kD * step) * ldx, c, n, row + kD * step < rows);
+        cp_commit();
+        if (y) {
+            act_n(act, v.p);
+            store8(y + row * ldy, c, n, in, v);
         }
     }
+    cp_wait<0>();
 }
 
+constexpr int kLoadRows = 2;  // rows a thread has in flight: 8 + 4 bytes a row are too little for the ring to pay
 template <typename T, bool kV>
 __global__ void __launch_bounds__(kThreads, kV ? 6 : 4)
     checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
     const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.y * kRowsIter;
-    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
-        KeptRaw<T, kV, true> raw[kUnroll];
+    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kLoadRows) {
+        KeptRaw<T, kV, true> raw[kLoadRows];
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) raw[u].load(k, r0 + u * step, c, n, nblk, r0 + u * step < rows);
+        for (int u = 0; u < kLoadRows; ++u) raw[u].load(k, r0 + u * step, c, n, nblk, r0 + u * step < rows);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
+        for (int u = 0; u < kLoadRows; ++u) {
             if (r0 + u * step >= rows) break;
             store8(out + (r0 + u * step) * ldo, c, n, true, raw[u].get(k));
         }
@@ -272,60 +367,67 @@ __device__ __forceinline__ void group_sums(const V8 &sums, float *partial_row, i
     }
 }
 
-// dx = dy act'(x) and partial sums of it over the CTA's rows
-template <typename T, bool kV, bool k8>
+// dx = dy act'(x) and partial sums of it over the CTA's rows; kAct: x is read
+template <typename T, bool kV, bool k8, bool kAct>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
                         float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
-    __shared__ float sh[kThreads * 8];
+    using FeedG = RowFeed<T, kV, kV, kThreads, 1>;
+    using FeedX = KeptFeed<T, kV, k8, kV, kThreads, 1>;
+    constexpr int kStep = FeedG::kStep + (kAct ? FeedX::kStep : 0);
+    constexpr int kD = kV ? ring_depth(kStep) : 1;
+    constexpr int kSums = kThreads * 8 * 4;
+    // the sums meet in the ring's memory when the rows are through
+    __shared__ __align__(16) unsigned char ring[kV && kD * kStep > kSums ? kD * kStep : kSums];
+    const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring);
     const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
     const int64_t step = (int64_t)gridDim.y * kRowsIter;
     V8 acc = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
-    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kUnroll) {
-        Raw8<T, kV> raw_g[kUnroll];
-        KeptRaw<T, kV, k8> raw[kUnroll];
+    int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4);
+    FeedG feed_g;
+    FeedX feed_x;
+    auto issue = [&](int slot, int64_t r) {
+        feed_g.issue(base + slot * kStep, 0, dy, r * lddy, c, n, r < rows);
+        if (kAct) feed_x.issue(base + slot * kStep + FeedG::kStep, 0, k, r, c, n, nblk, r < rows);
+        cp_commit();
+    };
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t row = r0 + u * step;
-            raw_g[u].load(dy + row * lddy, c, n, row < rows);
-            if (act != FCAI_ACT_NONE) raw[u].load(k, row, c, n, nblk, row < rows);
-        }
+    for (int d = 0; d < kD; ++d) issue(d, row + d * step);
+    for (int slot = 0; row < rows; row += step, slot = slot + 1 == kD ? 0 : slot + 1) {
+        cp_wait<kD - 1>();
+        V8 g = feed_g.get(base + slot * kStep, 0).get(), x;
+        if (kAct) x = feed_x.get(base + slot * kStep + FeedG::kStep, 0).get(k);
+        issue(slot, row + kD * step);
+        if (kAct) act_grad_n(act, x.p, g.p);
+        if (dx) store8(dx + row * lddx, c, n, true, g);
 #pragma unroll
-        for (int u = 0; u < kUnroll; ++u) {
-            const int64_t row = r0 + u * step;
-            if (row >= rows) break;
-            V8 g = raw_g[u].get();
-            if (act != FCAI_ACT_NONE) {
-                const V8 x = raw[u].get(k);
-                act_grad_n(act, x.p, g.p);
-            }
-            if (dx) store8(dx + row * lddx, c, n, true, g);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc.p[i] = add2(acc.p[i], g.p[i]);
-        }
+        for (int i = 0; i < 4; ++i) acc.p[i] = add2(acc.p[i], g.p[i]);
     }
-    if (partial) group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, sh);
+    cp_wait<0>();
+    if (partial) {
+        group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, reinterpret_cast<float *>(ring));
+    }
 }
 
 // Column sums of partial[rows][stride], in a fixed order: columns [0, n0) to
-// out0, [n0, n0 + n1) to out1.  32 columns a CTA, 16 threads down the rows.
+// out0, [n0, n0 + n1) to out1.  32 columns a CTA, 32 threads down the rows.
 template <typename T>
-__global__ void __launch_bounds__(512)
+__global__ void __launch_bounds__(1024)
     colsum_kernel(const float *__restrict__ partial, int rows, int64_t stride, T *__restrict__ out0, int n0, T *__restrict__ out1,
                   int n1) {
-    __shared__ float sh[16][33];
+    __shared__ float sh[32][33];
     const int col = blockIdx.x * 32 + threadIdx.x;
     float s = 0.f;
     if (col < n0 + n1) {
 #pragma unroll 8
-        for (int r = threadIdx.y; r < rows; r += 16) s += partial[r * stride + col];
+        for (int r = threadIdx.y; r < rows; r += 32) s += partial[r * stride + col];
     }
     sh[threadIdx.y][threadIdx.x] = s;
     __syncthreads();
     if (threadIdx.y == 0 && col < n0 + n1) {
         s = 0.f;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s += sh[i][threadIdx.x];
+        for (int i = 0; i < 32; ++i) s += sh[i][threadIdx.x];
         if (col < n0) {
             if (out0) out0[col] = from_f32<T>(s);
         } else if (out1) {
@@ -483,7 +585,7 @@ __global__ void __launch_bounds__(Group<kLanes>::kCta, norm_ctas(kLanes, kChunks
         for (int u = 0; u < kRows; ++u) {
             const int64_t row = r0 + u * G::kGroups + sub;
             const bool in = row < rows;
-            const float rs = 1.f / sqrtf(fmaf(rstd[u], inv_n, eps));
+            const float rs = rsqrtf(fmaf(rstd[u], inv_n, eps));
             if (mean_out && in && threadIdx.x % kLanes == 0) {
                 mean_out[row] = mean[u];
                 rstd_out[row] = rs;
@@ -748,14 +850,13 @@ static int64_t round256(int64_t v) { return (v + 255) / 256 * 256; }
 static int blocks_of(int n) { return (n + kBlock - 1) / kBlock; }
 static bool codes_vec(const void *codes, int n) { return !codes || ((reinterpret_cast<uintptr_t>(codes) & 7) == 0 && n % 8 == 0); }
 
-// Row shares of the strip kernels.  Without sums over rows: shares of kUnroll
-// steps, so that every thread has its kUnroll rows in flight once.  With sums:
-// about 8 CTAs per SM in all, since every share leaves a partial row.
-static int row_shares(int64_t rows, int strips, bool sums) {
+// Row shares of the strip kernels: enough CTAs to fill the device, and from
+// there on CTAs of 16 steps of 16 rows, long enough for the ring to run full and
+// for partial sums to be few, short enough to end evenly.
+static int row_shares(int64_t rows, int strips) {
     const int64_t steps = (rows + kRowsIter - 1) / kRowsIter;
-    const int64_t fill = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 8 + strips - 1) / strips);
-    if (sums || steps <= fill) return (int)std::min<int64_t>({steps, fill, 65535});
-    return (int)std::min<int64_t>(std::max(fill, (steps + kUnroll - 1) / kUnroll), 65535);
+    const int64_t fill = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 4 + strips - 1) / strips);
+    return (int)std::min<int64_t>(steps <= fill ? steps : std::max(fill, (steps + 15) / 16), 65535);
 }
 // How the layer norm runs rows of n channels: threads a row, 8-channel chunks a thread.
 struct Held {
@@ -780,12 +881,12 @@ static int norm_backward_grid(int64_t rows, int n) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
 }
 static int64_t act_workspace(int64_t rows, int n) {
-    return rows ? round256((int64_t)row_shares(rows, blocks_of(n), true) * n * 4) : 0;
+    return rows ? round256((int64_t)row_shares(rows, blocks_of(n)) * n * 4) : 0;
 }
 static int64_t norm_workspace(int64_t rows, int n) {
     if (rows == 0) return 0;
     if (n <= kMaxHeld) return round256((int64_t)norm_backward_grid(rows, n) * 2 * n * 4);
-    return round256(rows * 8) + round256((int64_t)row_shares(rows, blocks_of(n), true) * 2 * n * 4);
+    return round256(rows * 8) + round256((int64_t)row_shares(rows, blocks_of(n)) * 2 * n * 4);
 }
 
 static int check_sizes(const char *op, int64_t rows, int n, int dtype) {
@@ -816,7 +917,7 @@ static int check_ws(const char *op, int64_t need, const void *ws, int64_t bytes)
 }
 static int colsum(const float *partial, int rows, int64_t stride, void *out0, int n0, void *out1, int n1, int dtype,
                   cudaStream_t st) {
-    const dim3 block(32, 16);
+    const dim3 block(32, 32);
     const int grid = (n0 + n1 + 31) / 32;
     if (dtype == FCAI_DTYPE_BF16)
         colsum_kernel<<<grid, block, 0, st>>>(partial, rows, stride, static_cast<__nv_bfloat16 *>(out0), n0, static_cast<__nv_bfloat16 *>(out1), n1);
@@ -835,7 +936,7 @@ static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *c
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
     const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
     const int strips = blocks_of(n);
-    const dim3 grid(strips, row_shares(rows, strips, false));
+    const dim3 grid(strips, row_shares(rows, strips));
     auto kernel = vec ? act_forward_kernel<T, true> : act_forward_kernel<T, false>;
     kernel<<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales,
                                       rows, n, strips, act, q ? keep : FCAI_KEEP_NONE);
@@ -845,12 +946,13 @@ static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *c
 template <typename T>
 static int act_backward(const void *dy, int64_t lddy, const Kept &k, void *dx, int64_t lddx, void *bias_grad, int64_t rows, int n,
                         int dtype, int act, float *ws, cudaStream_t st) {
-    const int strips = blocks_of(n), shares = row_shares(rows, strips, bias_grad != nullptr);
+    const int strips = blocks_of(n), shares = row_shares(rows, strips);
     const bool k8 = act != FCAI_ACT_NONE && k.keep != FCAI_KEEP_FULL;
     const bool vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
                      (act == FCAI_ACT_NONE || (k8 ? codes_vec(k.codes, n) : aligned16(k.x, k.ldx, dtype)));
-    auto kernel = k8 ? (vec ? act_backward_kernel<T, true, true> : act_backward_kernel<T, false, true>)
-                     : (vec ? act_backward_kernel<T, true, false> : act_backward_kernel<T, false, false>);
+    auto kernel = act == FCAI_ACT_NONE ? (vec ? act_backward_kernel<T, true, false, false> : act_backward_kernel<T, false, false, false>)
+                  : k8 ? (vec ? act_backward_kernel<T, true, true, true> : act_backward_kernel<T, false, true, true>)
+                       : (vec ? act_backward_kernel<T, true, false, true> : act_backward_kernel<T, false, false, true>);
     kernel<<<dim3(strips, shares), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
                                                       bias_grad ? ws : nullptr, rows, n, strips, act);
     FCAI_CUDA_TRY(cudaGetLastError());
@@ -861,7 +963,7 @@ static int load_checkpoint(const Kept &k, void *out, int64_t ldo, int64_t rows, 
     const bool vec = n % 8 == 0 && aligned16(out, ldo, dtype) && codes_vec(k.codes, n);
     const int strips = blocks_of(n);
     auto kernel = vec ? checkpoint_load_kernel<T, true> : checkpoint_load_kernel<T, false>;
-    kernel<<<dim3(strips, row_shares(rows, strips, false)), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
+    kernel<<<dim3(strips, row_shares(rows, strips)), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
@@ -877,7 +979,7 @@ struct NormForward {
 };
 template <typename T, bool kV, bool k8, int kLanes, int kChunks>
 static int launch_norm_forward(const NormForward &a) {
-    constexpr int kRows = kLanes > 32 ? (kChunks == 1 && !k8 ? 2 : 1) : 2 / kChunks;
+    constexpr int kRows = kLanes > 32 ? (kChunks == 1 && !k8 ? 2 : 1) : kChunks == 1 ? 2 : 1;
     constexpr int64_t kPerCta = (int64_t)Group<kLanes>::kGroups * kRows;
     const int64_t want = (a.rows + kPerCta - 1) / kPerCta;
     const int grid = (int)std::min<int64_t>(want, (int64_t)fcai::sm_count() * (kLanes > 32 ? std::max(1, 1024 / kLanes) : 6));
@@ -976,7 +1078,7 @@ static int norm_backward(const void *dy, int64_t lddy, const Kept &k, const floa
     if (n > kMaxHeld) {
         stats = reinterpret_cast<float2 *>(ws);
         ws += round256(rows * 8);
-        parts = row_shares(rows, blocks_of(n), true);
+        parts = row_shares(rows, blocks_of(n));
     }
     float *partial = dweight || dbias ? reinterpret_cast<float *>(ws) : nullptr;
     const NormBackward a{dy, lddy, lddx, rows, k, mean, rstd, af, dx, partial, n, st};
