@@ -14,11 +14,14 @@
 // into the workspace with a padded stride (repack_kernel).
 //
 // CTA organisation (persistent, one CTA per SM, 18 warps):
-//   16 warps      epilogue: TMEM -> registers -> a per-warp 32 x 32 fp32
-//                 staging tile (XOR-swizzled, so both directions are free of
-//                 bank conflicts) -> bias, activation, residual and rounding
-//                 in a layout where 4 lanes cover 32 columns of a row, 16
-//                 bytes each
+//   16 warps      epilogue: a row of the tile a lane, 32 columns at a time, from
+//                 TMEM to bias, activation, residual and rounding; the 32 x 32
+//                 results go to a swizzled tile in shared memory and from there
+//                 by TMA (which also brought the residual's into the same
+//                 tile).  The first form moved fp32 values through shared memory
+//                 to store them from registers, and shared memory's bandwidth,
+//                 which the MMA's operands need too, was what bounded layers
+//                 with short contractions.
 //   one warp      TMA producer
 //   one warp      MMA issuer; owns the TMEM allocation
 // Two or four TMEM accumulators let the epilogue of a tile overlap the next
@@ -62,7 +65,8 @@ using namespace ly;
 
 constexpr int kBM = 128;            // tile rows of one CTA
 constexpr int kBK = 64;             // K per ring stage: one 128-byte swizzled row
-constexpr int kStagingWarp = 32 * 32 * 4;
+constexpr int kTileBytes = 32 * 32 * 2;       // a 32 x 32 tile of results
+constexpr int kStagingWarp = 2 * kTileBytes;  // two of them, or one of fp32 values
 constexpr uint64_t kWaitNs = 1000000000ull;
 
 // Division of n < 2^31 by a divisor known on the host (Granlund and Montgomery,
@@ -96,8 +100,9 @@ struct Params {
     int nblk, keep;
 };
 
-// A tile is kPair ? 256 : 128 rows by kBN columns.
-template <int kBN, bool kPair>
+// A tile is kPair ? 256 : 128 rows by kBN columns.  kKeep: what a backward pass
+// needs leaves too, through a third tile of each epilogue warp.
+template <int kBN, bool kPair, bool kKeep>
 struct Layout {
     static constexpr int kNB = kPair ? kBN / 2 : kBN;  // rows of B this CTA stages
     static constexpr int kTileM = kPair ? 2 * kBM : kBM;
@@ -109,10 +114,11 @@ struct Layout {
     static constexpr int kA = kBM * kBK * 2;
     static constexpr int kB = kNB * kBK * 2;
     static constexpr int kStage = kA + kB;
-    static constexpr int kStages = kNB == 64 ? 6 : 5;
+    static constexpr int kStages = kNB == 64 ? (kKeep ? 5 : 6) : (kKeep ? 4 : 5);
     static constexpr int offStaging = kStages * kStage;
-    static constexpr int offBar = offStaging + kEpiWarps * kStagingWarp;
-    static constexpr int kBars = 2 * kStages + 3 * kBufs + 1;
+    static constexpr int kWarpTile = kStagingWarp + (kKeep ? kTileBytes : 0);
+    static constexpr int offBar = offStaging + kEpiWarps * kWarpTile;
+    static constexpr int kBars = 2 * kStages + 3 * kBufs + 1 + 2 * kEpiWarps;
     static constexpr int offSlot = offBar + kBars * 8;
     static constexpr int kBytes = offSlot + 16;
     static constexpr int kAlloc = kBytes + 1024;  // the base is rounded up to 1024
@@ -171,41 +177,6 @@ __device__ __forceinline__ void unpack8(const uint4 &q, F2 *v) {
     }
 }
 
-// Epilogue of kR rows' 8 neighbouring columns from `col` on, bias already
-// added: rows row, row + 8, ..., those from M on left out; `res` holds the
-// residual's values if there is one.  All rows go through each step together,
-// so that their arithmetic overlaps.
-template <typename T, int kR>
-__device__ __forceinline__ void load_residual(const Params &p, int row, int col, uint4 (&res)[kR]) {
-    if (!p.residual || col >= p.N) return;
-    const T *r = static_cast<const T *>(p.residual) + row * p.ldr + col;
-#pragma unroll
-    for (int i = 0; i < kR; ++i)
-        if (row + i * 8 < p.M) res[i] = __ldg(reinterpret_cast<const uint4 *>(r + i * 8 * p.ldr));
-}
-template <typename T, int kR>
-__device__ __forceinline__ void finish(const Params &p, int row, int col, F2 (&v)[kR * 4], const uint4 (&res)[kR]) {
-    if (p.pre) {
-        T *o = static_cast<T *>(p.pre) + row * p.ldpre + col;
-#pragma unroll
-        for (int i = 0; i < kR; ++i)
-            if (row + i * 8 < p.M) *reinterpret_cast<uint4 *>(o + i * 8 * p.ldpre) = pack8<T>(v + 4 * i);
-    }
-    act_n(p.act, v);
-    if (p.residual) {
-#pragma unroll
-        for (int i = 0; i < kR; ++i) {
-            F2 r[4];
-            unpack8<T>(res[i], r);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) v[4 * i + e] = add2(v[4 * i + e], r[e]);
-        }
-    }
-    T *o = static_cast<T *>(p.y) + row * p.ldy + col;
-#pragma unroll
-    for (int i = 0; i < kR; ++i)
-        if (row + i * 8 < p.M) *reinterpret_cast<uint4 *>(o + i * 8 * p.ldy) = pack8<T>(v + 4 * i);
-}
 template <typename T>
 __device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, float v) {
     if (p.pre) static_cast<T *>(p.pre)[row * p.ldpre + col] = from_f32<T>(v);
@@ -232,93 +203,101 @@ __device__ __forceinline__ float4 lds128(uint32_t addr) {
     asm volatile("ld.shared.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
     return v;
 }
-__device__ __forceinline__ void sts32(uint32_t addr, float v) { asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory"); }
+__device__ __forceinline__ uint4 lds128u(uint32_t addr) {
+    uint4 v;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+    return v;
+}
 __device__ __forceinline__ float lds32(uint32_t addr) {
     float v;
     asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
     return v;
 }
 
-// One 32 x 32 chunk of a warp: rows [row0, row0 + 32) from the staging tile.
-// inv: 1 / scale of the lane's rows, for codes.
+// 8 bias values of columns that every lane has alike.
 template <typename T>
-__device__ __forceinline__ void write_chunk(const Params &p, uint32_t stg, int row0, int col0, int sp, int lane,
-                                            const uint4 (&res)[4], const float (&inv)[4]) {
-    if (p.partial || p.vec) {
-        const int col = col0 + (lane & 3) * 8, r0 = lane >> 2;
-        const bool in = col < (p.partial ? p.ldp : p.N);  // both multiples of 8
+__device__ __forceinline__ void add_bias32(const Params &p, int col0, F2 (&v)[16]) {
+    if (!p.bias) return;
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        if (col0 + 8 * g >= p.N) break;  // N is a multiple of 8
+        F2 b[4];
+        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.bias) + col0 + 8 * g)), b);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[4 * g + e] = add2(v[4 * g + e], b[e]);
+    }
+}
+// A lane's 32 values as its row of a 32 x 32 tile: 64 bytes, in the 64-byte
+// swizzle of the tensor maps (free of bank conflicts).
+template <typename T>
+__device__ __forceinline__ void put_row(uint32_t tile, int lane, const F2 (&v)[16]) {
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+        const uint4 q = pack8<T>(v + 4 * g);
+        sts128(tile + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4), q.x, q.y, q.z, q.w);
+    }
+}
+
+// The two ways around TMA: fp32 partial tiles, and outputs whose rows do not
+// take 16-byte accesses.  `stg`: the warp's 32 x 32 fp32 tile, row-swizzled.
+template <typename T>
+__device__ __forceinline__ void write_plain(const Params &p, uint32_t stg, int row0, int col0, int sp, int lane) {
+    if (p.partial) {
+        const int col = col0 + (lane & 3) * 8, r0 = lane >> 2, row = row0 + r0;
+        if (col >= p.ldp) return;  // a multiple of 8
         const uint32_t src = stg + r0 * 128;
         const uint32_t c0 = ((2 * (lane & 3)) ^ r0) << 4;  // r0 < 8: the rows' swizzle
-        F2 v[16];
+        float *dst = p.partial + ((int64_t)sp * p.M + row) * p.ldp + col;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float4 a = lds128(src + i * 1024 + c0), b = lds128(src + i * 1024 + (c0 ^ 16));
-            v[4 * i] = f2(a.x, a.y), v[4 * i + 1] = f2(a.z, a.w), v[4 * i + 2] = f2(b.x, b.y), v[4 * i + 3] = f2(b.z, b.w);
+            if (row + i * 8 >= p.M) break;
+            reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[0] = lds128(src + i * 1024 + c0);
+            reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[1] = lds128(src + i * 1024 + (c0 ^ 16));
         }
-        const int row = row0 + r0;
-        if (p.partial) {
-            if (!in) return;
-            float *dst = p.partial + ((int64_t)sp * p.M + row) * p.ldp + col;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (row + i * 8 >= p.M) break;
-                const float2 a = split(v[4 * i]), b = split(v[4 * i + 1]), c = split(v[4 * i + 2]), d = split(v[4 * i + 3]);
-                reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[0] = make_float4(a.x, a.y, b.x, b.y);
-                reinterpret_cast<float4 *>(dst + (int64_t)i * 8 * p.ldp)[1] = make_float4(c.x, c.y, d.x, d.y);
-            }
-            return;
-        }
-        if (in) add_bias8<T>(p, col, v, 4);
-        if (p.codes && in) {
-            uint8_t *codes = p.codes + (int64_t)row * p.N + col;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if (row + i * 8 >= p.M) break;
-                const V8 x = {v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]};
-                *reinterpret_cast<uint2 *>(codes + (int64_t)i * 8 * p.N) =
-                    p.keep == FCAI_KEEP_E4M3 ? encode8<true>(x, inv[i]) : encode8<false>(x, inv[i]);
-            }
-        }
-        if (in) finish<T, 4>(p, row, col, v, res);
-    } else {
-        const int col = col0 + lane;
-        if (col >= p.N) return;
-        const float bias = p.bias ? to_f32(static_cast<const T *>(p.bias)[col]) : 0.f;
-        // eight rows' residuals at a time are on their way before the first is used
+        return;
+    }
+    const int col = col0 + lane;
+    if (col >= p.N) return;
+    const float bias = p.bias ? to_f32(static_cast<const T *>(p.bias)[col]) : 0.f;
+    // eight rows' residuals at a time are on their way before the first is used
 #pragma unroll 1
-        for (int r = 0; r < 32 && row0 + r < p.M; r += 8) {
-            const int left = p.M - row0 - r;
-            float res[8], v[8];
+    for (int r = 0; r < 32 && row0 + r < p.M; r += 8) {
+        const int left = p.M - row0 - r;
+        float res[8], v[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+            res[e] = p.residual && e < left ? to_f32(static_cast<const T *>(p.residual)[(row0 + r + e) * p.ldr + col]) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = lds32(stg + (r + e) * 128 + (((lane >> 2) ^ e) << 4) + (lane & 3) * 4) + bias;
+        if (p.pre) {
 #pragma unroll
             for (int e = 0; e < 8; ++e)
-                res[e] = p.residual && e < left ? to_f32(static_cast<const T *>(p.residual)[(row0 + r + e) * p.ldr + col]) : 0.f;
+                if (e < left) static_cast<T *>(p.pre)[(row0 + r + e) * p.ldpre + col] = from_f32<T>(v[e]);
+        }
+        F2 w[4] = {f2(v[0], v[1]), f2(v[2], v[3]), f2(v[4], v[5]), f2(v[6], v[7])};
+        act_n(p.act, w);
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-                v[e] = lds32(stg + (r + e) * 128 + (((lane >> 2) ^ e) << 4) + (lane & 3) * 4) + bias;
-            if (p.pre) {
-#pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (e < left) static_cast<T *>(p.pre)[(row0 + r + e) * p.ldpre + col] = from_f32<T>(v[e]);
-            }
-            F2 w[4] = {f2(v[0], v[1]), f2(v[2], v[3]), f2(v[4], v[5]), f2(v[6], v[7])};
-            act_n(p.act, w);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float2 f = split(w[e / 2]);
-                if (e < left) static_cast<T *>(p.y)[(row0 + r + e) * p.ldy + col] = from_f32<T>((e & 1 ? f.y : f.x) + res[e]);
-            }
+        for (int e = 0; e < 8; ++e) {
+            const float2 f = split(w[e / 2]);
+            if (e < left) static_cast<T *>(p.y)[(row0 + r + e) * p.ldy + col] = from_f32<T>((e & 1 ? f.y : f.x) + res[e]);
         }
     }
 }
+
+struct Maps {
+    CUtensorMap a, b;           // operands
+    CUtensorMap y, res, extra;  // 32 x 32 tiles of y, the residual, and pre or the codes (where they are used)
+};
 
 // kTA / kTB: the operand's rows run along K (its M / N axis is contiguous).
 // kPair: clusters of two CTAs share each MMA (cta_group::2, M = 256): each CTA
 // stages its 128 rows of A and half the columns' rows of B and owns 128 rows
 // of the accumulator; the rank-0 CTA issues for both.
-template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
-__global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
-    linear_tc_kernel(const __grid_constant__ CUtensorMap tmA, const __grid_constant__ CUtensorMap tmB, const Params p) {
-    using Lay = Layout<kBN, kPair>;
+template <typename T, int kBN, bool kPair, bool kTA, bool kTB, bool kKeep>
+__global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
+    linear_tc_kernel(const __grid_constant__ Maps maps, const Params p) {
+    using Lay = Layout<kBN, kPair, kKeep>;
+    const CUtensorMap &tmA = maps.a, &tmB = maps.b;
     constexpr int kStages = Lay::kStages, kEpiWarps = Lay::kEpiWarps, kBufs = Lay::kBufs;
     extern __shared__ unsigned char smem_raw[];
     unsigned char *smem =
@@ -328,7 +307,8 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
     uint64_t *accf = empty + kStages;  // accumulator filled (by the MMA warp; pairs: in both CTAs)
     uint64_t *acce = accf + kBufs;     // accumulator read: one arrival per epilogue warp of this CTA that reads it
     uint64_t *pacce = acce + kBufs;    // pairs, rank 0: the peer's accumulator read
-    uint64_t *dbar = pacce + kBufs;        // abort path: this CTA's MMAs drained
+    uint64_t *resbar = pacce + kBufs;  // residual tiles loaded: two per epilogue warp
+    uint64_t *dbar = resbar + 2 * kEpiWarps;        // abort path: this CTA's MMAs drained
     uint32_t *tmem_slot = reinterpret_cast<uint32_t *>(smem + Lay::offSlot);
     volatile int *abort = reinterpret_cast<volatile int *>(smem + Lay::offSlot + 4);
 
@@ -350,6 +330,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
             mbar_init(&acce[b], p.coop ? (kBN < 128 ? kBN / 32 * 4 : kEpiWarps) : Lay::kGroupWarps);
             mbar_init(&pacce[b], 1);
         }
+        for (int b = 0; b < 2 * kEpiWarps; ++b) mbar_init(&resbar[b], 1);
         mbar_init(dbar, 1);
         *abort = 0;
         fence_barrier_init();
@@ -504,9 +485,19 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
         const int j0 = p.coop ? 0 : warp / Lay::kGroupWarps, jstep = p.coop ? 1 : kBufs;
         const int cbegin = p.coop ? (warp >> 2) * 32 : (warp % Lay::kGroupWarps) / 4 * 128;
         const int cstep = p.coop ? 128 : 32, cend = p.coop ? kBN : cbegin + Lay::kSpan;
-        const uint32_t staging = smem_u32(smem + Lay::offStaging) + warp * kStagingWarp;
-        const uint32_t stg = staging + lane * 128 + ((lane & 7) << 4);  // this row's chunk 0
-        const bool wide_res = p.vec && p.residual && !p.partial;
+        const uint32_t staging = smem_u32(smem + Lay::offStaging) + warp * Lay::kWarpTile;
+        const uint32_t extra = staging + kStagingWarp;
+        const uint32_t stg = staging + lane * 128 + ((lane & 7) << 4);  // this row of an fp32 tile, chunk 0
+        const uint32_t rbar = smem_u32(&resbar[2 * warp]);
+        const bool tma = p.vec && !p.partial, residual = tma && p.residual;
+        uint32_t n = 0;  // chunks through the two tiles so far
+        // Lane 0: the residual's rows and columns of chunk `i` into tile i % 2,
+        // whose last store (chunk i - 2) has been read.
+        auto fetch_residual = [&](uint32_t i, int col, int row) {
+            const uint32_t bar = rbar + (i & 1) * 8;
+            asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(kTileBytes) : "memory");
+            tma_load_2d(staging + (i & 1) * kTileBytes, &maps.res, bar, col, row);
+        };
         if (cbegin < kBN)
             for (int j = j0, unit = unit0 + j0 * unit_step; unit < p.units; j += jstep, unit += jstep * unit_step) {
                 int tm, tn, sp;
@@ -514,69 +505,122 @@ __global__ void __launch_bounds__(Layout<kBN, kPair>::kThreads, 1)
                 const int buf = j % kBufs;
                 const int row0 = tm * Lay::kTileM + (int)rank * kBM + q * 32;
                 const int ctile = tn * kBN;
-                uint4 res[4];  // the residual's rows: on their way while the accumulator fills
-                if (wide_res) load_residual<T, 4>(p, row0 + (lane >> 2), ctile + cbegin + (lane & 3) * 8, res);
+                const int cmax = row0 < p.M ? min(cend, p.N - ctile) : cbegin;  // columns that are there: chunks below it
+                if (residual && cbegin < cmax && lane == 0) {  // on its way while the accumulator fills
+                    bulk_wait_read_but_one();
+                    fetch_residual(n, ctile + cbegin, row0);
+                }
                 if (!mbar_wait_warp_idle(&accf[buf], (j / kBufs) & 1, abort, kWaitNs)) {
                     *abort = 1;
+                    if (residual && cbegin < cmax) mbar_wait(&resbar[2 * warp + (n & 1)], (n >> 1) & 1, nullptr, kWaitNs / 10);
                     break;
                 }
                 tc_fence_after();
                 const uint32_t taddr = tmem_base + buf * kBN + ((uint32_t)(q * 32) << 16);
-                float inv[4];  // codes: 1 / scale of this lane's four rows
-                if (p.codes && !p.partial && ctile + cbegin < p.N) {
-                    // first pass, a row a lane: the largest magnitude of the block;
-                    // the bias comes from the staging tile, 4 columns a load
-                    const int cb = ctile + cbegin + lane * 4;
-                    F2 b[2] = {f2(0.f), f2(0.f)};
-                    if (p.bias && lane * 4 < Lay::kSpan && cb < p.N) {
-                        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(static_cast<const T *>(p.bias) + cb));
-                        const float2 lo = unpack2(w.x, T()), hi = unpack2(w.y, T());
-                        b[0] = f2(lo.x, lo.y), b[1] = f2(hi.x, hi.y);
-                    }
-                    const float2 b0 = split(b[0]), b1 = split(b[1]);
-                    sts128(staging + lane * 16, __float_as_uint(b0.x), __float_as_uint(b0.y), __float_as_uint(b1.x), __float_as_uint(b1.y));
-                    __syncwarp();
+                float inv = 1.f;  // codes: 1 / scale of this lane's row
+                if (kKeep && p.codes && !p.partial && cbegin < cmax) {
+                    // first pass: the largest magnitude of the row's block
                     float m = 0.f;
 #pragma unroll 1
-                    for (int c = 0; c < Lay::kSpan; c += 32) {
-                        uint32_t v[32];
-                        tmem_ld32(taddr + cbegin + c, v);
+                    for (int c = cbegin; c < cmax; c += 32) {
+                        uint32_t w[32];
+                        tmem_ld32(taddr + c, w);
                         tmem_wait_ld();
+                        F2 v[16];
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) {
-                            const float4 bb = lds128(staging + c * 4 + e * 16);
-                            const float2 x = split(add2(f2(__uint_as_float(v[4 * e]), __uint_as_float(v[4 * e + 1])), f2(bb.x, bb.y)));
-                            const float2 y = split(add2(f2(__uint_as_float(v[4 * e + 2]), __uint_as_float(v[4 * e + 3])), f2(bb.z, bb.w)));
-                            m = max_nan(m, max_nan(max_nan(fabsf(x.x), fabsf(x.y)), max_nan(fabsf(y.x), fabsf(y.y))));
-                        }
+                        for (int e = 0; e < 16; ++e) v[e] = f2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+                        add_bias32<T>(p, ctile + c, v);
+#pragma unroll
+                        for (int e = 0; e < 16; e += 4) m = max_nan(m, amax8(v + e));
                     }
                     const float s = keep_scale(p.keep, m);
                     if (row0 + lane < p.M) p.scales[(int64_t)(row0 + lane) * p.nblk + (ctile + cbegin) / FCAI_KEEP_BLOCK] = s;
-                    const float r = __frcp_rn(s);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) inv[i] = __shfl_sync(0xffffffffu, r, i * 8 + (lane >> 2));
+                    inv = __frcp_rn(s);
                 }
+                bool ok = true;
 #pragma unroll 1
                 for (int c = cbegin; c < cend; c += cstep) {
-                    uint32_t v[32];
-                    tmem_ld32(taddr + c, v);
+                    uint32_t w[32];
+                    tmem_ld32(taddr + c, w);
                     tmem_wait_ld();
                     if (c + cstep >= cend) {  // this warp has read its part of the accumulator
                         tc_fence_before();
                         __syncwarp();
                         if (lane == 0) mbar_arrive(&acce[buf]);
                     }
-                    if (row0 < p.M && ctile + c < p.N) {
+                    if (c >= cmax) continue;
+                    const int col0 = ctile + c;
+                    if (!tma) {
 #pragma unroll
-                        for (int e = 0; e < 8; ++e) sts128(stg ^ (e << 4), v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        for (int e = 0; e < 8; ++e) sts128(stg ^ (e << 4), w[4 * e], w[4 * e + 1], w[4 * e + 2], w[4 * e + 3]);
                         __syncwarp();
-                        write_chunk<T>(p, staging, row0, ctile + c, sp, lane, res, inv);
+                        write_plain<T>(p, staging, row0, col0, sp, lane);
                         __syncwarp();
-                        if (wide_res && c + cstep < cend)
-                            load_residual<T, 4>(p, row0 + (lane >> 2), ctile + c + cstep + (lane & 3) * 8, res);
+                        continue;
                     }
+                    F2 v[16];
+#pragma unroll
+                    for (int e = 0; e < 16; ++e) v[e] = f2(__uint_as_float(w[2 * e]), __uint_as_float(w[2 * e + 1]));
+                    add_bias32<T>(p, col0, v);
+                    const uint32_t tile = staging + (n & 1) * kTileBytes;
+                    if (lane == 0) bulk_wait_read_but_one();  // this chunk's tile, and the extra one, may be written
+                    __syncwarp();
+                    if (kKeep && p.codes) {
+                        // the row's 32 codes, in the 32-byte swizzle of their map
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const V8 x = {v[8 * h], v[8 * h + 1], v[8 * h + 2], v[8 * h + 3]}, y = {v[8 * h + 4], v[8 * h + 5], v[8 * h + 6], v[8 * h + 7]};
+                            const uint2 a = p.keep == FCAI_KEEP_E4M3 ? encode8<true>(x, inv) : encode8<false>(x, inv);
+                            const uint2 b = p.keep == FCAI_KEEP_E4M3 ? encode8<true>(y, inv) : encode8<false>(y, inv);
+                            sts128(extra + lane * 32 + ((h ^ ((lane >> 2) & 1)) << 4), a.x, a.y, b.x, b.y);
+                        }
+                    } else if (kKeep && p.pre) {
+                        put_row<T>(extra, lane, v);
+                    }
+                    if (kKeep && (p.codes || p.pre)) {
+                        fence_proxy_async_smem();
+                        __syncwarp();
+                        if (lane == 0) {
+                            tma_store_2d(&maps.extra, extra, col0, row0);
+                            bulk_commit_group();
+                        }
+                    }
+                    act_n(p.act, v);
+                    if (residual) {
+                        if (lane == 0 && c + cstep < cmax) {
+                            // the other tile's store (the previous chunk's) has been read; the extra one's may be pending
+                            if (kKeep && (p.codes || p.pre)) bulk_wait_read_but_one();
+                            else bulk_wait_read_all();
+                            fetch_residual(n + 1, col0 + cstep, row0);
+                        }
+                        __syncwarp();
+                        ok = mbar_wait_warp_idle(&resbar[2 * warp + (n & 1)], (n >> 1) & 1, abort, kWaitNs);
+                        if (!ok) {
+                            *abort = 1;
+                            if (c + cstep < cmax) mbar_wait(&resbar[2 * warp + ((n + 1) & 1)], ((n + 1) >> 1) & 1, nullptr, kWaitNs / 10);
+                            break;
+                        }
+#pragma unroll
+                        for (int g = 0; g < 4; ++g) {
+                            F2 r[4];
+                            unpack8<T>(lds128u(tile + lane * 64 + ((g ^ ((lane >> 1) & 3)) << 4)), r);
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[4 * g + e] = add2(v[4 * g + e], r[e]);
+                        }
+                    }
+                    put_row<T>(tile, lane, v);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        tma_store_2d(&maps.y, tile, col0, row0);
+                        bulk_commit_group();
+                    }
+                    ++n;
                 }
+                if (!ok) break;
             }
+        if (lane == 0) bulk_wait_all();  // stores complete before the CTA exits
+        __syncwarp();
     }
 
     // ---------------------------------------------------------------- teardown
@@ -654,9 +698,15 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
         }
         if (!in) continue;
         if (p.vec) {
-            uint4 res[1];
-            load_residual<T, 1>(p, (int)row, col, res);
-            finish<T, 1>(p, (int)row, col, v, res);
+            if (p.pre) *reinterpret_cast<uint4 *>(static_cast<T *>(p.pre) + row * p.ldpre + col) = pack8<T>(v);
+            act_n(p.act, v);
+            if (p.residual) {
+                F2 r[4];
+                unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.residual) + row * p.ldr + col)), r);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[e] = add2(v[e], r[e]);
+            }
+            *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ldy + col) = pack8<T>(v);
         } else {
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
@@ -809,18 +859,27 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// A row-major matrix [outer][inner] as 128-byte swizzled boxes of 64 elements x box_rows.
-static int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_rows, int dtype) {
+constexpr int kCodeType = 100;  // a map of codes: bytes
+// A row-major matrix [outer][inner] as boxes of box_cols x box_rows elements,
+// swizzled over the box's row: 64 16-bit columns 128 bytes (operands), 32 64
+// bytes, 32 codes 32 bytes (results).
+static int make_map(CUtensorMap *map, const void *base, int64_t inner, int64_t outer, int64_t ld, int box_rows, int dtype,
+                    int box_cols = 64) {
     auto fn = encode_fn();
     if (!fn) return fcai::fail(FCAI_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+    const int size = dtype == kCodeType ? 1 : 2;
     const cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)outer};
-    const cuuint64_t strides[1] = {(cuuint64_t)ld * 2};
-    const cuuint32_t box[2] = {64, (cuuint32_t)box_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)ld * size};
+    const cuuint32_t box[2] = {(cuuint32_t)box_cols, (cuuint32_t)box_rows};
     const cuuint32_t es[2] = {1, 1};
-    const CUresult r = fn(map, dtype == FCAI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16,
-                          2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapSwizzle sw = box_cols * size == 128 ? CU_TENSOR_MAP_SWIZZLE_128B
+                                  : box_cols * size == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                                          : CU_TENSOR_MAP_SWIZZLE_32B;
+    const CUtensorMapDataType type = dtype == kCodeType         ? CU_TENSOR_MAP_DATA_TYPE_UINT8
+                                     : dtype == FCAI_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                                : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    const CUresult r = fn(map, type, 2, const_cast<void *>(base), dims, strides, box, es, CU_TENSOR_MAP_INTERLEAVE_NONE, sw,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return fcai::fail(FCAI_ERR_INVALID, "cuTensorMapEncodeTiled failed (%d)", (int)r);
     return FCAI_OK;
 }
@@ -910,10 +969,10 @@ static int prepare_operands(Operand &a, Operand &b, int dtype, unsigned char *ws
     return FCAI_OK;
 }
 
-template <typename T, int kBN, bool kPair, bool kTA, bool kTB>
-static int launch(const CUtensorMap &a, const CUtensorMap &b, const Params &p, cudaStream_t stream) {
-    using Lay = Layout<kBN, kPair>;
-    auto kernel = linear_tc_kernel<T, kBN, kPair, kTA, kTB>;
+template <typename T, int kBN, bool kPair, bool kTA, bool kTB, bool kKeep>
+static int launch(const Maps &maps, const Params &p, cudaStream_t stream) {
+    using Lay = Layout<kBN, kPair, kKeep>;
+    auto kernel = linear_tc_kernel<T, kBN, kPair, kTA, kTB, kKeep>;
     static int slots[64] = {0};  // CTAs (pairs) resident at once
     int dev = 0;
     FCAI_CUDA_TRY(cudaGetDevice(&dev));
@@ -942,9 +1001,9 @@ static int launch(const CUtensorMap &a, const CUtensorMap &b, const Params &p, c
     const int n = std::min(p.units, slots[dev]);
     if (kPair) {
         cfg.gridDim = dim3(2 * n, 1, 1);
-        FCAI_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, a, b, p));
+        FCAI_CUDA_TRY(cudaLaunchKernelEx(&cfg, kernel, maps, p));
     } else {
-        kernel<<<n, Lay::kThreads, Lay::kAlloc, stream>>>(a, b, p);
+        kernel<<<n, Lay::kThreads, Lay::kAlloc, stream>>>(maps, p);
     }
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
@@ -962,16 +1021,16 @@ static int launch_reduce(const Params &p, cudaStream_t stream) {
 static bool wide_outputs(const Params &p, int N, int dtype) {
     return N % 8 == 0 && aligned16(p.y, p.ldy, dtype) && (!p.pre || aligned16(p.pre, p.ldpre, dtype)) &&
            (!p.residual || aligned16(p.residual, p.ldr, dtype)) && (!p.bias || aligned16(p.bias, 0, dtype)) &&
-           (reinterpret_cast<uintptr_t>(p.codes) & 7) == 0;
+           (reinterpret_cast<uintptr_t>(p.codes) & (N % 16 ? 7 : 15)) == 0;
 }
 // A product with codes runs its epilogue in reduce_kernel when N alone rules
-// wide accesses out (the workspace is asked for by sizes); otherwise its outputs
+// tiles of codes out (the workspace is asked for by sizes); otherwise its outputs
 // take them, which the entry point has checked.
 template <typename T, bool kTA, bool kTB>
 static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Params p, unsigned char *ws,
                cudaStream_t stream) {
     p.vec = wide_outputs(p, N, dtype);
-    const bool reduce = p.codes && N % 8 != 0;
+    const bool reduce = p.codes && N % 16 != 0;
     const Plan pl = make_plan(M, N, K, reduce, p.codes != nullptr);
     p.M = (int)M;
     p.N = N;
@@ -994,13 +1053,23 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     }
     int rc;
     if ((rc = prepare_operands(A, B, dtype, ws, stream))) return rc;
-    CUtensorMap ma, mb;
-    if ((rc = make_map(&ma, A.ptr, A.cols, A.rows, A.ld, kTA ? kBK : kBM, dtype))) return rc;
-    if ((rc = make_map(&mb, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.pair ? pl.bn / 2 : pl.bn, dtype)))
-        return rc;
-    rc = pl.pair        ? launch<T, 256, true, kTA, kTB>(ma, mb, p, stream)
-         : pl.bn == 128 ? launch<T, 128, false, kTA, kTB>(ma, mb, p, stream)
-                        : launch<T, 64, false, kTA, kTB>(ma, mb, p, stream);
+    Maps maps;
+    if ((rc = make_map(&maps.a, A.ptr, A.cols, A.rows, A.ld, kTA ? kBK : kBM, dtype))) return rc;
+    if ((rc = make_map(&maps.b, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.pair ? pl.bn / 2 : pl.bn, dtype))) return rc;
+    const bool tma = p.vec && !p.partial, keep = !kTA && !kTB && tma && (p.pre || p.codes);
+    if (tma) {
+        if ((rc = make_map(&maps.y, p.y, N, M, p.ldy, 32, dtype, 32))) return rc;
+        if (p.residual && (rc = make_map(&maps.res, p.residual, N, M, p.ldr, 32, dtype, 32))) return rc;
+        if (p.codes && (rc = make_map(&maps.extra, p.codes, N, M, N, 32, kCodeType, 32))) return rc;
+        if (p.pre && (rc = make_map(&maps.extra, p.pre, N, M, p.ldpre, 32, dtype, 32))) return rc;
+    }
+#define LN_LAUNCH(keep_)                                                              \
+    (pl.pair        ? launch<T, 256, true, kTA, kTB, keep_>(maps, p, stream)          \
+     : pl.bn == 128 ? launch<T, 128, false, kTA, kTB, keep_>(maps, p, stream)         \
+                    : launch<T, 64, false, kTA, kTB, keep_>(maps, p, stream))
+    if constexpr (!kTA && !kTB) rc = keep ? LN_LAUNCH(true) : LN_LAUNCH(false);
+    else rc = LN_LAUNCH(false);
+#undef LN_LAUNCH
     if (rc) return rc;
     return p.partial ? launch_reduce<T>(p, stream) : FCAI_OK;
 }
@@ -1058,7 +1127,7 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
     switch (op) {
         case FCAI_LINEAR_FORWARD:
             if (rows <= kFewRows) return keep >= FCAI_KEEP_INT8 ? round256(rows * round8(cout) * 4) : 0;
-            if (keep >= FCAI_KEEP_INT8) n = make_plan(rows, cout, cin, cout % 8 != 0, true).partial_bytes;
+            if (keep >= FCAI_KEEP_INT8) n = make_plan(rows, cout, cin, cout % 16 != 0, true).partial_bytes;
             else n = make_plan(rows, cout, cin).partial_bytes;
             if (repack & 1) n += repack_bytes(rows, cin);
             if (repack & 2) n += repack_bytes(cout, cin);
@@ -1124,7 +1193,7 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     p.scales = scales;
     p.keep = keep;
     if (k8 && rows > kFewRows && cout % 8 == 0 && !wide_outputs(p, cout, dtype))
-        return fcai::fail(FCAI_ERR_INVALID, "linear: codes need 16-byte aligned y, bias and residual rows, and 8-byte aligned codes");
+        return fcai::fail(FCAI_ERR_INVALID, "linear: codes need 16-byte aligned y, bias and residual rows, and 16-byte aligned codes");
     if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, keep, workspace, workspace_bytes)))
         return rc;
     const Operand A{x, ldx, rows, cin}, B{w, ldw, cout, cin};

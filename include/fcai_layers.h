@@ -56,8 +56,8 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
  * rounding) as codes and scales.  Addresses and strides need only the elements'
  * alignment; 16-byte aligned addresses and strides (8 elements) are read
  * without a copy.  With an 8-bit keep, more than 32 rows and cout a multiple of
- * 8, the addresses and strides of y, bias and residual are 16-byte aligned and
- * codes 8-byte. */
+ * 8, the addresses and strides of y, bias and residual, and codes, are 16-byte
+ * aligned. */
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
 /* `repack`: bit 0 / bit 1 set when the call's first / second matrix is not
  * 16-byte aligned in address and row stride (x, w; dp, w; dp, x); `keep`: the
