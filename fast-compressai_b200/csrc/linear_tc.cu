@@ -647,26 +647,53 @@ __global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
     }
 }
 
-// Sums the splits in order and applies the epilogue: 16 lanes a row's 128
-// columns, 8 each, so that an 8-bit block is theirs.  Also the second half of a
-// product that keeps codes but whose rows do not take wide accesses.
-template <typename T>
+// Sums the splits in a fixed order and applies the epilogue: 16 lanes a row's 128
+// columns, 8 each, so that an 8-bit block is theirs.  Few rows: kParts groups of
+// 16 lanes share a row's splits (every kParts-th each) and the first one adds
+// their sums, since one group's loads alone would leave most SMs idle.  Also the
+// second half of a product that keeps codes but whose rows do not take wide
+// accesses.
+template <typename T, int kParts>
 __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
+    __shared__ float sums[kParts > 1 ? 16 : 1][kParts > 1 ? 128 : 1];
+    constexpr int kRows = 16 / kParts;  // rows a CTA and step
+    const int group = threadIdx.x >> 4, split0 = group / kRows;
     const int col = blockIdx.x * FCAI_KEEP_BLOCK + (threadIdx.x & 15) * 8;
     const int64_t step = (int64_t)p.M * p.ldp;
-    // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
-    for (int64_t r0 = (int64_t)blockIdx.y * 16 + (threadIdx.x >> 5) * 2; r0 < p.M; r0 += (int64_t)gridDim.y * 16) {
-        const int64_t row = r0 + ((threadIdx.x >> 4) & 1);
-        const bool in = row < p.M && col < p.N;
+    // every thread runs the same steps: barriers, and a block's shuffles need whole warps
+    for (int64_t r0 = (int64_t)blockIdx.y * kRows; r0 < p.M; r0 += (int64_t)gridDim.y * kRows) {
+        const int64_t row = r0 + group % kRows;
+        bool in = row < p.M && col < p.N;
         F2 v[4] = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
         if (in) {
-            const float *src = p.partial + row * p.ldp + col;
+            const float *src = p.partial + row * p.ldp + col + split0 * step;
 #pragma unroll 4
-            for (int s = 0; s < (int)p.splits.d; ++s, src += step) {
+            for (int s = split0; s < (int)p.splits.d; s += kParts, src += kParts * step) {
                 const float4 a = __ldg(reinterpret_cast<const float4 *>(src)), b = __ldg(reinterpret_cast<const float4 *>(src) + 1);
                 v[0] = add2(v[0], f2(a.x, a.y)), v[1] = add2(v[1], f2(a.z, a.w));
                 v[2] = add2(v[2], f2(b.x, b.y)), v[3] = add2(v[3], f2(b.z, b.w));
             }
+        }
+        if constexpr (kParts > 1) {
+            float *mine = &sums[group][(threadIdx.x & 15) * 8];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const float2 f = split(v[e]);
+                mine[2 * e] = f.x, mine[2 * e + 1] = f.y;
+            }
+            __syncthreads();
+            in = in && split0 == 0;
+            if (in) {
+#pragma unroll
+                for (int q = 1; q < kParts; ++q) {
+                    const float *o = &sums[group + q * kRows][(threadIdx.x & 15) * 8];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) v[e] = add2(v[e], f2(o[2 * e], o[2 * e + 1]));
+                }
+            }
+            __syncthreads();
+        }
+        if (in) {
             if (p.vec) {
                 add_bias8<T>(p, col, v, 1);
             } else if (p.bias) {
@@ -1011,8 +1038,14 @@ static int launch(const Maps &maps, const Params &p, cudaStream_t stream) {
 
 template <typename T>
 static int launch_reduce(const Params &p, cudaStream_t stream) {
-    const int shares = (int)std::min<int64_t>({((int64_t)p.M + 15) / 16, std::max<int64_t>(1, (int64_t)fcai::sm_count() * 8 / p.nblk), 65535});
-    reduce_kernel<T><<<dim3(p.nblk, shares), 256, 0, stream>>>(p);
+    const int64_t sms = fcai::sm_count(), ctas = ((int64_t)p.M + 15) / 16 * p.nblk;  // with one part
+    const int parts = p.splits.d < 8 || ctas >= 2 * sms ? 1 : ctas * 4 >= 2 * sms ? 4 : 16;
+    const int rows = 16 / parts;
+    const int shares = (int)std::min<int64_t>({((int64_t)p.M + rows - 1) / rows, std::max<int64_t>(1, sms * 8 / p.nblk), 65535});
+    const dim3 grid(p.nblk, shares);
+    if (parts == 1) reduce_kernel<T, 1><<<grid, 256, 0, stream>>>(p);
+    else if (parts == 4) reduce_kernel<T, 4><<<grid, 256, 0, stream>>>(p);
+    else reduce_kernel<T, 16><<<grid, 256, 0, stream>>>(p);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }

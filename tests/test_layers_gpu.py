@@ -293,6 +293,35 @@ def test_layer_norm(cuda_device, rows, n, dtype, keep):
         assert torch.equal(layers.layer_norm_backward(dy, saved, w, needs=(True, False, False))[0], grads[0])
 
 
+# enough rows for the kernels that take several rows a CTA at a time: tails, widths that leave threads idle, two
+# chunks a thread
+@pytest.mark.parametrize("rows,n,dtype", [(9500, 520, torch.bfloat16), (6001, 1032, torch.float16), (6000, 1024, torch.bfloat16),
+                                          (2500, 4096, torch.bfloat16), (2405, 2048, torch.float32), (3001, 6160, torch.float16),
+                                          (1300, 8192, torch.bfloat16), (1301, 4096, torch.float32)])
+@pytest.mark.parametrize("keep", [None, "full", "int8", "e4m3"])
+def test_layer_norm_many_rows(cuda_device, rows, n, dtype, keep):
+    x = _randn(rows, n, dtype=dtype) + _randn(rows, 1, dtype=dtype, seed=9) * 3
+    w, b = 1 + _randn(n, dtype=torch.float32, seed=1, scale=0.3), _randn(n, dtype=torch.float32, seed=2)
+    dy = _randn(rows, n, dtype=dtype, seed=4)
+    wide = torch.zeros(rows, n + 64, dtype=dtype, device="cuda")  # rows with a stride of their own
+    wide[:, 64:] = x
+    got = layers.layer_norm_forward(wide[:, 64:], w, b, eps=1e-4, keep=keep)
+    y, saved = got if keep else (got, None)
+    want, bound, *_ = R.norm64(x, w, b, 1e-4, dtype)
+    R.check(y, want, bound, "y")
+    if saved is None:
+        return
+    kept = x
+    if keep != "full":
+        kept = saved.kept.load(torch.float32)
+        assert torch.equal(kept, R.keep8(x, keep)[0])
+    grads = layers.layer_norm_backward(dy, saved, w)
+    for name, t, (g, e) in zip(("dx", "dw", "db"), grads, R.norm_grads(dy, kept, x, w, 1e-4, dtype, torch.float32)):
+        R.check(t, g, e, name)
+    assert torch.equal(layers.layer_norm_backward(dy, saved, w, needs=(True, False, False))[0], grads[0])
+    assert torch.equal(layers.layer_norm_backward(dy, saved, w, needs=(False, True, False))[1], grads[1])
+
+
 def test_layer_norm_constant_rows(cuda_device):
     # no variance: the centred values are zero, and y is the bias
     x = torch.full((4, 200), 3.25, dtype=torch.bfloat16, device="cuda")
