@@ -9,6 +9,7 @@
 // a Python one.
 #include <ATen/ATen.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/GradMode.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -154,6 +155,7 @@ PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F &&f) {
         return nullptr;
     }
     try {
+        const c10::AutoGradMode no_graph(false);  // a copy made here is no operation of the caller's
         return f();
     } catch (const Refused &r) {
         PyErr_SetString(PyExc_ValueError, r.what.c_str());

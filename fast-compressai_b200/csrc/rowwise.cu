@@ -448,11 +448,12 @@ struct Group {
     static constexpr int kGroups = kCta / kLanes;
     static constexpr int kWarpsRow = kLanes <= 32 ? 1 : kLanes / 32;
 };
-// CTAs an SM is to hold of the norm kernels: 64 registers a thread for 16-bit
-// rows, 128 for f32 ones and two chunks.
-constexpr int norm_ctas(int lanes, int chunks, bool f32, int warp_groups) {
+// CTAs an SM is to hold of the norm kernels, which also sets their grids: whole
+// CTAs a row with two chunks a thread get 128 registers (the forward kernel of
+// 16-bit rows makes do with 84).
+constexpr int norm_ctas(int lanes, int chunks, bool f32, int warp_groups, bool lean = false) {
     if (lanes <= 32) return f32 && chunks == 2 ? 1 : f32 ? 2 : warp_groups;
-    const int threads = f32 || chunks > 1 ? 512 : 1024;
+    const int threads = f32 ? 512 : chunks == 1 ? 1024 : lean ? 768 : 512;
     return threads > lanes ? threads / lanes : 1;
 }
 // Sums of kN values over the group, exchanged together.
@@ -508,10 +509,12 @@ __device__ __forceinline__ V8 load_affine(const Affine &a, const void *p, const 
     return o;
 }
 
-// kRows rows a group and step, their sums exchanged together; whole-CTA groups
-// fetch the next step's rows before they sum this one's.
+// kRows rows a group and step, their sums exchanged together; the next step's
+// rows are fetched before this one's are summed.  16 channels a thread of a
+// whole-CTA group: with 8, a row's sums (shuffles, which share the data path of
+// shared memory, and the exchange) took half of all instructions.
 template <typename T, bool kV, bool k8, int kLanes, int kChunks, int kRows>
-__global__ void __launch_bounds__(Group<kLanes>::kCta, norm_ctas(kLanes, kChunks, sizeof(T) == 4, k8 || kChunks == 2 ? 2 : 3))
+__global__ void __launch_bounds__(Group<kLanes>::kCta, norm_ctas(kLanes, kChunks, sizeof(T) == 4, k8 || kChunks == 2 ? 2 : 3, !k8 && kV))
     norm_forward_kernel(const T *__restrict__ x, int64_t ldx, Affine af, T *__restrict__ y, int64_t ldy,
                         float *__restrict__ mean_out, float *__restrict__ rstd_out, uint8_t *__restrict__ codes,
                         float *__restrict__ scales, int64_t rows, int n, int nblk, float eps, int keep) {
@@ -868,8 +871,8 @@ static Held held(int n) {
     if (n <= 256) return {32, 1};
     if (n <= 512) return {32, 2};
     if (n <= 1024) return {128, 1};
-    if (n <= 2048) return {256, 1};
-    if (n <= 4096) return {512, 1};
+    if (n <= 2048) return {128, 2};
+    if (n <= 4096) return {256, 2};
     return {512, 2};
 }
 // Rows a group has in flight in the backward kernel.
@@ -877,7 +880,7 @@ constexpr int backward_rows(int lanes, int chunks) { return lanes <= 32 ? 2 / ch
 static int norm_backward_grid(int64_t rows, int n) {
     const Held h = held(n);
     const int groups = (h.lanes <= 32 ? kThreads / h.lanes : 1) * backward_rows(h.lanes, h.chunks);
-    const int per_sm = h.lanes <= 32 ? 3 : std::max(1, 1024 / h.lanes / h.chunks);
+    const int per_sm = h.lanes <= 32 ? 3 : norm_ctas(h.lanes, h.chunks, false, 0);
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
 }
 static int64_t act_workspace(int64_t rows, int n) {
@@ -979,10 +982,10 @@ struct NormForward {
 };
 template <typename T, bool kV, bool k8, int kLanes, int kChunks>
 static int launch_norm_forward(const NormForward &a) {
-    constexpr int kRows = kLanes > 32 ? (kChunks == 1 && !k8 ? 2 : 1) : kChunks == 1 ? 2 : 1;
+    constexpr int kRows = kLanes <= 32 && kChunks == 1 ? 2 : 1;
     constexpr int64_t kPerCta = (int64_t)Group<kLanes>::kGroups * kRows;
     const int64_t want = (a.rows + kPerCta - 1) / kPerCta;
-    const int grid = (int)std::min<int64_t>(want, (int64_t)fcai::sm_count() * (kLanes > 32 ? std::max(1, 1024 / kLanes) : 6));
+    const int grid = (int)std::min<int64_t>(want, (int64_t)fcai::sm_count() * (kLanes > 32 ? norm_ctas(kLanes, kChunks, sizeof(T) == 4, 0, !k8 && kV) : 6));
     norm_forward_kernel<T, kV, k8, kLanes, kChunks, kRows><<<grid, Group<kLanes>::kCta, 0, a.st>>>(
         static_cast<const T *>(a.x), a.ldx, a.af, static_cast<T *>(a.y), a.ldy, a.mean, a.rstd, static_cast<uint8_t *>(a.codes),
         a.scales, a.rows, a.n, blocks_of(a.n), a.eps, a.keep);
@@ -1015,8 +1018,8 @@ static int launch_norm_backward(const NormBackward &a) {
         case 32 * 8 + 1: return call(32, 1);                         \
         case 32 * 8 + 2: return call(32, 2);                         \
         case 128 * 8 + 1: return call(128, 1);                       \
-        case 256 * 8 + 1: return call(256, 1);                       \
-        case 512 * 8 + 1: return call(512, 1);                       \
+        case 128 * 8 + 2: return call(128, 2);                       \
+        case 256 * 8 + 2: return call(256, 2);                       \
         default: return call(512, 2);                                \
     }
 template <typename T, bool kV, bool k8>

@@ -119,6 +119,39 @@ def test_linear_kept_in_8_bits(cuda_device, rows, cin, cout, fmt, dtype):
         R.check(got, g, e, name)
 
 
+# residual and everything kept at once: results and what is kept leave through different tiles of the same epilogue;
+# 20000 x 512 gives every CTA several tiles, widths that are no multiple of 16 or 8 take the other ways out
+@pytest.mark.parametrize("rows,cin,cout", [(20, 64, 72), (40, 64, 24), (300, 200, 136), (333, 72, 96), (700, 264, 577),
+                                           (5000, 64, 1040), (20000, 128, 512), (20001, 96, 264)])
+@pytest.mark.parametrize("keep", layers.KEEPS)
+@pytest.mark.parametrize("dtype", T16)
+def test_linear_residual_and_keep(cuda_device, rows, cin, cout, keep, dtype):
+    x, w = _randn(rows, cin, dtype=dtype), _randn(cout, cin, dtype=dtype, seed=1, scale=cin ** -0.5)
+    b = _randn(cout + 1, dtype=dtype, seed=2)[1:]  # 2-byte aligned
+    r = _sliced(_randn(rows, cout, dtype=dtype, seed=3)) if cout % 3 else _randn(rows, cout, dtype=dtype, seed=3)
+    y, saved = layers.linear_forward(x, w, b, activation="gelu", residual=r, keep=keep)
+    want, bound = R.linear_bound(x, w, b, r, "gelu", dtype)
+    R.check(y, want, bound, "y")
+    p64, _ = R.linear64(x, w, b)
+    e = (cin + 2) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    if keep == "full":
+        R.check(saved.pre, p64, e + R.half_step(dtype) * (p64.abs() + e) + R.tiny(dtype), "pre")
+        pre = saved.pre.double()
+    else:
+        pre = saved.pre.load(torch.float32).double()
+        # the scale comes from the largest of 128 values that are off by e at most
+        amax = torch.nn.functional.pad(p64.abs(), (0, -cout % 128)).reshape(rows, -1, 128).amax(2)
+        top = 127 if keep == "int8" else 448
+        slack = torch.nn.functional.pad(e, (0, -cout % 128)).reshape(rows, -1, 128).amax(2) / top + amax / top * 2.0 ** -22
+        R.check(saved.pre.scales, amax / top, slack, "scales")
+        R.check(pre, p64, e + R.keep8_step(p64.abs() + e, saved.pre.scales, keep), "pre")
+    dy = _randn(rows, cout, dtype=dtype, seed=4)
+    kept = x if keep == "full" else saved.kept.load()
+    for name, got, (g, bound) in zip(("dx", "dw", "db"), layers.linear_backward(dy, saved, w),
+                                     R.linear_grads(dy, kept, w, pre, "gelu", dtype)):
+        R.check(got, g, bound, name)
+
+
 def test_linear_needs_and_shapes(cuda_device):
     x, w = _randn(2, 5, 64, dtype=torch.bfloat16), _randn(40, 64, dtype=torch.bfloat16, seed=1)
     y, saved = layers.linear_forward(x, w, keep="full")
@@ -443,6 +476,41 @@ def test_captured_in_graphs(cuda_device):
     torch.cuda.synchronize()
     for (x, dy), out in zip(ins, outs):
         assert all(torch.equal(a, e) for a, e in zip(out, step(x, dy)))
+
+
+def test_first_calls_of_a_process_can_be_captured(cuda_device):
+    # nothing has to be set up outside a capture
+    code = """
+import sys
+sys.path[:0] = [%r, %r]
+import torch
+from fast_compressai import layers
+x = torch.randn(700, 200, device="cuda", dtype=torch.bfloat16)
+w = torch.randn(264, 200, device="cuda", dtype=torch.bfloat16) / 14
+dy = torch.randn(700, 264, device="cuda", dtype=torch.bfloat16)
+def step():
+    h, s0 = layers.layer_norm_forward(x, keep="int8")
+    y, s1 = layers.linear_forward(h, w, activation="gelu", keep="e4m3")
+    dh, dw, _ = layers.linear_backward(dy, s1, w)
+    one = layers.linear_forward(x[:1], w)
+    return y, dw, layers.layer_norm_backward(dh, s0)[0], one
+torch.cuda.synchronize()
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(out, step()))
+print("captured")
+"""
+    import subprocess
+    import sys
+    from pathlib import Path
+
+    root = Path(__file__).resolve().parents[1]
+    done = subprocess.run([sys.executable, "-c", code % (str(root), str(root / "fast-compressai_b200"))], capture_output=True,
+                          text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
 
 
 def test_in_place_change_of_a_kept_tensor_is_noticed(cuda_device):
