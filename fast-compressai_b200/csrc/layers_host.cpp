@@ -271,14 +271,15 @@ PyObject *py_activation_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
 }
 
 // dx = g * act'(kept) and its column sums (either may be undefined)
-void act_backward(const at::Tensor &like, const Rows &g, int64_t n, const Kept &k, int act, const at::Tensor &dx, const at::Tensor &sums) {
+void act_backward(const at::Tensor &like, const Rows &g, int64_t n, const Kept &k, int act, const at::Tensor &dx, const at::Tensor &sums,
+                  int64_t lddx) {
     Scratch ws;
     int64_t bytes = 0;
     if (sums.defined()) {
         bytes = fcai_activation_workspace(g.rows, (int)n);
         ws = scratch(bytes);
     }
-    status(fcai_activation_backward(g.p, g.ld, k.m.p, k.m.ld, k.codes, k.scales, ptr(dx), n, ptr(sums), g.rows, (int)n,
+    status(fcai_activation_backward(g.p, g.ld, k.m.p, k.m.ld, k.codes, k.scales, ptr(dx), lddx, ptr(sums), g.rows, (int)n,
                                     dtype_code(like, "an activation"), act, k.keep, ws.get(), bytes, stream_of(like)));
 }
 
@@ -294,7 +295,7 @@ PyObject *py_activation_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (k.m.rows != g.rows) refuse("grad does not fit what was kept");
         if (keep < FCAI_KEEP_INT8) same(grad, "grad", THPVariable_Unpack(a[1]));
         at::Tensor dx = fresh(grad.sizes(), grad);
-        act_backward(grad, g, c, k, act, dx, at::Tensor());
+        act_backward(grad, g, c, k, act, dx, at::Tensor(), c);
         return wrap(dx);
     });
 }
@@ -384,11 +385,12 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (act != FCAI_ACT_NONE) {
             const Kept p = kept_of(a[4], a[5], keep, cout);
             if (p.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
-            dp = fresh({g.rows, cout}, grad);
-            act_backward(grad, g, cout, p, act, dp, db);
-            g = Rows{dp, dp.data_ptr(), cout, g.rows};
+            const int64_t ld = (cout + 7) / 8 * 8;  // rows that the products read without a copy
+            dp = fresh({g.rows, ld}, grad);
+            act_backward(grad, g, cout, p, act, dp, db, ld);
+            g = Rows{dp, dp.data_ptr(), ld, g.rows};
         } else if (needs & 4) {
-            act_backward(grad, g, cout, Kept{}, FCAI_ACT_NONE, at::Tensor(), db);
+            act_backward(grad, g, cout, Kept{}, FCAI_ACT_NONE, at::Tensor(), db, cout);
         }
         const int gpack = unaligned(g.p, g.ld) ? 1 : 0;
         if (needs & 1) {
@@ -406,10 +408,11 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
             dw = fresh({cout, cin}, grad);
             Rows m = x.m;
             if (keep >= FCAI_KEEP_INT8) {
-                at::Tensor v = fresh({x.m.rows, cin}, grad);
-                status(fcai_checkpoint_load(x.codes, x.scales, v.data_ptr(), cin, x.m.rows, (int)cin, dtype, keep, st));
+                const int64_t ld = (cin + 7) / 8 * 8;
+                at::Tensor v = fresh({x.m.rows, ld}, grad);
+                status(fcai_checkpoint_load(x.codes, x.scales, v.data_ptr(), ld, x.m.rows, (int)cin, dtype, keep, st));
                 const void *p = v.data_ptr();
-                m = Rows{std::move(v), p, cin, x.m.rows};
+                m = Rows{std::move(v), p, ld, x.m.rows};
             } else {
                 same(m.hold, "x", grad);
             }

@@ -745,20 +745,49 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
 }
 
 // One or two matrices that TMA cannot read, [rows][cols] with row stride ld,
-// into dst[rows][ldd]: a warp a row.
+// into dst[rows][ldd], 16 bytes a thread and step.  Rows start at any element,
+// so a thread's eight come as 4-byte words: four of them, or, from an odd
+// element on, three between two single elements, shifted together; nothing
+// outside the row is read.
 struct Repack {
     const uint16_t *src;
     uint16_t *dst;
     int64_t ld, rows;
     int cols, ldd;
+    FastDiv chunks;  // of 8 elements a row
 };
+constexpr int kRepackRows = 64;  // rows of a CTA and step
 __global__ void __launch_bounds__(256) repack_kernel(const Repack a, const Repack b) {
     const Repack &o = blockIdx.y ? b : a;
-    for (int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); row < o.rows; row += (int64_t)gridDim.x * 8) {
-        const uint16_t *src = o.src + row * o.ld;
-        uint16_t *dst = o.dst + row * o.ldd;
-#pragma unroll 4
-        for (int c = threadIdx.x & 31; c < o.ldd; c += 32) dst[c] = c < o.cols ? __ldg(src + c) : (uint16_t)0;
+    const int chunks = (int)o.chunks.d;
+    for (int64_t row0 = (int64_t)blockIdx.x * kRepackRows; row0 < o.rows; row0 += (int64_t)gridDim.x * kRepackRows) {
+        const int n = (int)min((int64_t)kRepackRows, o.rows - row0) * chunks;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const int r = divide(i, o.chunks), col = (i - r * chunks) * 8;
+            const uint16_t *src = o.src + (row0 + r) * o.ld + col;
+            uint32_t w[4];
+            if (col + 8 > o.cols) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    w[e] = col + 2 * e < o.cols ? (uint32_t)__ldg(src + 2 * e) : 0u;
+                    if (col + 2 * e + 1 < o.cols) w[e] |= (uint32_t)__ldg(src + 2 * e + 1) << 16;
+                }
+            } else if (reinterpret_cast<uintptr_t>(src) & 2) {
+                const uint32_t first = __ldg(src), end = __ldg(src + 7);
+                const uint32_t *q = reinterpret_cast<const uint32_t *>(src + 1);
+                const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2);
+                w[0] = first | q0 << 16;
+                w[1] = __funnelshift_r(q0, q1, 16);
+                w[2] = __funnelshift_r(q1, q2, 16);
+                w[3] = q2 >> 16 | end << 16;
+            } else {
+                const uint32_t *q = reinterpret_cast<const uint32_t *>(src);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) w[e] = __ldg(q + e);
+            }
+            *reinterpret_cast<uint4 *>(o.dst + (row0 + r) * o.ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
     }
 }
 
@@ -983,14 +1012,14 @@ static int prepare_operands(Operand &a, Operand &b, int dtype, unsigned char *ws
     for (Operand *o : {&a, &b}) {
         if (aligned16(o->ptr, o->ld, dtype)) continue;
         const int ldd = round8(o->cols);
-        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd};
+        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd, fast_div(ldd / 8)};
         rows = std::max(rows, o->rows);
         o->ptr = ws;
         o->ld = ldd;
         ws += repack_bytes(o->rows, o->cols);
     }
     if (!n) return FCAI_OK;
-    const int grid = (int)std::min<int64_t>((rows + 7) / 8, (int64_t)fcai::sm_count() * 16);
+    const int grid = (int)std::min<int64_t>((rows + kRepackRows - 1) / kRepackRows, (int64_t)fcai::sm_count() * 16);
     repack_kernel<<<dim3(grid, n), 256, 0, stream>>>(r[0], r[n - 1]);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;

@@ -18,6 +18,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "layers_common.cuh"
 
@@ -27,7 +28,10 @@ using namespace ly;
 
 constexpr int kThreads = 256;
 constexpr int kBlock = FCAI_KEEP_BLOCK;
-constexpr int kRowsIter = kThreads / 16;  // rows a strip CTA handles at a time
+// Lanes a row of a strip: 16 cover a block of 128 channels; rows of up to 32
+// channels take 4, or most lanes would idle.
+constexpr int strip_lanes(int n) { return n <= 32 ? 4 : 16; }
+constexpr int kRowsIter = kThreads / 16;  // rows a strip CTA handles at a time (with 16 lanes)
 
 // The eight channels a thread holds of its group's 8 * g: consecutive ones where
 // rows take 16-byte accesses (kV), else every g-th, so that neighbouring lanes
@@ -290,7 +294,7 @@ __device__ __forceinline__ void keep_block(int keep, float amax, const V8 &v, ui
 
 // ---- strips: activations, checkpoint load ------------------------------------
 // grid (strips, row shares): the CTAs that run at the same time cover whole rows, which DRAM pages like.
-template <typename T, bool kV>
+template <typename T, bool kV, int kLanes>
 __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
     act_forward_kernel(const T *__restrict__ x, int64_t ldx, T *__restrict__ y, int64_t ldy, uint8_t *__restrict__ codes,
                        float *__restrict__ scales, int64_t rows, int n, int nblk, int act, int keep) {
@@ -299,11 +303,11 @@ __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
     __shared__ __align__(16) unsigned char ring[kV ? kD * Feed::kStep : 16];
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring);
     const int strip = blockIdx.x;
-    const Cols<kV> c(strip * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.y * kRowsIter;
-    const int sub = (threadIdx.x >> 4) & 1;
-    // the loop runs on the warp's first row: a block's shuffles need both halves of the warp
-    int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 5) * 2;
+    const Cols<kV> c(strip * kBlock, threadIdx.x % kLanes, kLanes);
+    const int64_t step = (int64_t)gridDim.y * (kThreads / kLanes);
+    const int sub = (threadIdx.x & 31) / kLanes;
+    // the loop runs on the warp's first row: a block's shuffles need the whole warp
+    int64_t r0 = (int64_t)blockIdx.y * (kThreads / kLanes) + (threadIdx.x >> 5) * (32 / kLanes);
     Feed feed;
 #pragma unroll
     for (int d = 0; d < kD; ++d) {
@@ -316,7 +320,7 @@ __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
         V8 v = raw.get();
         const int64_t row = r0 + sub;
         const bool in = row < rows;
-        if (keep != FCAI_KEEP_NONE) keep_block<16>(keep, raw.amax(), v, codes + row * n, scales + row * nblk + strip, c, n, in);
+        if (keep != FCAI_KEEP_NONE) keep_block<kLanes>(keep, raw.amax(), v, codes + row * n, scales + row * nblk + strip, c, n, in);
         feed.issue(base + slot * Feed::kStep, 0, x, (row + kD * step) * ldx, c, n, row + kD * step < rows);
         cp_commit();
         if (y) {
@@ -328,12 +332,12 @@ __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
 }
 
 constexpr int kLoadRows = 2;  // rows a thread has in flight: 8 + 4 bytes a row are too little for the ring to pay
-template <typename T, bool kV>
+template <typename T, bool kV, int kLanes>
 __global__ void __launch_bounds__(kThreads, kV ? 6 : 4)
     checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
-    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.y * kRowsIter;
-    for (int64_t r0 = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4); r0 < rows; r0 += step * kLoadRows) {
+    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x % kLanes, kLanes);
+    const int64_t step = (int64_t)gridDim.y * (kThreads / kLanes);
+    for (int64_t r0 = (int64_t)blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes; r0 < rows; r0 += step * kLoadRows) {
         KeptRaw<T, kV, true> raw[kLoadRows];
 #pragma unroll
         for (int u = 0; u < kLoadRows; ++u) raw[u].load(k, r0 + u * step, c, n, nblk, r0 + u * step < rows);
@@ -368,7 +372,7 @@ __device__ __forceinline__ void group_sums(const V8 &sums, float *partial_row, i
 }
 
 // dx = dy act'(x) and partial sums of it over the CTA's rows; kAct: x is read
-template <typename T, bool kV, bool k8, bool kAct>
+template <typename T, bool kV, bool k8, bool kAct, int kLanes>
 __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
                         float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
@@ -380,10 +384,10 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
     // the sums meet in the ring's memory when the rows are through
     __shared__ __align__(16) unsigned char ring[kV && kD * kStep > kSums ? kD * kStep : kSums];
     const uint32_t base = (uint32_t)__cvta_generic_to_shared(ring);
-    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x & 15, 16);
-    const int64_t step = (int64_t)gridDim.y * kRowsIter;
+    const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x % kLanes, kLanes);
+    const int64_t step = (int64_t)gridDim.y * (kThreads / kLanes);
     V8 acc = {f2(0.f), f2(0.f), f2(0.f), f2(0.f)};
-    int64_t row = (int64_t)blockIdx.y * kRowsIter + (threadIdx.x >> 4);
+    int64_t row = (int64_t)blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes;
     FeedG feed_g;
     FeedX feed_x;
     auto issue = [&](int slot, int64_t r) {
@@ -405,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
     }
     cp_wait<0>();
     if (partial) {
-        group_sums<16, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, reinterpret_cast<float *>(ring));
+        group_sums<kLanes, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, reinterpret_cast<float *>(ring));
     }
 }
 
@@ -856,8 +860,8 @@ static bool codes_vec(const void *codes, int n) { return !codes || ((reinterpret
 // Row shares of the strip kernels: enough CTAs to fill the device, and from
 // there on CTAs of 16 steps of 16 rows, long enough for the ring to run full and
 // for partial sums to be few, short enough to end evenly.
-static int row_shares(int64_t rows, int strips) {
-    const int64_t steps = (rows + kRowsIter - 1) / kRowsIter;
+static int row_shares(int64_t rows, int strips, int lanes = 16) {
+    const int64_t steps = (rows + kThreads / lanes - 1) / (kThreads / lanes);
     const int64_t fill = std::max<int64_t>(1, ((int64_t)fcai::sm_count() * 4 + strips - 1) / strips);
     return (int)std::min<int64_t>(steps <= fill ? steps : std::max(fill, (steps + 15) / 16), 65535);
 }
@@ -884,7 +888,7 @@ static int norm_backward_grid(int64_t rows, int n) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
 }
 static int64_t act_workspace(int64_t rows, int n) {
-    return rows ? round256((int64_t)row_shares(rows, blocks_of(n)) * n * 4) : 0;
+    return rows ? round256((int64_t)row_shares(rows, blocks_of(n), strip_lanes(n)) * n * 4) : 0;
 }
 static int64_t norm_workspace(int64_t rows, int n) {
     if (rows == 0) return 0;
@@ -939,8 +943,9 @@ static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *c
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
     const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
     const int strips = blocks_of(n);
-    const dim3 grid(strips, row_shares(rows, strips));
-    auto kernel = vec ? act_forward_kernel<T, true> : act_forward_kernel<T, false>;
+    const dim3 grid(strips, row_shares(rows, strips, strip_lanes(n)));
+    auto kernel = strip_lanes(n) == 4 ? (vec ? act_forward_kernel<T, true, 4> : act_forward_kernel<T, false, 4>)
+                                      : (vec ? act_forward_kernel<T, true, 16> : act_forward_kernel<T, false, 16>);
     kernel<<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales,
                                       rows, n, strips, act, q ? keep : FCAI_KEEP_NONE);
     FCAI_CUDA_TRY(cudaGetLastError());
@@ -949,13 +954,17 @@ static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *c
 template <typename T>
 static int act_backward(const void *dy, int64_t lddy, const Kept &k, void *dx, int64_t lddx, void *bias_grad, int64_t rows, int n,
                         int dtype, int act, float *ws, cudaStream_t st) {
-    const int strips = blocks_of(n), shares = row_shares(rows, strips);
+    const int strips = blocks_of(n), shares = row_shares(rows, strips, strip_lanes(n));
     const bool k8 = act != FCAI_ACT_NONE && k.keep != FCAI_KEEP_FULL;
     const bool vec = n % 8 == 0 && aligned16(dy, lddy, dtype) && (!dx || aligned16(dx, lddx, dtype)) &&
                      (act == FCAI_ACT_NONE || (k8 ? codes_vec(k.codes, n) : aligned16(k.x, k.ldx, dtype)));
-    auto kernel = act == FCAI_ACT_NONE ? (vec ? act_backward_kernel<T, true, false, false> : act_backward_kernel<T, false, false, false>)
-                  : k8 ? (vec ? act_backward_kernel<T, true, true, true> : act_backward_kernel<T, false, true, true>)
-                       : (vec ? act_backward_kernel<T, true, false, true> : act_backward_kernel<T, false, false, true>);
+    auto pick = [&](auto lanes) {
+        constexpr int kL = decltype(lanes)::value;
+        return act == FCAI_ACT_NONE ? (vec ? act_backward_kernel<T, true, false, false, kL> : act_backward_kernel<T, false, false, false, kL>)
+               : k8 ? (vec ? act_backward_kernel<T, true, true, true, kL> : act_backward_kernel<T, false, true, true, kL>)
+                    : (vec ? act_backward_kernel<T, true, false, true, kL> : act_backward_kernel<T, false, false, true, kL>);
+    };
+    auto kernel = strip_lanes(n) == 4 ? pick(std::integral_constant<int, 4>()) : pick(std::integral_constant<int, 16>());
     kernel<<<dim3(strips, shares), kThreads, 0, st>>>(static_cast<const T *>(dy), lddy, k, static_cast<T *>(dx), lddx,
                                                       bias_grad ? ws : nullptr, rows, n, strips, act);
     FCAI_CUDA_TRY(cudaGetLastError());
@@ -965,8 +974,9 @@ template <typename T>
 static int load_checkpoint(const Kept &k, void *out, int64_t ldo, int64_t rows, int n, int dtype, cudaStream_t st) {
     const bool vec = n % 8 == 0 && aligned16(out, ldo, dtype) && codes_vec(k.codes, n);
     const int strips = blocks_of(n);
-    auto kernel = vec ? checkpoint_load_kernel<T, true> : checkpoint_load_kernel<T, false>;
-    kernel<<<dim3(strips, row_shares(rows, strips)), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
+    auto kernel = strip_lanes(n) == 4 ? (vec ? checkpoint_load_kernel<T, true, 4> : checkpoint_load_kernel<T, false, 4>)
+                                      : (vec ? checkpoint_load_kernel<T, true, 16> : checkpoint_load_kernel<T, false, 16>);
+    kernel<<<dim3(strips, row_shares(rows, strips, strip_lanes(n))), kThreads, 0, st>>>(k, static_cast<T *>(out), ldo, rows, n, strips);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
