@@ -655,7 +655,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
 // accesses.
 template <typename T, int kParts>
 __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
-    __shared__ float sums[kParts > 1 ? 16 : 1][kParts > 1 ? 128 : 1];
+    __shared__ __align__(16) float sums[16][128];  // the parts' sums; rows on their way to narrow stores
     constexpr int kRows = 16 / kParts;  // rows a CTA and step
     const int group = threadIdx.x >> 4, split0 = group / kRows;
     const int col = blockIdx.x * FCAI_KEEP_BLOCK + (threadIdx.x & 15) * 8;
@@ -704,6 +704,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
                 }
             }
         }
+        uint2 codes = make_uint2(0u, 0u);
         if (p.codes) {
             // columns from N on are zeros: their weights were, and no bias was added
             float m = in ? amax8(v) : 0.f;
@@ -712,19 +713,13 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
             if (in) {
                 const float s = keep_scale(p.keep, m);
                 const uint2 q = keep_codes(p.keep, V8{v[0], v[1], v[2], v[3]}, s);
-                uint8_t *dst = p.codes + row * p.N + col;
-                if (p.vec) {
-                    *reinterpret_cast<uint2 *>(dst) = q;
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        if (col + e < p.N) dst[e] = (uint8_t)((e < 4 ? q.x : q.y) >> (8 * (e & 3)));
-                }
+                if (p.vec) *reinterpret_cast<uint2 *>(p.codes + row * p.N + col) = q;
+                codes = q;
                 if ((threadIdx.x & 15) == 0) p.scales[row * p.nblk + blockIdx.x] = s;
             }
         }
-        if (!in) continue;
         if (p.vec) {
+            if (!in) continue;
             if (p.pre) *reinterpret_cast<uint4 *>(static_cast<T *>(p.pre) + row * p.ldpre + col) = pack8<T>(v);
             act_n(p.act, v);
             if (p.residual) {
@@ -735,11 +730,50 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
             }
             *reinterpret_cast<uint4 *>(static_cast<T *>(p.y) + row * p.ldy + col) = pack8<T>(v);
         } else {
+            // narrow accesses: the row through shared memory, so that neighbouring lanes have neighbouring columns
+            float *mine = sums[group];
+            const int l = threadIdx.x & 15;
+            auto put = [&]() {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 f = split(v[e]);
+                    mine[l * 8 + 2 * e] = f.x, mine[l * 8 + 2 * e + 1] = f.y;
+                }
+            };
+            const bool here = row < p.M && (kParts == 1 || split0 == 0);
+            __syncwarp();
+            if (p.codes) {
+                reinterpret_cast<uint2 *>(mine)[l] = codes;
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = blockIdx.x * FCAI_KEEP_BLOCK + l + 16 * e;
+                    if (here && c < p.N) p.codes[row * p.N + c] = reinterpret_cast<const uint8_t *>(mine)[l + 16 * e];
+                }
+                __syncwarp();
+            }
+            if (p.pre) {
+                put();
+                __syncwarp();
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const int c = blockIdx.x * FCAI_KEEP_BLOCK + l + 16 * e;
+                    if (here && c < p.N) static_cast<T *>(p.pre)[row * p.ldpre + c] = from_f32<T>(mine[l + 16 * e]);
+                }
+                __syncwarp();
+            }
+            act_n(p.act, v);
+            put();
+            __syncwarp();
 #pragma unroll
             for (int e = 0; e < 8; ++e) {
-                const float2 f = split(v[e / 2]);
-                if (col + e < p.N) finish1<T>(p, row, col + e, e & 1 ? f.y : f.x);
+                const int c = blockIdx.x * FCAI_KEEP_BLOCK + l + 16 * e;
+                if (!here || c >= p.N) continue;
+                const float r = p.residual ? to_f32(static_cast<const T *>(p.residual)[row * p.ldr + c]) : 0.f;
+                static_cast<T *>(p.y)[row * p.ldy + c] = from_f32<T>(mine[l + 16 * e] + r);
             }
+            if constexpr (kParts > 1) __syncthreads();  // the rows' sums come to the same memory
+            else __syncwarp();
         }
     }
 }
@@ -755,13 +789,13 @@ struct Repack {
     int64_t ld, rows;
     int cols, ldd;
     FastDiv chunks;  // of 8 elements a row
+    int step;        // rows of a CTA and step: about 2048 chunks
 };
-constexpr int kRepackRows = 64;  // rows of a CTA and step
 __global__ void __launch_bounds__(256) repack_kernel(const Repack a, const Repack b) {
     const Repack &o = blockIdx.y ? b : a;
     const int chunks = (int)o.chunks.d;
-    for (int64_t row0 = (int64_t)blockIdx.x * kRepackRows; row0 < o.rows; row0 += (int64_t)gridDim.x * kRepackRows) {
-        const int n = (int)min((int64_t)kRepackRows, o.rows - row0) * chunks;
+    for (int64_t row0 = (int64_t)blockIdx.x * o.step; row0 < o.rows; row0 += (int64_t)gridDim.x * o.step) {
+        const int n = (int)min((int64_t)o.step, o.rows - row0) * chunks;
 #pragma unroll 2
         for (int i = threadIdx.x; i < n; i += 256) {
             const int r = divide(i, o.chunks), col = (i - r * chunks) * 8;
@@ -1008,18 +1042,19 @@ static int elementwise_grid(int64_t n, int threads) {
 static int prepare_operands(Operand &a, Operand &b, int dtype, unsigned char *ws, cudaStream_t stream) {
     Repack r[2];
     int n = 0;
-    int64_t rows = 0;
+    int64_t steps = 0;
     for (Operand *o : {&a, &b}) {
         if (aligned16(o->ptr, o->ld, dtype)) continue;
         const int ldd = round8(o->cols);
-        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd, fast_div(ldd / 8)};
-        rows = std::max(rows, o->rows);
+        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd, fast_div(ldd / 8),
+                  std::max(1, std::min(64, 2048 / (ldd / 8)))};
+        steps = std::max(steps, (o->rows + r[n - 1].step - 1) / r[n - 1].step);
         o->ptr = ws;
         o->ld = ldd;
         ws += repack_bytes(o->rows, o->cols);
     }
     if (!n) return FCAI_OK;
-    const int grid = (int)std::min<int64_t>((rows + kRepackRows - 1) / kRepackRows, (int64_t)fcai::sm_count() * 16);
+    const int grid = (int)std::min<int64_t>(steps, (int64_t)fcai::sm_count() * 16);
     repack_kernel<<<dim3(grid, n), 256, 0, stream>>>(r[0], r[n - 1]);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
