@@ -338,9 +338,10 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         }
         const Rows m = rows_of(x, cin), wm = rows_of(w, cin);
         at::Tensor y = fresh(shape, x), pre;
+        const int64_t ldpre = (cout + 7) / 8 * 8;  // pre: padded rows, which leave the kernel (and enter the backward pass) in wide accesses
         Codes k;
         const int kp = act == FCAI_ACT_NONE ? FCAI_KEEP_NONE : keep;  // what of the activation's input is kept
-        if (kp == FCAI_KEEP_FULL) pre = fresh(shape, x);
+        if (kp == FCAI_KEEP_FULL) pre = fresh({m.rows, ldpre}, x);
         if (kp >= FCAI_KEEP_INT8) {
             k = new_codes(x, m.rows, cout);
             if (cout % 8 == 0) {  // the codes leave with y's rows, in wide accesses
@@ -352,14 +353,15 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
                 }
             }
         }
-        const int repack = (unaligned(m.p, m.ld) ? 1 : 0) | (unaligned(wm.p, wm.ld) ? 2 : 0);
+        const int repack = (unaligned(m.p, m.ld) ? 1 : 0) | (unaligned(wm.p, wm.ld) ? 2 : 0) | (unaligned(y.data_ptr(), cout) ? 4 : 0) |
+                           (r.p && unaligned(r.p, r.ld) ? 8 : 0);
         const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_FORWARD, m.rows, (int)cin, (int)cout, repack, kp);
         const Scratch ws = scratch(bytes);
-        status(fcai_linear_forward(m.p, m.ld, wm.p, wm.ld, ptr(bias), r.p, r.ld, y.data_ptr(), cout, ptr(pre), cout, ptr(k.codes),
+        status(fcai_linear_forward(m.p, m.ld, wm.p, wm.ld, ptr(bias), r.p, r.ld, y.data_ptr(), cout, ptr(pre), ldpre, ptr(k.codes),
                                    static_cast<float *>(ptr(k.scales)), m.rows, (int)cin, (int)cout, dtype_code(x, "linear"), act, kp,
                                    ws.get(), bytes, stream_of(x)));
         if (keep == FCAI_KEEP_NONE) return wrap(y);
-        if (keep == FCAI_KEEP_FULL) return wrap_all(y, pre);
+        if (keep == FCAI_KEEP_FULL) return wrap_all(y, pre.defined() && ldpre != cout ? pre.narrow(1, 0, cout) : pre);
         const Codes kx = save8(x, m, cin, keep);
         return wrap_all(y, kx.codes, kx.scales, k.codes, k.scales);
     });
@@ -399,7 +401,7 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
             dx = fresh(shape, grad);
             const Rows wm = rows_of(w, cin);
             const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_BACKWARD_INPUT, g.rows, (int)cin, (int)cout,
-                                                        gpack | (unaligned(wm.p, wm.ld) ? 2 : 0), 0);
+                                                        gpack | (unaligned(wm.p, wm.ld) ? 2 : 0) | (unaligned(dx.data_ptr(), cin) ? 4 : 0), 0);
             const Scratch ws = scratch(bytes);
             status(fcai_linear_backward_input(g.p, g.ld, wm.p, wm.ld, dx.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ws.get(),
                                               bytes, st));
@@ -417,7 +419,7 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
                 same(m.hold, "x", grad);
             }
             const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, g.rows, (int)cin, (int)cout,
-                                                        gpack | (unaligned(m.p, m.ld) ? 2 : 0), 0);
+                                                        gpack | (unaligned(m.p, m.ld) ? 2 : 0) | (unaligned(dw.data_ptr(), cin) ? 4 : 0), 0);
             const Scratch ws = scratch(bytes);
             status(fcai_linear_backward_weight(g.p, g.ld, m.p, m.ld, dw.data_ptr(), cin, g.rows, (int)cin, (int)cout, dtype, ws.get(),
                                                bytes, st));

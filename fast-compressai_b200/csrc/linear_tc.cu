@@ -48,6 +48,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <initializer_list>
 #include <mutex>
 
 #include "layers_common.cuh"
@@ -89,7 +90,8 @@ struct Params {
     int units;
     int ldp;                             // partial tiles: row stride (N rounded up to 8)
     int coop;                            // all epilogue warps on each tile
-    int vec;                             // y, residual, pre, bias and codes take wide accesses
+    int vec;                             // N % 8 == 0, and y, residual, pre, bias and codes take wide accesses
+    int tma, bias_vec;                   // y, residual, pre and codes are tiles of tensor maps; bias takes wide accesses
     int act;
     const void *bias, *residual;
     void *y, *pre;
@@ -218,11 +220,18 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
 template <typename T>
 __device__ __forceinline__ void add_bias32(const Params &p, int col0, F2 (&v)[16]) {
     if (!p.bias) return;
+    const T *bias = static_cast<const T *>(p.bias) + col0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
-        if (col0 + 8 * g >= p.N) break;  // N is a multiple of 8
+        if (col0 + 8 * g >= p.N) break;
         F2 b[4];
-        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.bias) + col0 + 8 * g)), b);
+        if (p.bias_vec && col0 + 8 * g + 8 <= p.N) {
+            unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(bias + 8 * g)), b);
+        } else {
+            auto at = [&](int c) { return col0 + c < p.N ? to_f32(bias[c]) : 0.f; };
+#pragma unroll
+            for (int e = 0; e < 4; ++e) b[e] = f2(at(8 * g + 2 * e), at(8 * g + 2 * e + 1));
+        }
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * g + e] = add2(v[4 * g + e], b[e]);
     }
@@ -489,7 +498,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
         const uint32_t extra = staging + kStagingWarp;
         const uint32_t stg = staging + lane * 128 + ((lane & 7) << 4);  // this row of an fp32 tile, chunk 0
         const uint32_t rbar = smem_u32(&resbar[2 * warp]);
-        const bool tma = p.vec && !p.partial, residual = tma && p.residual;
+        const bool tma = p.tma, residual = tma && p.residual;
         uint32_t n = 0;  // chunks through the two tiles so far
         // Lane 0: the residual's rows and columns of chunk `i` into tile i % 2,
         // whose last store (chunk i - 2) has been read.
@@ -778,7 +787,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
     }
 }
 
-// One or two matrices that TMA cannot read, [rows][cols] with row stride ld,
+// Up to three matrices that TMA cannot read, [rows][cols] with row stride ld,
 // into dst[rows][ldd], 16 bytes a thread and step.  Rows start at any element,
 // so a thread's eight come as 4-byte words: four of them, or, from an odd
 // element on, three between two single elements, shifted together; nothing
@@ -791,8 +800,11 @@ struct Repack {
     FastDiv chunks;  // of 8 elements a row
     int step;        // rows of a CTA and step: about 2048 chunks
 };
-__global__ void __launch_bounds__(256) repack_kernel(const Repack a, const Repack b) {
-    const Repack &o = blockIdx.y ? b : a;
+struct Repacks {
+    Repack r[3];
+};
+__global__ void __launch_bounds__(256) repack_kernel(const Repacks all) {
+    const Repack &o = all.r[blockIdx.y];
     const int chunks = (int)o.chunks.d;
     for (int64_t row0 = (int64_t)blockIdx.x * o.step; row0 < o.rows; row0 += (int64_t)gridDim.x * o.step) {
         const int n = (int)min((int64_t)o.step, o.rows - row0) * chunks;
@@ -821,6 +833,54 @@ __global__ void __launch_bounds__(256) repack_kernel(const Repack a, const Repac
                 for (int e = 0; e < 4; ++e) w[e] = __ldg(q + e);
             }
             *reinterpret_cast<uint4 *>(o.dst + (row0 + r) * o.ldd + col) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+}
+
+// The way back: padded rows src[rows][lds] to dst[rows][cols] with row stride ldd,
+// whose rows start at any element.  A thread's 16 bytes are aligned in dst, so
+// that all but a row's first and last sectors are written whole; the direct narrow
+// stores left most sectors partial, and the backward pass of 28106 x 1730 -> 24 took
+// 197 us instead of 167.
+struct Unpad {
+    const uint16_t *src;
+    uint16_t *dst;
+    int64_t lds, ldd, rows;
+    int cols;
+    FastDiv chunks;  // aligned 16-byte pieces of a row: one more than its length asks for
+    int step;        // rows of a CTA and step
+};
+__global__ void __launch_bounds__(256) unpad_kernel(const Unpad o) {
+    const int chunks = (int)o.chunks.d;
+    for (int64_t row0 = (int64_t)blockIdx.x * o.step; row0 < o.rows; row0 += (int64_t)gridDim.x * o.step) {
+        const int n = (int)min((int64_t)o.step, o.rows - row0) * chunks;
+#pragma unroll 2
+        for (int i = threadIdx.x; i < n; i += 256) {
+            const int r = divide(i, o.chunks);
+            uint16_t *dst = o.dst + (row0 + r) * o.ldd;
+            const int col = (i - r * chunks) * 8 - (int)((reinterpret_cast<uintptr_t>(dst) & 15) >> 1);
+            const uint16_t *src = o.src + (row0 + r) * o.lds + col;
+            if (col >= 0 && col + 8 <= o.cols) {
+                uint32_t w[4];
+                if (col & 1) {
+                    const uint32_t first = __ldg(src), end = __ldg(src + 7);
+                    const uint32_t *q = reinterpret_cast<const uint32_t *>(src + 1);
+                    const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2);
+                    w[0] = first | q0 << 16;
+                    w[1] = __funnelshift_r(q0, q1, 16);
+                    w[2] = __funnelshift_r(q1, q2, 16);
+                    w[3] = q2 >> 16 | end << 16;
+                } else {
+                    const uint32_t *q = reinterpret_cast<const uint32_t *>(src);
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) w[e] = __ldg(q + e);
+                }
+                *reinterpret_cast<uint4 *>(dst + col) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (col + e >= 0 && col + e < o.cols) dst[col + e] = __ldg(src + e);
+            }
         }
     }
 }
@@ -1038,27 +1098,33 @@ static int elementwise_grid(int64_t n, int threads) {
     return (int)std::max<int64_t>(1, std::min<int64_t>((n + threads - 1) / threads, (int64_t)fcai::sm_count() * 8));
 }
 
-// Makes both operands readable by TMA, from the workspace if they have to be copied.
-static int prepare_operands(Operand &a, Operand &b, int dtype, unsigned char *ws, cudaStream_t stream) {
-    Repack r[2];
+static int rows_a_step(int chunks) { return std::max(1, std::min(64, 2048 / chunks)); }
+// Makes matrices readable by TMA, from the workspace if they have to be copied.
+static int prepare_operands(std::initializer_list<Operand *> all, int dtype, unsigned char *&ws, cudaStream_t stream) {
+    Repacks r{};
     int n = 0;
     int64_t steps = 0;
-    for (Operand *o : {&a, &b}) {
-        if (aligned16(o->ptr, o->ld, dtype)) continue;
-        const int ldd = round8(o->cols);
-        r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd, fast_div(ldd / 8),
-                  std::max(1, std::min(64, 2048 / (ldd / 8)))};
-        steps = std::max(steps, (o->rows + r[n - 1].step - 1) / r[n - 1].step);
+    for (Operand *o : all) {
+        if (!o->ptr || aligned16(o->ptr, o->ld, dtype)) continue;
+        const int ldd = round8(o->cols), step = rows_a_step(ldd / 8);
+        r.r[n++] = {static_cast<const uint16_t *>(o->ptr), reinterpret_cast<uint16_t *>(ws), o->ld, o->rows, o->cols, ldd,
+                    fast_div(ldd / 8), step};
+        steps = std::max(steps, (o->rows + step - 1) / step);
         o->ptr = ws;
         o->ld = ldd;
         ws += repack_bytes(o->rows, o->cols);
     }
     if (!n) return FCAI_OK;
     const int grid = (int)std::min<int64_t>(steps, (int64_t)fcai::sm_count() * 16);
-    repack_kernel<<<dim3(grid, n), 256, 0, stream>>>(r[0], r[n - 1]);
+    repack_kernel<<<dim3(grid, n), 256, 0, stream>>>(r);
     FCAI_CUDA_TRY(cudaGetLastError());
     return FCAI_OK;
 }
+// Outputs of at least this many elements go through padded rows when their own
+// are not 16-byte aligned; below, the second launch and pass cost more than the
+// narrow stores (4000 x 1027 from 2023: 52 against 48 us; 20000 x 333 from 501: 44
+// against 50).
+constexpr int64_t kPadFrom = 6 << 20;
 
 template <typename T, int kBN, bool kPair, bool kTA, bool kTB, bool kKeep>
 static int launch(const Maps &maps, const Params &p, cudaStream_t stream) {
@@ -1148,13 +1214,31 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
         p.partial = reinterpret_cast<float *>(ws);
         ws += pl.partial_bytes;
     }
+    // unaligned results and residual: through copies with padded rows, or (few elements, or a split product) narrow accesses
+    const bool y_aligned = aligned16(p.y, p.ldy, dtype), r_aligned = !p.residual || aligned16(p.residual, p.ldr, dtype);
+    const bool pad = !p.partial && M * N >= kPadFrom && (!y_aligned || !r_aligned);
+    p.tma = !p.partial && (pad || (y_aligned && r_aligned)) && (!p.pre || aligned16(p.pre, p.ldpre, dtype));
+    p.bias_vec = !p.bias || aligned16(p.bias, 0, dtype);
+    Operand R{p.tma ? p.residual : nullptr, p.ldr, M, N};
     int rc;
-    if ((rc = prepare_operands(A, B, dtype, ws, stream))) return rc;
+    if ((rc = prepare_operands({&A, &B, &R}, dtype, ws, stream))) return rc;
+    Unpad back{};
+    if (p.tma) {
+        p.residual = R.ptr;
+        p.ldr = R.ld;
+        if (!y_aligned) {
+            const int chunks = (N + 7) / 8 + 1;
+            back = {reinterpret_cast<const uint16_t *>(ws), static_cast<uint16_t *>(p.y), round8(N), p.ldy, M, N, fast_div(chunks),
+                    rows_a_step(chunks)};
+            p.y = ws;
+            p.ldy = round8(N);
+        }
+    }
     Maps maps;
     if ((rc = make_map(&maps.a, A.ptr, A.cols, A.rows, A.ld, kTA ? kBK : kBM, dtype))) return rc;
     if ((rc = make_map(&maps.b, B.ptr, B.cols, B.rows, B.ld, kTB ? kBK : pl.pair ? pl.bn / 2 : pl.bn, dtype))) return rc;
-    const bool tma = p.vec && !p.partial, keep = !kTA && !kTB && tma && (p.pre || p.codes);
-    if (tma) {
+    const bool keep = !kTA && !kTB && p.tma && (p.pre || p.codes);
+    if (p.tma) {
         if ((rc = make_map(&maps.y, p.y, N, M, p.ldy, 32, dtype, 32))) return rc;
         if (p.residual && (rc = make_map(&maps.res, p.residual, N, M, p.ldr, 32, dtype, 32))) return rc;
         if (p.codes && (rc = make_map(&maps.extra, p.codes, N, M, N, 32, kCodeType, 32))) return rc;
@@ -1168,6 +1252,10 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     else rc = LN_LAUNCH(false);
 #undef LN_LAUNCH
     if (rc) return rc;
+    if (back.src) {
+        unpad_kernel<<<(int)std::min<int64_t>((M + back.step - 1) / back.step, (int64_t)fcai::sm_count() * 16), 256, 0, stream>>>(back);
+        FCAI_CUDA_TRY(cudaGetLastError());
+    }
     return p.partial ? launch_reduce<T>(p, stream) : FCAI_OK;
 }
 
@@ -1219,33 +1307,29 @@ static int check_common(int64_t rows, int cin, int cout, int dtype, const void *
 
 static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repack, int keep) {
     if (rows < 0 || rows > 0x7FFFFFFF - 256 || cin < 1 || cout < 1 || cin > (1 << 24) || cout > (1 << 24)) return -1;
+    if (op < FCAI_LINEAR_FORWARD || op > FCAI_LINEAR_BACKWARD_WEIGHT) return -1;
     if (rows == 0) return 0;
-    int64_t n;
-    switch (op) {
-        case FCAI_LINEAR_FORWARD:
-            if (rows <= kFewRows) return keep >= FCAI_KEEP_INT8 ? round256(rows * round8(cout) * 4) : 0;
-            if (keep >= FCAI_KEEP_INT8) n = make_plan(rows, cout, cin, cout % 16 != 0, true).partial_bytes;
-            else n = make_plan(rows, cout, cin).partial_bytes;
-            if (repack & 1) n += repack_bytes(rows, cin);
-            if (repack & 2) n += repack_bytes(cout, cin);
-            return n;
-        case FCAI_LINEAR_BACKWARD_INPUT:
-            n = make_plan(rows, cin, cout).partial_bytes;
-            if (repack & 1) n += repack_bytes(rows, cout);
-            if (repack & 2) n += repack_bytes(cout, cin);
-            return n;
-        case FCAI_LINEAR_BACKWARD_WEIGHT:
-            n = make_plan(cout, cin, rows).partial_bytes;
-            if (repack & 1) n += repack_bytes(rows, cout);
-            if (repack & 2) n += repack_bytes(rows, cin);
-            return n;
-        default:
-            return -1;
+    const bool forward = op == FCAI_LINEAR_FORWARD, weight = op == FCAI_LINEAR_BACKWARD_WEIGHT;
+    const bool k8 = forward && keep >= FCAI_KEEP_INT8;
+    if (forward && rows <= kFewRows) return k8 ? round256(rows * round8(cout) * 4) : 0;
+    // the product's sizes, and its operands'
+    const int64_t M = weight ? cout : rows, K = weight ? rows : forward ? cin : cout, a_rows = rows, b_rows = weight ? rows : cout;
+    const int N = forward ? cout : cin, a_cols = forward ? cin : cout, b_cols = cin;
+    const int64_t partial = make_plan(M, N, K, k8 && cout % 16 != 0, k8).partial_bytes;
+    int64_t n = partial;
+    if (repack & 1) n += repack_bytes(a_rows, a_cols);
+    if (repack & 2) n += repack_bytes(b_rows, b_cols);
+    if (!partial && M * N >= kPadFrom) {
+        if (repack & 4) n += repack_bytes(M, N);
+        if (repack & 8) n += repack_bytes(M, N);
     }
+    return n;
 }
 static int check_workspace(int op, int64_t rows, int cin, int cout, const void *a, int64_t lda, const void *b, int64_t ldb,
-                           int dtype, int keep, const void *ws, int64_t bytes) {
-    const int repack = (aligned16(a, lda, dtype) ? 0 : 1) | (aligned16(b, ldb, dtype) ? 0 : 2);
+                           const void *y, int64_t ldy, const void *residual, int64_t ldr, int dtype, int keep, const void *ws,
+                           int64_t bytes) {
+    const int repack = (aligned16(a, lda, dtype) ? 0 : 1) | (aligned16(b, ldb, dtype) ? 0 : 2) | (aligned16(y, ldy, dtype) ? 0 : 4) |
+                       (!residual || aligned16(residual, ldr, dtype) ? 0 : 8);
     const int64_t need = workspace_bytes(op, rows, cin, cout, repack, keep);
     if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
         return fcai::fail(FCAI_ERR_WORKSPACE, "linear: needs a 256-byte aligned workspace of %lld bytes", (long long)need);
@@ -1291,7 +1375,8 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     p.keep = keep;
     if (k8 && rows > kFewRows && cout % 8 == 0 && !wide_outputs(p, cout, dtype))
         return fcai::fail(FCAI_ERR_INVALID, "linear: codes need 16-byte aligned y, bias and residual rows, and 16-byte aligned codes");
-    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, dtype, keep, workspace, workspace_bytes)))
+    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, y, ldy, residual, ldr, dtype, keep, workspace,
+                              workspace_bytes)))
         return rc;
     const Operand A{x, ldx, rows, cin}, B{w, ldw, cout, cin};
     auto *ws = static_cast<unsigned char *>(workspace);
@@ -1314,7 +1399,7 @@ int fcai_linear_backward_input(const void *dp, int64_t lddp, const void *w, int6
     if (rc) return rc;
     if (rows == 0) return FCAI_OK;
     if (!dp || !w || !dx) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dtype, 0, workspace,
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dx, lddx, nullptr, 0, dtype, 0, workspace,
                               workspace_bytes)))
         return rc;
     Params p{};
@@ -1347,7 +1432,7 @@ int fcai_linear_backward_weight(const void *dp, int64_t lddp, const void *x, int
         FCAI_CUDA_TRY(cudaGetLastError());
         return FCAI_OK;
     }
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dtype, 0, workspace,
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dw, lddw, nullptr, 0, dtype, 0, workspace,
                               workspace_bytes)))
         return rc;
     const Operand A{dp, lddp, rows, cout}, B{x, ldx, rows, cin};

@@ -59,9 +59,10 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
  * 8, the addresses and strides of y, bias and residual, and codes, are 16-byte
  * aligned. */
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
-/* `repack`: bit 0 / bit 1 set when the call's first / second matrix is not
- * 16-byte aligned in address and row stride (x, w; dp, w; dp, x); `keep`: the
- * forward call's (0 for the others). */
+/* `repack`: bits set for matrices of the call that are not 16-byte aligned in
+ * address and row stride: 1 the first operand (x; dp; dp), 2 the second (w; w;
+ * x), 4 the output (y; dx; dw), 8 the residual.  `keep`: the forward call's (0
+ * for the others). */
 int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack, int32_t keep);
 int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                         const void *residual, int64_t ldr, void *y, int64_t ldy, void *pre, int64_t ldpre,

@@ -77,7 +77,7 @@ def test_linear_strided(cuda_device, rows, cin, cout, which):
 
 @pytest.mark.parametrize("rows,cin,cout", [(1, 64, 40), (7, 33, 65), (130, 64, 128), (129, 321, 577), (1000, 192, 320),
                                            (20000, 128, 64), (5000, 24, 8), (300, 1032, 2056), (16, 4096, 128),
-                                           (70001, 16, 40)])
+                                           (70001, 16, 40), (6001, 333, 100), (901, 1001, 577), (20001, 333, 100)])
 @pytest.mark.parametrize("dtype", T16)
 @pytest.mark.parametrize("kind", ["none", "relu", "gelu", "silu"])
 def test_linear_backward(cuda_device, rows, cin, cout, dtype, kind):
@@ -122,7 +122,8 @@ def test_linear_kept_in_8_bits(cuda_device, rows, cin, cout, fmt, dtype):
 # residual and everything kept at once: results and what is kept leave through different tiles of the same epilogue;
 # 20000 x 512 gives every CTA several tiles, widths that are no multiple of 16 or 8 take the other ways out
 @pytest.mark.parametrize("rows,cin,cout", [(20, 64, 72), (40, 64, 24), (300, 200, 136), (333, 72, 96), (700, 264, 577),
-                                           (5000, 64, 1040), (20000, 128, 512), (20001, 96, 264)])
+                                           (5000, 64, 1040), (20000, 128, 512), (20001, 96, 264), (2001, 72, 333),
+                                           (1000, 100, 1030), (20001, 72, 333)])
 @pytest.mark.parametrize("keep", layers.KEEPS)
 @pytest.mark.parametrize("dtype", T16)
 def test_linear_residual_and_keep(cuda_device, rows, cin, cout, keep, dtype):
