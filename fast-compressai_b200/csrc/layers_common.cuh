@@ -212,8 +212,9 @@ __device__ __forceinline__ void act_grad_n(int kind, const F2 (&x)[kN], F2 (&g)[
     if (kind == FCAI_ACT_RELU) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
-            const float2 xx = split(x[i]);
-            g[i] = mul2(g[i], f2(xx.x > 0.f ? 1.f : 0.f, xx.y > 0.f ? 1.f : 0.f));
+            // a choice, not a product: an infinite gradient does not meet a zero, and a NaN x passes the gradient on
+            const float2 xx = split(x[i]), gg = split(g[i]);
+            g[i] = f2(xx.x <= 0.f ? 0.f : gg.x, xx.y <= 0.f ? 0.f : gg.y);
         }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll

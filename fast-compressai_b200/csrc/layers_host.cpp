@@ -41,7 +41,7 @@ const at::Tensor &tensor(PyObject *o, const char *name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
     const at::Tensor &t = THPVariable_Unpack(o);
     if (!t.is_cuda()) refuse(std::string(name) + " must be on a CUDA device");
-    if (t.layout() != at::kStrided) refuse(std::string(name) + " must be a dense tensor");
+    if (t.layout() != at::kStrided || t.is_neg() || t._is_zerotensor()) refuse(std::string(name) + " must be a dense tensor");
     return t;
 }
 void same(const at::Tensor &t, const char *name, const at::Tensor &as) {
@@ -207,9 +207,10 @@ struct Kept {
     const float *scales = nullptr;
     int keep = FCAI_KEEP_FULL;
 };
-Kept kept_of(PyObject *x, PyObject *scales, int keep, int64_t n) {
+Kept kept_of(PyObject *x, PyObject *scales, int keep, int64_t n, const at::Tensor &as) {
     Kept k;
     const at::Tensor &t = tensor(x, "what was kept");
+    if (t.device() != as.device()) refuse("what was kept is on " + t.device().str() + ", expected " + as.device().str());
     if (keep >= FCAI_KEEP_INT8) {
         const at::Tensor &s = tensor(scales, "the scales kept");
         if (t.scalar_type() != at::kByte || s.scalar_type() != at::kFloat || t.dim() != 2 || t.size(1) != n || !t.is_contiguous() ||
@@ -221,6 +222,7 @@ Kept kept_of(PyObject *x, PyObject *scales, int keep, int64_t n) {
         k.keep = keep;
     } else {
         if (t.dim() < 1 || t.size(-1) != n) refuse("what was kept does not fit the gradient");
+        same(t, "what was kept", as);
         k.m = rows_of(t, n);
     }
     return k;
@@ -234,7 +236,7 @@ PyObject *py_load8(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (codes.dim() != 2) refuse("codes are [rows, channels]");
         const int64_t c = codes.size(1);
         const c10::cuda::CUDAGuard guard(codes.device());
-        const Kept k = kept_of(a[0], a[1], keep, c);
+        const Kept k = kept_of(a[0], a[1], keep, c, codes);
         std::vector<int64_t> shape;
         if (!PyTuple_Check(a[4])) refuse("a shape is expected");
         int64_t total = 1;
@@ -291,9 +293,8 @@ PyObject *py_activation_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t c = channels(grad, "an activation");
         const c10::cuda::CUDAGuard guard(grad.device());
         const Rows g = rows_of(grad, c);
-        const Kept k = kept_of(a[1], a[2], keep, c);
+        const Kept k = kept_of(a[1], a[2], keep, c, grad);
         if (k.m.rows != g.rows) refuse("grad does not fit what was kept");
-        if (keep < FCAI_KEEP_INT8) same(grad, "grad", THPVariable_Unpack(a[1]));
         at::Tensor dx = fresh(grad.sizes(), grad);
         act_backward(grad, g, c, k, act, dx, at::Tensor(), c);
         return wrap(dx);
@@ -380,12 +381,12 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int dtype = dtype_code(grad, "linear");
         const fcai_stream_t st = stream_of(grad);
         Rows g = rows_of(grad, cout);
-        const Kept x = kept_of(a[2], a[3], keep, cin);
+        const Kept x = kept_of(a[2], a[3], keep, cin, grad);
         if (x.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
         at::Tensor dx, dw, db, dp;
         if (needs & 4) db = fresh({cout}, grad);
         if (act != FCAI_ACT_NONE) {
-            const Kept p = kept_of(a[4], a[5], keep, cout);
+            const Kept p = kept_of(a[4], a[5], keep, cout, grad);
             if (p.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
             const int64_t ld = (cout + 7) / 8 * 8;  // rows that the products read without a copy
             dp = fresh({g.rows, ld}, grad);
@@ -415,8 +416,6 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
                 status(fcai_checkpoint_load(x.codes, x.scales, v.data_ptr(), ld, x.m.rows, (int)cin, dtype, keep, st));
                 const void *p = v.data_ptr();
                 m = Rows{std::move(v), p, ld, x.m.rows};
-            } else {
-                same(m.hold, "x", grad);
             }
             const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, g.rows, (int)cin, (int)cout,
                                                         gpack | (unaligned(m.p, m.ld) ? 2 : 0) | (unaligned(dw.data_ptr(), cin) ? 4 : 0), 0);
@@ -483,11 +482,10 @@ PyObject *py_layer_norm_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         const int64_t c = channels(grad, "layer_norm");
         const c10::cuda::CUDAGuard guard(grad.device());
         const Rows g = rows_of(grad, c);
-        const Kept x = kept_of(a[1], a[2], keep, c);
+        const Kept x = kept_of(a[1], a[2], keep, c, grad);
         if (x.m.rows != g.rows || stats.scalar_type() != at::kFloat || stats.numel() != 2 * g.rows || !stats.is_contiguous() ||
             stats.device() != grad.device())
             refuse("layer_norm: grad does not fit what was kept");
-        if (keep < FCAI_KEEP_INT8) same(grad, "grad", THPVariable_Unpack(a[1]));
         const at::Tensor w = affine(a[4], "weight", grad, c);
         if (w.defined() && dtype_code(w, "layer_norm") != wdtype) refuse("layer_norm: weight has another dtype than in the forward call");
         const at::ScalarType wt = wdtype == FCAI_DTYPE_F32 ? at::kFloat : grad.scalar_type();

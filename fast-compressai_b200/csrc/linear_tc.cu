@@ -42,6 +42,10 @@
 // sums the splits in order (bitwise the same on every run) and applies the
 // epilogue.
 //
+// Every wait is bounded (1 s).  One that runs out, which no product should see,
+// makes its CTA stop, drain what it has in flight and set a word in host memory,
+// from which the next call returns FCAI_ERR_CUDA.
+//
 // Up to 32 rows the forward product is a matter of reading w once:
 // few_rows_kernel does it with warp-level MMAs, w as their 16-row operand.
 #include <cuda_runtime.h>
@@ -100,6 +104,7 @@ struct Params {
     uint8_t *codes;                      // [M][N], or NULL
     float *scales;                       // [M][nblk]
     int nblk, keep;
+    int32_t *error;                      // host memory: set if a wait ran out
 };
 
 // A tile is kPair ? 256 : 128 rows by kBN columns.  kKeep: what a backward pass
@@ -141,7 +146,7 @@ __device__ __forceinline__ void unit_coords(const Params &p, int unit, int &tm, 
     tm = m0 + rest - tn * (int)(last ? p.gm_last.d : p.gm.d);
 }
 
-// A block's scale and the codes of kR rows' 8 columns (pairs v[4 * i ...]).
+// A block's scale, and the codes of eight of its values.
 __device__ __forceinline__ float keep_scale(int keep, float amax) {
     return keep == FCAI_KEEP_E4M3 ? block_scale<true>(amax) : block_scale<false>(amax);
 }
@@ -187,12 +192,12 @@ __device__ __forceinline__ void finish1(const Params &p, int64_t row, int col, f
     static_cast<T *>(p.y)[row * p.ldy + col] = from_f32<T>(v);
 }
 template <typename T>
-__device__ __forceinline__ void add_bias8(const Params &p, int col, F2 *v, int rows) {
+__device__ __forceinline__ void add_bias8(const Params &p, int col, F2 (&v)[4]) {
     if (!p.bias) return;
     F2 b[4];
     unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.bias) + col)), b);
 #pragma unroll
-    for (int i = 0; i < rows * 4; ++i) v[i] = add2(v[i], b[i & 3]);
+    for (int i = 0; i < 4; ++i) v[i] = add2(v[i], b[i]);
 }
 
 // Shared memory by its 32-bit address: through a pointer computed from a
@@ -216,7 +221,7 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
     return v;
 }
 
-// 8 bias values of columns that every lane has alike.
+// The bias of 32 columns that every lane has alike.
 template <typename T>
 __device__ __forceinline__ void add_bias32(const Params &p, int col0, F2 (&v)[16]) {
     if (!p.bias) return;
@@ -634,6 +639,7 @@ __global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
 
     // ---------------------------------------------------------------- teardown
     __syncthreads();
+    if (*abort && threadIdx.x == 0) *static_cast<volatile int32_t *>(p.error) = 1;
     if (*abort && leader) {
         // TMEM is freed only once every MMA issued has completed
         if (warp == kEpiWarps + 1) {
@@ -704,7 +710,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
         }
         if (in) {
             if (p.vec) {
-                add_bias8<T>(p, col, v, 1);
+                add_bias8<T>(p, col, v);
             } else if (p.bias) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
@@ -984,12 +990,11 @@ __global__ void __launch_bounds__(kWarps * 32) few_rows_kernel(const FewRows f, 
     }
 }
 
-// y = act(bias) + residual, for an empty contraction (a weight gradient over no rows).
-template <typename T>
+// y = 0, a weight gradient over no rows; zero is the same bits in both types.
 __global__ void empty_product_kernel(const Params p) {
     const int64_t n = (int64_t)p.M * p.N;
     for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x)
-        static_cast<T *>(p.y)[i / p.N * p.ldy + i % p.N] = from_f32<T>(0.f);
+        static_cast<uint16_t *>(p.y)[i / p.N * p.ldy + i % p.N] = 0;
 }
 
 // ---------------------------------------------------------------------------
@@ -1007,6 +1012,31 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
             fn = reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(ptr);
     });
     return fn;
+}
+
+// One word for the process, of pinned memory that every device can write; NULL
+// without a device.  It is made outside any capture that the first call is part of.
+static volatile int32_t *error_word() {
+    static int32_t *word = nullptr;
+    static std::once_flag once;
+    std::call_once(once, [] {
+        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return;
+        void *p = nullptr;
+        if (cudaHostAlloc(&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+            word = static_cast<int32_t *>(p);
+            *word = 0;
+        }
+        cudaThreadExchangeStreamCaptureMode(&mode);
+    });
+    return word;
+}
+static int check_errors() {
+    volatile int32_t *word = error_word();
+    if (!word) return fcai::fail(FCAI_ERR_CUDA, "linear: no pinned memory for the error word");
+    if (!*word) return FCAI_OK;
+    *word = 0;
+    return fcai::fail(FCAI_ERR_CUDA, "linear: a pipeline wait of an earlier product ran out; its results are wrong");
 }
 
 constexpr int kCodeType = 100;  // a map of codes: bytes
@@ -1192,6 +1222,7 @@ static bool wide_outputs(const Params &p, int N, int dtype) {
 template <typename T, bool kTA, bool kTB>
 static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Params p, unsigned char *ws,
                cudaStream_t stream) {
+    p.error = const_cast<int32_t *>(error_word());
     p.vec = wide_outputs(p, N, dtype);
     const bool reduce = p.codes && N % 16 != 0;
     const Plan pl = make_plan(M, N, K, reduce, p.codes != nullptr);
@@ -1325,6 +1356,7 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
     }
     return n;
 }
+// The last check before a launch.
 static int check_workspace(int op, int64_t rows, int cin, int cout, const void *a, int64_t lda, const void *b, int64_t ldb,
                            const void *y, int64_t ldy, const void *residual, int64_t ldr, int dtype, int keep, const void *ws,
                            int64_t bytes) {
@@ -1333,12 +1365,14 @@ static int check_workspace(int op, int64_t rows, int cin, int cout, const void *
     const int64_t need = workspace_bytes(op, rows, cin, cout, repack, keep);
     if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
         return fcai::fail(FCAI_ERR_WORKSPACE, "linear: needs a 256-byte aligned workspace of %lld bytes", (long long)need);
-    return FCAI_OK;
+    return check_errors();
 }
 
 }  // namespace ln
 
 extern "C" {
+
+int32_t *fcai_linear_error_word(void) { return const_cast<int32_t *>(ln::error_word()); }
 
 int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack, int32_t keep) {
     return ln::workspace_bytes(op, rows, cin, cout, repack, keep);
@@ -1357,8 +1391,10 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     const bool k8 = keep >= FCAI_KEEP_INT8;
     if ((rows && k8 && (!codes || !scales)) || (keep == FCAI_KEEP_FULL && rows && !pre) || (reinterpret_cast<uintptr_t>(scales) & 3))
         return fcai::fail(FCAI_ERR_INVALID, "linear: the keep needs its output");
-    if ((residual && ldr < cout) || (keep == FCAI_KEEP_FULL && ldpre < cout))
-        return fcai::fail(FCAI_ERR_INVALID, "linear: a row stride is smaller than its row");
+    if ((residual && (ldr < cout || ldr > (1ll << 36))) || (keep == FCAI_KEEP_FULL && (ldpre < cout || ldpre > (1ll << 36))))
+        return fcai::fail(FCAI_ERR_INVALID, "linear: a row stride is smaller than its row or too large");
+    if (((reinterpret_cast<uintptr_t>(bias) | reinterpret_cast<uintptr_t>(residual) | reinterpret_cast<uintptr_t>(pre)) & 1) != 0)
+        return fcai::fail(FCAI_ERR_INVALID, "linear: misaligned pointer");
     if (rows == 0) return FCAI_OK;
     if (!x || !w || !y) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
     Params p{};
@@ -1427,8 +1463,7 @@ int fcai_linear_backward_weight(const void *dp, int64_t lddp, const void *x, int
     if (rows == 0) {
         p.M = cout;
         p.N = cin;
-        // zero is the same bits in both types
-        empty_product_kernel<__half><<<elementwise_grid((int64_t)cout * cin, 256), 256, 0, st>>>(p);
+        empty_product_kernel<<<elementwise_grid((int64_t)cout * cin, 256), 256, 0, st>>>(p);
         FCAI_CUDA_TRY(cudaGetLastError());
         return FCAI_OK;
     }

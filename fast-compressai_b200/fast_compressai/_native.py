@@ -109,6 +109,7 @@ SIGNATURES: dict[str, tuple] = {
     "fcai_layer_forward": (ctypes.c_int, [_P, _I32, _I32, _I32, _P, _P, _P, _P]),
     "fcai_nchw_f32_to_nhwc_bf16": (ctypes.c_int, [_P, _P, _I32, _I32, _I32, _I32, _P]),
     "fcai_linear_workspace": (_I64, [_I32, _I64, _I32, _I32, _I32, _I32]),
+    "fcai_linear_error_word": (ctypes.POINTER(ctypes.c_int32), []),
     "fcai_linear_forward": (
         ctypes.c_int,
         [_P, _I64, _P, _I64, _P, _P, _I64, _P, _I64, _P, _I64, _P, _P, _I64, _I32, _I32, _I32, _I32, _I32, _P, _I64, _P],

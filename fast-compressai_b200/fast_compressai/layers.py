@@ -288,7 +288,7 @@ class _Activation(torch.autograd.Function):
 
 
 def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
 
 
 def linear(x, weight, bias=None, *, activation: str = "none", residual=None, keep: str = "full") -> torch.Tensor:

@@ -43,6 +43,13 @@ def test_unknown_names_are_refused():
         layers.linear_backward(t, None, t)
 
 
+def test_other_objects_are_refused():
+    t = torch.zeros(4, 4, dtype=torch.bfloat16)
+    for call in (lambda: layers.linear([1.0], t), lambda: layers.layer_norm(None), lambda: layers.activation(2.0, "relu")):
+        with pytest.raises(ValueError, match="tensor"):
+            call()
+
+
 def _code(name, *args):
     return getattr(_native.lib(), name)(*args)
 
@@ -165,3 +172,11 @@ def test_norm_formula_against_differences():
         v = torch.randn_like(t)
         diff = (put(t + h * v) - put(t - h * v)) / (2 * h)
         assert abs(float(diff - (g * v).sum())) < 1e-7
+
+
+@pytest.mark.parametrize("bad", [
+    dict(bias=P + 1), dict(res=P + 1, ldr=32), dict(res=P, ldr=2 ** 37), dict(keep=1, pre=P + 1, ldpre=32),
+    dict(keep=1, pre=P, ldpre=2 ** 37),
+])
+def test_linear_refuses_pointers_of_its_options(bad):
+    assert _forward(**bad) == _native.FCAI_ERR_INVALID

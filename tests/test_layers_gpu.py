@@ -551,3 +551,47 @@ def test_gpu_refusals(cuda_device):
                  lambda: layers.linear_backward(y, saved, w[:20]), lambda: layers.layer_norm_backward(y, saved)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_relu_gradient_at_special_values(cuda_device):
+    inf, nan = float("inf"), float("nan")
+    x = torch.tensor([[-1.0, 0.0, -0.0, 2.0, nan, -inf, inf, 3.0]], device="cuda")
+    g = torch.tensor([[inf, -inf, nan, inf, 5.0, inf, 7.0, nan]], device="cuda")
+    want = torch.tensor([[0.0, 0.0, 0.0, inf, 5.0, 0.0, 7.0, nan]], device="cuda")
+    for dtype in (torch.float32, torch.bfloat16, torch.float16):
+        _, saved = layers.activation_forward(x.to(dtype), "relu", keep="full")
+        dx = layers.activation_backward(g.to(dtype), saved)
+        assert torch.equal(dx.float().nan_to_num(nan=99.0), want.nan_to_num(nan=99.0))
+
+
+def test_what_was_kept_must_fit(cuda_device):
+    x, w = _randn(40, 64, dtype=torch.bfloat16), _randn(40, 64, dtype=torch.bfloat16, seed=1)
+    y, saved = layers.linear_forward(x, w, activation="gelu", keep="full")
+    for part in ("kept", "pre"):
+        whole = getattr(saved, part)
+        for bad in (whole.half(), whole.cpu(), whole[:, :8], whole[:8]):
+            setattr(saved, part, bad)
+            with pytest.raises(ValueError):
+                layers.linear_backward(y, saved, w, (True, False, False))
+        setattr(saved, part, whole)
+    layers.linear_backward(y, saved, w)
+    with pytest.raises(ValueError, match="dense"):
+        layers.linear_forward(torch._neg_view(x), w)
+
+
+def test_a_wait_that_ran_out_is_reported_by_the_next_call(cuda_device):
+    from fast_compressai import _native
+
+    word = _native.lib().fcai_linear_error_word()
+    assert word and word[0] == 0  # no product so far ran into it
+    for rows in (1, 300):
+        x, w = _randn(rows, 64, dtype=torch.bfloat16), _randn(40, 64, dtype=torch.bfloat16, seed=1)
+        want, saved = layers.linear_forward(x, w, keep="full")
+        word[0] = 1
+        with pytest.raises(_native.NativeCallError, match="ran out"):
+            layers.linear_forward(x, w)
+        assert word[0] == 0 and torch.equal(layers.linear_forward(x, w), want)
+        word[0] = 1
+        with pytest.raises(_native.NativeCallError, match="ran out"):
+            layers.linear_backward(want, saved, w)
+        assert word[0] == 0
