@@ -355,7 +355,7 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
             }
         }
         const int repack = (unaligned(m.p, m.ld) ? 1 : 0) | (unaligned(wm.p, wm.ld) ? 2 : 0) | (unaligned(y.data_ptr(), cout) ? 4 : 0) |
-                           (r.p && unaligned(r.p, r.ld) ? 8 : 0);
+                           (r.p && unaligned(r.p, r.ld) ? 8 : 0) | (bias.defined() && unaligned(bias.data_ptr(), cout) ? 16 : 0);
         const int64_t bytes = fcai_linear_workspace(FCAI_LINEAR_FORWARD, m.rows, (int)cin, (int)cout, repack, kp);
         const Scratch ws = scratch(bytes);
         status(fcai_linear_forward(m.p, m.ld, wm.p, wm.ld, ptr(bias), r.p, r.ld, y.data_ptr(), cout, ptr(pre), ldpre, ptr(k.codes),

@@ -95,7 +95,7 @@ struct Params {
     int ldp;                             // partial tiles: row stride (N rounded up to 8)
     int coop;                            // all epilogue warps on each tile
     int vec;                             // N % 8 == 0, and y, residual, pre, bias and codes take wide accesses
-    int tma, bias_vec;                   // y, residual, pre and codes are tiles of tensor maps; bias takes wide accesses
+    int tma;                             // y, residual, pre and codes are tiles of tensor maps; bias takes wide accesses, to a multiple of 8
     int act;
     const void *bias, *residual;
     void *y, *pre;
@@ -221,22 +221,17 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
     return v;
 }
 
-// The bias of 32 columns that every lane has alike.
+// The bias of 32 columns that every lane has alike, 8 at a time (a ragged or
+// unaligned bias was copied: narrow loads here, even where no call takes them,
+// cost every product registers; 36864 x 192 -> 768 took 34.3 us instead of 32.1).
 template <typename T>
 __device__ __forceinline__ void add_bias32(const Params &p, int col0, F2 (&v)[16]) {
     if (!p.bias) return;
-    const T *bias = static_cast<const T *>(p.bias) + col0;
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
         if (col0 + 8 * g >= p.N) break;
         F2 b[4];
-        if (p.bias_vec && col0 + 8 * g + 8 <= p.N) {
-            unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(bias + 8 * g)), b);
-        } else {
-            auto at = [&](int c) { return col0 + c < p.N ? to_f32(bias[c]) : 0.f; };
-#pragma unroll
-            for (int e = 0; e < 4; ++e) b[e] = f2(at(8 * g + 2 * e), at(8 * g + 2 * e + 1));
-        }
+        unpack8<T>(__ldg(reinterpret_cast<const uint4 *>(static_cast<const T *>(p.bias) + col0 + 8 * g)), b);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[4 * g + e] = add2(v[4 * g + e], b[e]);
     }
@@ -639,10 +634,10 @@ __global__ void __launch_bounds__(Layout<kBN, kPair, kKeep>::kThreads, 1)
 
     // ---------------------------------------------------------------- teardown
     __syncthreads();
-    if (*abort && threadIdx.x == 0) *static_cast<volatile int32_t *>(p.error) = 1;
-    if (*abort && leader) {
+    if (*abort) {
+        if (threadIdx.x == 0) *static_cast<volatile int32_t *>(p.error) = 1;
         // TMEM is freed only once every MMA issued has completed
-        if (warp == kEpiWarps + 1) {
+        if (leader && warp == kEpiWarps + 1) {
             if (lane == 0) {
                 if (kPair) mma_commit_pair(dbar);
                 else mma_commit(dbar);
@@ -793,7 +788,7 @@ __global__ void __launch_bounds__(256) reduce_kernel(const Params p) {
     }
 }
 
-// Up to three matrices that TMA cannot read, [rows][cols] with row stride ld,
+// Up to four matrices that TMA cannot read, [rows][cols] with row stride ld,
 // into dst[rows][ldd], 16 bytes a thread and step.  Rows start at any element,
 // so a thread's eight come as 4-byte words: four of them, or, from an odd
 // element on, three between two single elements, shifted together; nothing
@@ -807,7 +802,7 @@ struct Repack {
     int step;        // rows of a CTA and step: about 2048 chunks
 };
 struct Repacks {
-    Repack r[3];
+    Repack r[4];
 };
 __global__ void __launch_bounds__(256) repack_kernel(const Repacks all) {
     const Repack &o = all.r[blockIdx.y];
@@ -1249,14 +1244,14 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     const bool y_aligned = aligned16(p.y, p.ldy, dtype), r_aligned = !p.residual || aligned16(p.residual, p.ldr, dtype);
     const bool pad = !p.partial && M * N >= kPadFrom && (!y_aligned || !r_aligned);
     p.tma = !p.partial && (pad || (y_aligned && r_aligned)) && (!p.pre || aligned16(p.pre, p.ldpre, dtype));
-    p.bias_vec = !p.bias || aligned16(p.bias, 0, dtype);
-    Operand R{p.tma ? p.residual : nullptr, p.ldr, M, N};
+    Operand R{p.tma ? p.residual : nullptr, p.ldr, M, N}, bias{p.tma ? p.bias : nullptr, N, 1, N};
     int rc;
-    if ((rc = prepare_operands({&A, &B, &R}, dtype, ws, stream))) return rc;
+    if ((rc = prepare_operands({&A, &B, &R, &bias}, dtype, ws, stream))) return rc;
     Unpad back{};
     if (p.tma) {
         p.residual = R.ptr;
         p.ldr = R.ld;
+        p.bias = bias.ptr;
         if (!y_aligned) {
             const int chunks = (N + 7) / 8 + 1;
             back = {reinterpret_cast<const uint16_t *>(ws), static_cast<uint16_t *>(p.y), round8(N), p.ldy, M, N, fast_div(chunks),
@@ -1350,6 +1345,7 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
     int64_t n = partial;
     if (repack & 1) n += repack_bytes(a_rows, a_cols);
     if (repack & 2) n += repack_bytes(b_rows, b_cols);
+    if (!partial && (repack & 16)) n += repack_bytes(1, N);
     if (!partial && M * N >= kPadFrom) {
         if (repack & 4) n += repack_bytes(M, N);
         if (repack & 8) n += repack_bytes(M, N);
@@ -1358,10 +1354,10 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
 }
 // The last check before a launch.
 static int check_workspace(int op, int64_t rows, int cin, int cout, const void *a, int64_t lda, const void *b, int64_t ldb,
-                           const void *y, int64_t ldy, const void *residual, int64_t ldr, int dtype, int keep, const void *ws,
-                           int64_t bytes) {
+                           const void *y, int64_t ldy, const void *residual, int64_t ldr, const void *bias, int dtype, int keep,
+                           const void *ws, int64_t bytes) {
     const int repack = (aligned16(a, lda, dtype) ? 0 : 1) | (aligned16(b, ldb, dtype) ? 0 : 2) | (aligned16(y, ldy, dtype) ? 0 : 4) |
-                       (!residual || aligned16(residual, ldr, dtype) ? 0 : 8);
+                       (!residual || aligned16(residual, ldr, dtype) ? 0 : 8) | (!bias || aligned16(bias, cout, dtype) ? 0 : 16);
     const int64_t need = workspace_bytes(op, rows, cin, cout, repack, keep);
     if (need > 0 && (!ws || bytes < need || (reinterpret_cast<uintptr_t>(ws) & 255)))
         return fcai::fail(FCAI_ERR_WORKSPACE, "linear: needs a 256-byte aligned workspace of %lld bytes", (long long)need);
@@ -1411,8 +1407,8 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
     p.keep = keep;
     if (k8 && rows > kFewRows && cout % 8 == 0 && !wide_outputs(p, cout, dtype))
         return fcai::fail(FCAI_ERR_INVALID, "linear: codes need 16-byte aligned y, bias and residual rows, and 16-byte aligned codes");
-    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, y, ldy, residual, ldr, dtype, keep, workspace,
-                              workspace_bytes)))
+    if ((rc = check_workspace(FCAI_LINEAR_FORWARD, rows, cin, cout, x, ldx, w, ldw, y, ldy, residual, ldr, bias, dtype, keep,
+                              workspace, workspace_bytes)))
         return rc;
     const Operand A{x, ldx, rows, cin}, B{w, ldw, cout, cin};
     auto *ws = static_cast<unsigned char *>(workspace);
@@ -1435,8 +1431,8 @@ int fcai_linear_backward_input(const void *dp, int64_t lddp, const void *w, int6
     if (rc) return rc;
     if (rows == 0) return FCAI_OK;
     if (!dp || !w || !dx) return fcai::fail(FCAI_ERR_INVALID, "linear: null pointer");
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dx, lddx, nullptr, 0, dtype, 0, workspace,
-                              workspace_bytes)))
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_INPUT, rows, cin, cout, dp, lddp, w, ldw, dx, lddx, nullptr, 0, nullptr, dtype, 0,
+                              workspace, workspace_bytes)))
         return rc;
     Params p{};
     p.y = dx;
@@ -1467,8 +1463,8 @@ int fcai_linear_backward_weight(const void *dp, int64_t lddp, const void *x, int
         FCAI_CUDA_TRY(cudaGetLastError());
         return FCAI_OK;
     }
-    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dw, lddw, nullptr, 0, dtype, 0, workspace,
-                              workspace_bytes)))
+    if ((rc = check_workspace(FCAI_LINEAR_BACKWARD_WEIGHT, rows, cin, cout, dp, lddp, x, ldx, dw, lddw, nullptr, 0, nullptr, dtype, 0,
+                              workspace, workspace_bytes)))
         return rc;
     const Operand A{dp, lddp, rows, cout}, B{x, ldx, rows, cin};
     auto *ws = static_cast<unsigned char *>(workspace);

@@ -61,8 +61,9 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
 /* `repack`: bits set for matrices of the call that are not 16-byte aligned in
  * address and row stride: 1 the first operand (x; dp; dp), 2 the second (w; w;
- * x), 4 the output (y; dx; dw), 8 the residual.  `keep`: the forward call's (0
- * for the others). */
+ * x), 4 the output (y; dx; dw), 8 the residual, and 16 for a bias whose address
+ * is not, or whose length is no multiple of 8.  `keep`: the forward call's (0 for
+ * the others). */
 int64_t fcai_linear_workspace(int32_t op, int64_t rows, int32_t cin, int32_t cout, int32_t repack, int32_t keep);
 int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, const void *bias,
                         const void *residual, int64_t ldr, void *y, int64_t ldy, void *pre, int64_t ldpre,
