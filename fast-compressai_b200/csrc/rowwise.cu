@@ -9,12 +9,14 @@
 //     CTA, which colsum_kernel adds in a fixed order (the same bits every run);
 //   * rows: a CTA takes whole rows, for sums over channels.
 //
-// Both read through a ring of shared memory that cp.async fills, every thread
+// The strips read through a ring of shared memory that cp.async fills, every thread
 // its own 16 bytes a row, several rows ahead of the one it works on: what is in
 // flight costs no registers, needs no barrier, and never drains while a row is
 // worked on (with the next rows in registers instead, too few bytes were in
-// flight: 3.3 to 4.7 TB/s).  Rows that do not take 16-byte accesses keep the
-// next row in registers.
+// flight: 3.3 to 4.7 TB/s).  Rows that do not take 16-byte accesses go by single
+// elements, with the next row in registers or with more warps.  The layer norm
+// keeps its next rows in registers (a ring for it was slower, 89 us against 62 at
+// 16384 x 4096).
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -77,7 +79,7 @@ __device__ __forceinline__ uint2 load_codes(const uint8_t *row, const Cols<kV> &
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (in && c[i] < n) (i < 4 ? q.x : q.y) |= (uint32_t)row[c[i]] << (8 * (i & 3));
+            if (in && c[i] < n) (i < 4 ? q.x : q.y) |= (uint32_t)__ldg(row + c[i]) << (8 * (i & 3));
     }
     return q;
 }
@@ -331,10 +333,12 @@ __global__ void __launch_bounds__(kThreads, kV ? 5 : 4)
     cp_wait<0>();
 }
 
-constexpr int kLoadRows = 2;  // rows a thread has in flight: 8 + 4 bytes a row are too little for the ring to pay
+// Rows a thread has in flight: 8 + 4 bytes a row are too little for the ring to
+// pay.  By single elements one row and more warps (31 us -> 27 at 30000 x 1021).
 template <typename T, bool kV, int kLanes>
-__global__ void __launch_bounds__(kThreads, kV ? 6 : 4)
+__global__ void __launch_bounds__(kThreads, 6)
     checkpoint_load_kernel(Kept k, T *__restrict__ out, int64_t ldo, int64_t rows, int n, int nblk) {
+    constexpr int kLoadRows = kV ? 2 : 1;
     const Cols<kV> c(blockIdx.x * kBlock, threadIdx.x % kLanes, kLanes);
     const int64_t step = (int64_t)gridDim.y * (kThreads / kLanes);
     for (int64_t r0 = (int64_t)blockIdx.y * (kThreads / kLanes) + threadIdx.x / kLanes; r0 < rows; r0 += step * kLoadRows) {
@@ -371,9 +375,17 @@ __device__ __forceinline__ void group_sums(const V8 &sums, float *partial_row, i
     }
 }
 
+// Rows that take single elements only: with the next row in registers, packing it
+// waits for its loads in the middle of this one's work, and 24 warps an SM do not
+// hide that (30000 x 1021 bf16 from int8: 127 us); 48 warps without a row ahead do
+// (59).  f32 from f32, with nothing to pack, stays ahead (64 us, 77 without).
+template <typename T, bool k8>
+constexpr bool act_ahead() {
+    return sizeof(T) == 4 && !k8;
+}
 // dx = dy act'(x) and partial sums of it over the CTA's rows; kAct: x is read
 template <typename T, bool kV, bool k8, bool kAct, int kLanes>
-__global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
+__global__ void __launch_bounds__(kThreads, !kV ? (act_ahead<T, k8>() ? 3 : 6) : sizeof(T) == 4 ? 3 : 4)
     act_backward_kernel(const T *__restrict__ dy, int64_t lddy, Kept k, T *__restrict__ dx, int64_t lddx,
                         float *__restrict__ partial, int64_t rows, int n, int nblk, int act) {
     using FeedG = RowFeed<T, kV, kV, kThreads, 1>;
@@ -395,19 +407,36 @@ __global__ void __launch_bounds__(kThreads, sizeof(T) == 4 || !kV ? 3 : 4)
         if (kAct) feed_x.issue(base + slot * kStep + FeedG::kStep, 0, k, r, c, n, nblk, r < rows);
         cp_commit();
     };
-#pragma unroll
-    for (int d = 0; d < kD; ++d) issue(d, row + d * step);
-    for (int slot = 0; row < rows; row += step, slot = slot + 1 == kD ? 0 : slot + 1) {
-        cp_wait<kD - 1>();
-        V8 g = feed_g.get(base + slot * kStep, 0).get(), x;
-        if (kAct) x = feed_x.get(base + slot * kStep + FeedG::kStep, 0).get(k);
-        issue(slot, row + kD * step);
+    auto finish = [&](V8 g, V8 x) {
         if (kAct) act_grad_n(act, x.p, g.p);
         if (dx) store8(dx + row * lddx, c, n, true, g);
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc.p[i] = add2(acc.p[i], g.p[i]);
+    };
+    if constexpr (kV || act_ahead<T, k8>()) {
+#pragma unroll
+        for (int d = 0; d < kD; ++d) issue(d, row + d * step);
+        for (int slot = 0; row < rows; row += step, slot = slot + 1 == kD ? 0 : slot + 1) {
+            cp_wait<kD - 1>();
+            V8 g = feed_g.get(base + slot * kStep, 0).get(), x;
+            if (kAct) x = feed_x.get(base + slot * kStep + FeedG::kStep, 0).get(k);
+            issue(slot, row + kD * step);
+            finish(g, x);
+        }
+        cp_wait<0>();
+    } else {
+        for (; row < rows; row += step) {
+            Raw8<T, kV> raw_g;
+            KeptRaw<T, kV, k8> raw_x;
+            raw_g.load(dy + row * lddy, c, n, true);
+            V8 x;
+            if (kAct) {
+                raw_x.load(k, row, c, n, nblk, true);
+                x = raw_x.get(k);
+            }
+            finish(raw_g.get(), x);
+        }
     }
-    cp_wait<0>();
     if (partial) {
         group_sums<kLanes, kThreads, kV>(acc, partial + (int64_t)blockIdx.y * n, blockIdx.x * kBlock, n, reinterpret_cast<float *>(ring));
     }
@@ -941,11 +970,15 @@ template <typename T>
 static int act_forward(const void *x, int64_t ldx, void *y, int64_t ldy, void *codes, float *scales, int64_t rows, int n,
                        int dtype, int act, int keep, cudaStream_t st) {
     const bool q = keep == FCAI_KEEP_INT8 || keep == FCAI_KEEP_E4M3;
-    const bool vec = n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
+    // f32 goes by single elements: a lane's 32 bytes as two 16-byte accesses leave
+    // every store half a sector (30000 x 1024: 60 us, 65 with codes, against 44 and 55;
+    // only 64 channels with codes lose by it, 200000 x 64: 32 against 39)
+    constexpr bool kWide = sizeof(T) == 2;
+    const bool vec = kWide && n % 8 == 0 && aligned16(x, ldx, dtype) && (!y || aligned16(y, ldy, dtype)) && (!q || codes_vec(codes, n));
     const int strips = blocks_of(n);
     const dim3 grid(strips, row_shares(rows, strips, strip_lanes(n)));
-    auto kernel = strip_lanes(n) == 4 ? (vec ? act_forward_kernel<T, true, 4> : act_forward_kernel<T, false, 4>)
-                                      : (vec ? act_forward_kernel<T, true, 16> : act_forward_kernel<T, false, 16>);
+    auto kernel = strip_lanes(n) == 4 ? (vec ? act_forward_kernel<T, kWide, 4> : act_forward_kernel<T, false, 4>)
+                                      : (vec ? act_forward_kernel<T, kWide, 16> : act_forward_kernel<T, false, 16>);
     kernel<<<grid, kThreads, 0, st>>>(static_cast<const T *>(x), ldx, static_cast<T *>(y), ldy, static_cast<uint8_t *>(codes), scales,
                                       rows, n, strips, act, q ? keep : FCAI_KEEP_NONE);
     FCAI_CUDA_TRY(cudaGetLastError());
