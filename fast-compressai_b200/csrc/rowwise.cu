@@ -910,11 +910,18 @@ static Held held(int n) {
 }
 // Rows a group has in flight in the backward kernel.
 constexpr int backward_rows(int lanes, int chunks) { return lanes <= 32 ? 2 / chunks : 1; }
+// CTAs of the backward kernel: each leaves a partial row of 2 n sums, so it is to
+// have 6 steps of rows, once there are two CTAs an SM; rows by single elements 3,
+// whose loads more warps hide (fp16 from int8, inputs in memory: 1000 x 1024 10.8 us,
+// with as many CTAs as fit 17.3; 5003 x 1024 20.5 and 23.0; 20000 x 200 12.0 and 14.2;
+// 2000 x 1021 13.7 with 3 steps, 16.1 with 6).
 static int norm_backward_grid(int64_t rows, int n) {
     const Held h = held(n);
     const int groups = (h.lanes <= 32 ? kThreads / h.lanes : 1) * backward_rows(h.lanes, h.chunks);
     const int per_sm = h.lanes <= 32 ? 3 : norm_ctas(h.lanes, h.chunks, false, 0);
-    return (int)std::max<int64_t>(1, std::min<int64_t>((rows + groups - 1) / groups, (int64_t)fcai::sm_count() * per_sm));
+    const int64_t sms = fcai::sm_count(), steps = (rows + groups - 1) / groups;
+    const int64_t want = std::max<int64_t>(std::min<int64_t>(steps, sms * 2), steps / (n % 8 ? 3 : 6));
+    return (int)std::max<int64_t>(1, std::min<int64_t>(want, sms * per_sm));
 }
 static int64_t act_workspace(int64_t rows, int n) {
     return rows ? round256((int64_t)row_shares(rows, blocks_of(n), strip_lanes(n)) * n * 4) : 0;
