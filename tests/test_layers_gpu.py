@@ -595,3 +595,82 @@ def test_a_wait_that_ran_out_is_reported_by_the_next_call(cuda_device):
         with pytest.raises(_native.NativeCallError, match="ran out"):
             layers.linear_backward(want, saved, w)
         assert word[0] == 0
+
+
+@pytest.mark.parametrize("rows,cout", [(50003, 136), (20001, 333), (40, 136), (8, 40), (300, 65)])
+def test_linear_unaligned_residual_of_any_size(cuda_device, rows, cout):
+    dtype = torch.float16
+    x, w = _randn(rows, 24, dtype=dtype), _randn(cout, 24, dtype=dtype, seed=1, scale=0.2)
+    b, r = _randn(cout + 1, dtype=dtype, seed=2)[1:], _randn(rows, cout, dtype=dtype, seed=3)
+    want, bound = R.linear_bound(x, w, b, r, "silu", dtype)
+    for keep in (None, "full", "int8"):
+        out = layers.linear_forward(x, w, b, activation="silu", residual=_sliced(r), keep=keep)
+        R.check(out if keep is None else out[0], want, bound, f"{keep}")
+
+
+@pytest.mark.parametrize("rows,cin,cout", [(50003, 24, 136), (20001, 24, 333), (300, 72, 65), (20, 64, 40), (3, 33, 17)])
+@pytest.mark.parametrize("ld_more,offset", [(0, 0), (8, 0), (8, 8), (5, 0), (7, 3)])
+def test_outputs_inside_wider_matrices(cuda_device, rows, cin, cout, ld_more, offset):
+    # the C entry writes y's columns and nothing beside them
+    from fast_compressai import _native
+
+    lib, dtype = _native.lib(), torch.bfloat16
+    x, w = _randn(rows, cin, dtype=dtype), _randn(cout, cin, dtype=dtype, seed=1, scale=cin ** -0.5)
+    b = _randn(cout, dtype=dtype, seed=2)
+    ld = cout + ld_more + offset
+    big = torch.full((rows + 2, ld), 7.0, dtype=dtype, device="cuda")
+    y = big[1:-1, offset:offset + cout]
+
+    def bits(p, stride, bit):
+        return 0 if p % 16 == 0 and stride % 8 == 0 else bit
+
+    repack = (bits(x.data_ptr(), cin, 1) | bits(w.data_ptr(), cin, 2) | bits(y.data_ptr(), ld, 4) | bits(b.data_ptr(), cout, 16))
+    n = lib.fcai_linear_workspace(0, rows, cin, cout, repack, 0)
+    ws = torch.empty(max(n, 1), dtype=torch.uint8, device="cuda")
+    code = lib.fcai_linear_forward(x.data_ptr(), cin, w.data_ptr(), cin, b.data_ptr(), None, 0, y.data_ptr(), ld, None, 0, None,
+                                   None, rows, cin, cout, 0, 2, 0, ws.data_ptr(), n, torch.cuda.current_stream().cuda_stream)
+    assert code == 0, lib.fcai_last_error()
+    want, bound = R.linear_bound(x, w, b, None, "gelu", dtype)
+    R.check(y, want, bound, "y")
+    assert (big[0] == 7).all() and (big[-1] == 7).all()
+    assert (big[:, :offset] == 7).all() and (big[:, offset + cout:] == 7).all()
+
+
+@pytest.mark.parametrize("rows,n", [(33, 40), (5, 1021), (70, 24), (9, 9000), (300, 200)])
+@pytest.mark.parametrize("ld_more,offset", [(8, 0), (8, 8), (5, 3)])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_rowwise_outputs_inside_wider_matrices(cuda_device, rows, n, ld_more, offset, dtype):
+    # the same numbers as the calls that allocate, and nothing written beside them
+    from fast_compressai import _native
+
+    lib, code = _native.lib(), {torch.bfloat16: 0, torch.float32: 2}[dtype]
+    x, dy = _randn(rows, n, dtype=dtype), _randn(rows, n, dtype=dtype, seed=1)
+    ld = n + ld_more + offset
+    stream = torch.cuda.current_stream().cuda_stream
+
+    def inside(call, want, exact=True):
+        big = torch.full((rows + 2, ld), 7.0, dtype=dtype, device="cuda")
+        y = big[1:-1, offset:offset + n]
+        assert call(y.data_ptr()) == 0, lib.fcai_last_error()
+        # another alignment sums a row's channels in another order: fp32 results some 2^-20 apart (values of order 1, hence
+        # 1e-5), whose roundings are at most one step, eps of the value, apart
+        assert torch.equal(y, want) if exact else torch.allclose(y.float(), want.float(), rtol=2 * torch.finfo(dtype).eps, atol=1e-5)
+        assert (big[0] == 7).all() and (big[-1] == 7).all()
+        assert (big[:, :offset] == 7).all() and (big[:, offset + n:] == 7).all()
+
+    inside(lambda p: lib.fcai_activation_forward(x.data_ptr(), n, p, ld, None, None, rows, n, code, 3, 0, stream),
+           layers.activation_forward(x, "silu"))
+    _, saved = layers.activation_forward(x, "silu", keep="int8")
+    c, s = saved.kept.codes.data_ptr(), saved.kept.scales.data_ptr()
+    inside(lambda p: lib.fcai_activation_backward(dy.data_ptr(), n, None, 0, c, s, p, ld, None, rows, n, code, 3, 2, None, 0,
+                                                  stream), layers.activation_backward(dy, saved))
+    inside(lambda p: lib.fcai_checkpoint_load(c, s, p, ld, rows, n, code, 2, stream), saved.kept.load())
+    y, saved = layers.layer_norm_forward(x, keep="full")
+    mean, rstd = saved.stats[0].data_ptr(), saved.stats[1].data_ptr()
+    inside(lambda p: lib.fcai_layer_norm_forward(x.data_ptr(), n, None, None, code, p, ld, None, None, None, None, rows, n, 1e-5,
+                                                 code, 0, stream), y, exact=False)
+    need = lib.fcai_layer_norm_workspace(rows, n)
+    ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+    inside(lambda p: lib.fcai_layer_norm_backward(dy.data_ptr(), n, x.data_ptr(), n, None, None, mean, rstd, None, code, p, ld,
+                                                  None, None, rows, n, code, 1, ws.data_ptr(), need, stream),
+           layers.layer_norm_backward(dy, saved, needs=(True, False, False))[0], exact=False)
