@@ -167,6 +167,11 @@ __device__ __forceinline__ float clamp_nan(float x) {  // to +-30; a NaN stays
     asm("{\n\t.reg .f32 t;\n\tmin.NaN.f32 t, %1, %2;\n\tmax.NaN.f32 %0, t, %3;\n\t}" : "=f"(y) : "f"(x), "f"(30.f), "f"(-30.f));
     return y;
 }
+__device__ __forceinline__ float finite(float x) {  // to +-FLT_MAX: the smaller magnitude, with x's sign
+    float y;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(y) : "f"(x), "f"(FLT_MAX));
+    return y;
+}
 // x Phi(x) = max(x, 0) - |x| Q(|x|)
 __device__ __forceinline__ F2 gelu2(F2 v) {
     const float2 x = split(v);
@@ -183,6 +188,8 @@ __device__ __forceinline__ F2 gelu_grad2(F2 v) {
     const F2 cdf = f2(x.x < 0.f ? lo.x : hi.x, x.y < 0.f ? lo.y : hi.y);
     return fma2(mul2(f2(clamp_nan(x.x), clamp_nan(x.y)), e), f2(0.398942280f), cdf);
 }
+// Exponential and reciprocal flush to zero: SiLU and its derivative are 0 below
+// x = -87.3, where they are less than 1.2e-36, for one special function each.
 __device__ __forceinline__ F2 sigmoid2(F2 x) {
     const float2 a = split(mul2(x, f2(-1.44269504f)));
     const float2 d = split(add2(f2(ex2_approx(a.x), ex2_approx(a.y)), f2(1.f)));
@@ -223,7 +230,11 @@ __device__ __forceinline__ void act_grad_n(int kind, const F2 (&x)[kN], F2 (&g)[
 #pragma unroll
         for (int i = 0; i < kN; ++i) {
             const F2 s = sigmoid2(x[i]);
-            g[i] = mul2(g[i], mul2(s, fma2(x[i], fma2(s, f2(-1.f), f2(1.f)), f2(1.f))));
+            // x as a finite number: where it is infinite, s or 1 - s is zero and the limit is wanted, not a NaN.
+            // A NaN comes through s.  16-bit types reach infinities from values of 65520 on.
+            const float2 xx = split(x[i]);
+            const F2 xf = f2(finite(xx.x), finite(xx.y));
+            g[i] = mul2(g[i], mul2(s, fma2(xf, fma2(s, f2(-1.f), f2(1.f)), f2(1.f))));
         }
     }
 }
