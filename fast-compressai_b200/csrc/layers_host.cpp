@@ -8,8 +8,11 @@
 // Plain CPython functions over torch's C++ tensors; every C++ exception ends in
 // a Python one.
 #include <ATen/ATen.h>
+#include <ATen/TracerMode.h>
 #include <ATen/cuda/EmptyTensor.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/GradMode.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDACachingAllocator.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -37,9 +40,21 @@ std::string sizes_text(at::IntArrayRef s) {
     return t + (s.size() == 1 ? ",)" : ")");
 }
 
+// The calls write their outputs past torch's dispatcher, where nothing follows what
+// they do: a trace would hold their results as constants, and a forward-mode tangent
+// would be lost.  Both are refused instead.  (Inside an autograd function, whose
+// forward runs with forward mode off, torch looks after tangents itself.)
+void check_not_traced() {
+    using Modes = c10::impl::TorchDispatchModeTLS;
+    if (at::tracer::impl::is_dispatch_enabled() ||
+        (Modes::any_modes_set() && Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY)))
+        refuse("this call cannot be traced (torch.jit.trace takes layers.linear, layers.layer_norm and layers.activation)");
+}
 const at::Tensor &tensor(PyObject *o, const char *name) {
     if (!THPVariable_Check(o)) refuse(std::string(name) + " must be a tensor");
     const at::Tensor &t = THPVariable_Unpack(o);
+    if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t._fw_grad(0).defined())
+        refuse(std::string(name) + " has a forward-mode tangent, which these calls do not carry on");
     if (!t.is_cuda()) refuse(std::string(name) + " must be on a CUDA device");
     if (t.layout() != at::kStrided || t.is_neg() || t._is_zerotensor()) refuse(std::string(name) + " must be a dense tensor");
     return t;
@@ -155,6 +170,7 @@ PyObject *guarded(Py_ssize_t n, Py_ssize_t want, F &&f) {
         return nullptr;
     }
     try {
+        check_not_traced();
         const c10::AutoGradMode no_graph(false);  // a copy made here is no operation of the caller's
         return f();
     } catch (const Refused &r) {

@@ -25,6 +25,11 @@ the explicit calls, or release eager autograd graphs of the same parameters
 first (torch's own gradient accumulation ties them to the stream they were
 first used on).
 
+The results of the explicit calls carry no gradient.  Under ``torch.jit.trace``
+the differentiable calls are recorded as nodes that run them again; the explicit
+calls refuse it, and all refuse ``make_fx`` and tensors with a forward-mode
+tangent, since nothing would follow what they do.
+
 Arguments that do not fit raise ``ValueError`` before anything is launched.
 There is no fallback: the tensors are on a CUDA device and the native library
 is built.
@@ -244,10 +249,28 @@ def _unpack(ctx) -> tuple[Saved, torch.Tensor | None]:
     return Saved(op, kept, shape, dtype, pre=pre, stats=stats, activation=kind, bias=bias), weight
 
 
+class _Paused:
+    """torch.jit's tracing, off for as long as an autograd function runs, which
+    the trace holds as one node."""
+
+    def __enter__(self):
+        self.state = torch._C._get_tracing_state()
+        torch._C._set_tracing_state(None)
+
+    def __exit__(self, *exc):
+        torch._C._set_tracing_state(self.state)
+        return False
+
+
+def _traced() -> bool:
+    return torch._C._get_tracing_state() is not None
+
+
 class _Linear(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, residual, activation, keep):
-        y, saved = linear_forward(x, weight, bias, activation=activation, residual=residual, keep=keep)
+        with _Paused() if _traced() else _native._NOTHING:
+            y, saved = linear_forward(x, weight, bias, activation=activation, residual=residual, keep=keep)
         _pack(ctx, saved, weight)
         return y
 
@@ -263,7 +286,8 @@ class _Linear(torch.autograd.Function):
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, keep):
-        y, saved = layer_norm_forward(x, weight, bias, eps=eps, keep=keep)
+        with _Paused() if _traced() else _native._NOTHING:
+            y, saved = layer_norm_forward(x, weight, bias, eps=eps, keep=keep)
         _pack(ctx, saved, weight)
         return y
 
@@ -277,7 +301,8 @@ class _LayerNorm(torch.autograd.Function):
 class _Activation(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, kind, keep):
-        y, saved = activation_forward(x, kind, keep=keep)
+        with _Paused() if _traced() else _native._NOTHING:
+            y, saved = activation_forward(x, kind, keep=keep)
         _pack(ctx, saved, None)
         return y
 
@@ -287,8 +312,11 @@ class _Activation(torch.autograd.Function):
         return activation_backward(grad, _unpack(ctx)[0]), None, None
 
 
-def _needs_grad(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors)
+def _recorded(*tensors) -> bool:
+    """Whether a call goes through its autograd function: for a gradient, or for a trace."""
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        return True
+    return _traced()
 
 
 def linear(x, weight, bias=None, *, activation: str = "none", residual=None, keep: str = "full") -> torch.Tensor:
@@ -296,7 +324,7 @@ def linear(x, weight, bias=None, *, activation: str = "none", residual=None, kee
     activation's input wait for the backward pass."""
     if keep is None:
         raise ValueError("keep must say how tensors wait for the backward pass (one of 'full', 'int8', 'e4m3')")
-    if not _needs_grad(x, weight, bias, residual):
+    if not _recorded(x, weight, bias, residual):
         return linear_forward(x, weight, bias, activation=activation, residual=residual)
     return _Linear.apply(x, weight, bias, residual, activation, keep)
 
@@ -305,7 +333,7 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, keep: str = "ful
     """Differentiable ``layer_norm_forward``."""
     if keep is None:
         raise ValueError("keep must say how tensors wait for the backward pass (one of 'full', 'int8', 'e4m3')")
-    if not _needs_grad(x, weight, bias):
+    if not _recorded(x, weight, bias):
         return layer_norm_forward(x, weight, bias, eps=eps)
     return _LayerNorm.apply(x, weight, bias, eps, keep)
 
@@ -314,6 +342,6 @@ def activation(x, kind: str, *, keep: str = "int8") -> torch.Tensor:
     """Differentiable ``activation_forward``; keeps x in 8 bits unless asked otherwise."""
     if keep is None:
         raise ValueError("keep must say how tensors wait for the backward pass (one of 'full', 'int8', 'e4m3')")
-    if not _needs_grad(x):
+    if not _recorded(x):
         return activation_forward(x, kind)
     return _Activation.apply(x, kind, keep)

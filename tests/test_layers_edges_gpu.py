@@ -43,3 +43,58 @@ def test_linear_gradients_where_the_activation_input_leaves_fp16(cuda_device, ki
     for name, got, (g, e) in zip(("dx", "dw"), layers.linear_backward(dy, saved, w),
                                  R.linear_grads(dy, x, w, p64, kind, torch.float16)):
         R.check(got, g, e, name)
+
+
+# ------------------------------------------------- transforms of torch around the calls
+
+def _three_calls():
+    w = _randn(64, 64, dtype=torch.bfloat16, seed=1, scale=0.1)
+    return {"linear": lambda q: layers.linear(q, w, activation="gelu"),
+            "linear trained": lambda q: layers.linear(q, w.clone().requires_grad_()),
+            "layer_norm": lambda q: layers.layer_norm(q),
+            "activation": lambda q: layers.activation(q, "silu")}
+
+
+@pytest.mark.parametrize("name", ["linear", "layer_norm", "activation"])
+def test_a_trace_runs_the_kernels_again(cuda_device, name):
+    call = _three_calls()[name]
+    x = _randn(40, 64, dtype=torch.bfloat16)
+    traced = torch.jit.trace(lambda q: call(q) * 2, (x,), check_trace=False)
+    z = _randn(40, 64, dtype=torch.bfloat16, seed=5).requires_grad_()
+    out = traced(z)
+    assert torch.equal(out, call(z) * 2)
+    dy = _randn(40, 64, dtype=torch.bfloat16, seed=6)
+    assert torch.equal(torch.autograd.grad(out, z, dy)[0], torch.autograd.grad(call(z) * 2, z, dy)[0])
+
+
+@pytest.mark.parametrize("name", ["linear", "linear trained", "layer_norm", "activation"])
+def test_transforms_of_torch_do_not_lose_anything(cuda_device, name):
+    # refused, each with an error of its own
+    call = _three_calls()[name]
+    x = _randn(40, 64, dtype=torch.bfloat16)
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(x, torch.ones_like(x))
+        with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+            call(dual)
+    for transform in (lambda: torch.vmap(call)(x[None]), lambda: torch.func.jvp(call, (x,), (x,)),
+                      lambda: torch.func.grad(lambda q: call(q).float().sum())(x)):
+        with pytest.raises((ValueError, RuntimeError, NotImplementedError)):
+            transform()
+
+
+def test_a_function_with_a_forward_mode_of_its_own_uses_the_calls(cuda_device):
+    w = _randn(48, 64, dtype=torch.bfloat16, seed=1, scale=0.1)
+
+    class Linear(torch.autograd.Function):
+        @staticmethod
+        def forward(ctx, x):
+            return layers.linear_forward(x, w)
+
+        @staticmethod
+        def jvp(ctx, t):
+            return layers.linear_forward(t, w)
+
+    x, t = _randn(40, 64, dtype=torch.bfloat16), _randn(40, 64, dtype=torch.bfloat16, seed=2)
+    with torch.autograd.forward_ad.dual_level():
+        y = torch.autograd.forward_ad.unpack_dual(Linear.apply(torch.autograd.forward_ad.make_dual(x, t)))
+    assert torch.equal(y.primal, layers.linear_forward(x, w)) and torch.equal(y.tangent, layers.linear_forward(t, w))
