@@ -139,12 +139,15 @@ __device__ __forceinline__ float hsum(F2 v) {
 // t in [0, 40], largest relative error 7.6e-7 evaluated in fp32.  `e` comes
 // back for the density.
 // One reciprocal serves the pair (1 / a = b / (a b)): the special function
-// unit, not the arithmetic, bounds GELU.  t <= 30, where Q is zero in fp32.
+// unit, not the arithmetic, bounds GELU.  The last bits of a value then depend on
+// the other one, so pairs of two rows (kApart) take a reciprocal each: a row's
+// results are the same whatever stands beside it.  t <= 30, where Q is zero in fp32.
+template <bool kApart>
 __device__ __forceinline__ F2 normal_tail2(F2 t, F2 &e) {
     const float2 a = split(mul2(mul2(t, f2(-0.72134752f)), t));  // log2(e) / 2
     const float2 d = split(fma2(f2(0.24f), t, f2(1.f)));
     e = f2(ex2_approx(a.x), ex2_approx(a.y));
-    const F2 u = mul2(f2(d.y, d.x), f2(rcp_approx(d.x * d.y)));
+    const F2 u = kApart ? f2(rcp_approx(d.x), rcp_approx(d.y)) : mul2(f2(d.y, d.x), f2(rcp_approx(d.x * d.y)));
     F2 r = fma2(u, f2(-0.0529928472f), f2(0.152797519f));
     r = fma2(u, r, f2(-0.0657069748f));
     r = fma2(u, r, f2(0.118390834f));
@@ -173,17 +176,18 @@ __device__ __forceinline__ float finite(float x) {  // to +-FLT_MAX: the smaller
     return y;
 }
 // x Phi(x) = max(x, 0) - |x| Q(|x|)
+template <bool kApart>
 __device__ __forceinline__ F2 gelu2(F2 v) {
     const float2 x = split(v);
     F2 e;
     const F2 t = tail_arg(x);
-    return fma2(mul2(t, f2(-1.f)), normal_tail2(t, e), f2(relu_nan(x.x), relu_nan(x.y)));
+    return fma2(mul2(t, f2(-1.f)), normal_tail2<kApart>(t, e), f2(relu_nan(x.x), relu_nan(x.y)));
 }
 // its derivative, Phi(x) + x phi(x)
 __device__ __forceinline__ F2 gelu_grad2(F2 v) {
     const float2 x = split(v);
     F2 e;
-    const F2 q = normal_tail2(tail_arg(x), e);
+    const F2 q = normal_tail2<false>(tail_arg(x), e);
     const float2 lo = split(q), hi = split(fma2(q, f2(-1.f), f2(1.f)));
     const F2 cdf = f2(x.x < 0.f ? lo.x : hi.x, x.y < 0.f ? lo.y : hi.y);
     return fma2(mul2(f2(clamp_nan(x.x), clamp_nan(x.y)), e), f2(0.398942280f), cdf);
@@ -196,8 +200,9 @@ __device__ __forceinline__ F2 sigmoid2(F2 x) {
     return f2(rcp_approx(d.x), rcp_approx(d.y));
 }
 
-// v = act(v) of kN pairs; `kind` is the same for the whole kernel.
-template <int kN>
+// v = act(v) of kN pairs; `kind` is the same for the whole kernel.  kApart: the
+// values of a pair belong to different rows.
+template <int kN, bool kApart = false>
 __device__ __forceinline__ void act_n(int kind, F2 (&v)[kN]) {
     if (kind == FCAI_ACT_RELU) {
 #pragma unroll
@@ -207,7 +212,7 @@ __device__ __forceinline__ void act_n(int kind, F2 (&v)[kN]) {
         }
     } else if (kind == FCAI_ACT_GELU) {
 #pragma unroll
-        for (int i = 0; i < kN; ++i) v[i] = gelu2(v[i]);
+        for (int i = 0; i < kN; ++i) v[i] = gelu2<kApart>(v[i]);
     } else if (kind == FCAI_ACT_SILU) {
 #pragma unroll
         for (int i = 0; i < kN; ++i) v[i] = mul2(v[i], sigmoid2(v[i]));

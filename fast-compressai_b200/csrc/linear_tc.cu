@@ -284,7 +284,7 @@ __device__ __forceinline__ void write_plain(const Params &p, uint32_t stg, int r
                 if (e < left) static_cast<T *>(p.pre)[(row0 + r + e) * p.ldpre + col] = from_f32<T>(v[e]);
         }
         F2 w[4] = {f2(v[0], v[1]), f2(v[2], v[3]), f2(v[4], v[5]), f2(v[6], v[7])};
-        act_n(p.act, w);
+        act_n<4, true>(p.act, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             const float2 f = split(w[e / 2]);

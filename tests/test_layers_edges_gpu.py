@@ -98,3 +98,18 @@ def test_a_function_with_a_forward_mode_of_its_own_uses_the_calls(cuda_device):
     with torch.autograd.forward_ad.dual_level():
         y = torch.autograd.forward_ad.unpack_dual(Linear.apply(torch.autograd.forward_ad.make_dual(x, t)))
     assert torch.equal(y.primal, layers.linear_forward(x, w)) and torch.equal(y.tangent, layers.linear_forward(t, w))
+
+
+# ------------------------------------------------------------- rows beside other rows
+
+# every way out of a product: narrow stores, padded copies, tiles, few rows, kept values
+@pytest.mark.parametrize("rows,cout,keep", [(777, 577, None), (2001, 333, "full"), (40, 65, None), (20001, 333, None),
+                                            (30, 577, None), (1000, 1030, "int8"), (2000, 512, None)])
+@pytest.mark.parametrize("kind", ["relu", "gelu", "silu"])
+def test_rows_do_not_depend_on_their_neighbours(cuda_device, kind, rows, cout, keep):
+    x, w = _randn(rows, 72, dtype=torch.float16), _randn(cout, 72, dtype=torch.float16, seed=1, scale=0.12)
+    other = x.clone()
+    other[1::2] = _randn(rows, 72, dtype=torch.float16, seed=9)[1::2]
+    a, b = (layers.linear_forward(v, w, activation=kind, keep=keep) for v in (x, other))
+    a, b = (a, b) if keep is None else (a[0], b[0])
+    assert torch.equal(a[::2], b[::2])
