@@ -113,3 +113,15 @@ def test_rows_do_not_depend_on_their_neighbours(cuda_device, kind, rows, cout, k
     a, b = (layers.linear_forward(v, w, activation=kind, keep=keep) for v in (x, other))
     a, b = (a, b) if keep is None else (a[0], b[0])
     assert torch.equal(a[::2], b[::2])
+
+
+@pytest.mark.parametrize("dtype", T16)
+@pytest.mark.parametrize("n", [7, 28, 112, 224, 448, 896, 1792, 3584, 7168, 8960])
+@pytest.mark.parametrize("keep", [None, "full", "int8"])
+def test_layer_norm_of_any_constant_row(cuda_device, dtype, n, keep):
+    # n equal values of 8 significant bits sum without rounding in 32 bits (n < 2^14), so their mean is the value
+    c = torch.arange(128, 256, device="cuda", dtype=torch.float32)
+    x = torch.cat([c, c * 128]).to(dtype)[:, None].expand(-1, n).contiguous()
+    y = layers.layer_norm_forward(x, keep=keep)
+    y = y if keep is None else y[0]
+    assert not y.any()
