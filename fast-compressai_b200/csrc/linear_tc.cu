@@ -43,8 +43,8 @@
 // epilogue.
 //
 // Every wait is bounded (1 s).  One that runs out, which no product should see,
-// makes its CTA stop, drain what it has in flight and set a word in host memory,
-// from which the next call returns FCAI_ERR_CUDA.
+// makes its CTA stop, drain what it has in flight and set its device's word in host
+// memory, from which the device's next call returns FCAI_ERR_CUDA.
 //
 // Up to 32 rows the forward product is a matter of reading w once:
 // few_rows_kernel does it with warp-level MMAs, w as their 16-row operand.
@@ -52,6 +52,7 @@
 #include <cudaTypedefs.h>
 
 #include <algorithm>
+#include <atomic>
 #include <initializer_list>
 #include <mutex>
 
@@ -1009,29 +1010,35 @@ static PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
     return fn;
 }
 
-// One word for the process, of pinned memory that every device can write; NULL
-// without a device.  It is made outside any capture that the first call is part of.
+// One word for each device, of pinned memory that the device can write; NULL
+// without a device.  It is made outside any capture that a first call is part of.
 static volatile int32_t *error_word() {
-    static int32_t *word = nullptr;
-    static std::once_flag once;
-    std::call_once(once, [] {
-        cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
-        if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return;
-        void *p = nullptr;
-        if (cudaHostAlloc(&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
-            word = static_cast<int32_t *>(p);
-            *word = 0;
-        }
-        cudaThreadExchangeStreamCaptureMode(&mode);
-    });
+    static std::atomic<int32_t *> words[64];
+    static std::mutex making;
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return nullptr;
+    int32_t *word = words[dev].load(std::memory_order_acquire);
+    if (word) return word;
+    const std::lock_guard<std::mutex> lock(making);
+    word = words[dev].load(std::memory_order_acquire);
+    if (word) return word;
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    if (cudaThreadExchangeStreamCaptureMode(&mode) != cudaSuccess) return nullptr;
+    void *p = nullptr;
+    if (cudaHostAlloc(&p, sizeof(int32_t), cudaHostAllocPortable | cudaHostAllocMapped) == cudaSuccess) {
+        word = static_cast<int32_t *>(p);
+        *word = 0;
+        words[dev].store(word, std::memory_order_release);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
     return word;
 }
 static int check_errors() {
     volatile int32_t *word = error_word();
-    if (!word) return fcai::fail(FCAI_ERR_CUDA, "linear: no pinned memory for the error word");
+    if (!word) return fcai::fail(FCAI_ERR_CUDA, "linear: no device, or no pinned memory for its error word");
     if (!*word) return FCAI_OK;
     *word = 0;
-    return fcai::fail(FCAI_ERR_CUDA, "linear: a pipeline wait of an earlier product ran out; its results are wrong");
+    return fcai::fail(FCAI_ERR_CUDA, "linear: a pipeline wait of an earlier product on this device ran out; its results are wrong");
 }
 
 constexpr int kCodeType = 100;  // a map of codes: bytes

@@ -32,7 +32,10 @@ tangent, since nothing would follow what they do.
 
 Arguments that do not fit raise ``ValueError`` before anything is launched.
 There is no fallback: the tensors are on a CUDA device and the native library
-is built.
+is built.  The products' kernels give up a wait that takes longer than a second
+(a bug, never expected) and leave wrong results; the next product on the device
+then raises ``NativeCallError``.  After the last product, or a replayed graph,
+``check()`` asks.
 """
 
 from __future__ import annotations
@@ -120,6 +123,24 @@ def _check_saved(saved, op: str, grad) -> None:
         raise ValueError(f"grad must be a tensor of shape {tuple(saved.shape)}")
     if grad.dtype is not saved.dtype:
         raise ValueError(f"grad has dtype {grad.dtype}, expected {saved.dtype}")
+
+
+def check(device: torch.device | str | int | None = None) -> None:
+    """Waits for ``device`` (the current one by default) and raises
+    ``NativeCallError`` if a product on it, run by a call or by a replayed graph,
+    gave up a wait since the last report: its results are wrong."""
+    index = torch.cuda.current_device() if device is None else device
+    device = torch.device("cuda", index) if isinstance(index, int) else torch.device(index)
+    if device.type != "cuda":
+        raise ValueError(f"check takes a CUDA device, not {device}")
+    with torch.cuda.device(device):
+        torch.cuda.synchronize()
+        word = _native.lib().fcai_linear_error_word()
+        if not word:
+            raise _native.NativeCallError(_native.FCAI_ERR_CUDA, f"no error word for {device}")
+        if word[0]:
+            word[0] = 0
+            raise _native.NativeCallError(_native.FCAI_ERR_CUDA, f"a pipeline wait of a product on {device} ran out; its results are wrong")
 
 
 # ------------------------------------------------------------------ activations

@@ -70,9 +70,11 @@ int fcai_linear_forward(const void *x, int64_t ldx, const void *w, int64_t ldw, 
                         void *codes, float *scales, int64_t rows, int32_t cin, int32_t cout, int32_t dtype, int32_t act,
                         int32_t keep, void *workspace, int64_t workspace_bytes, fcai_stream_t stream);
 /* The kernels' waits are bounded.  One that runs out (a bug, never expected)
- * ends its product early and sets this word (host memory; NULL without a
- * device); the next call that launches a product clears it and returns
- * FCAI_ERR_CUDA instead.  After a synchronise it may also be read directly. */
+ * ends its product early and sets its device's word (host memory; this returns
+ * the current device's, NULL without a device).  The next call that launches a
+ * product on that device clears the word and returns FCAI_ERR_CUDA instead of
+ * running.  Replays of a captured graph make no such call, and the last product
+ * has none after it: read the word, and clear it, after a synchronise. */
 int32_t *fcai_linear_error_word(void);
 /* dx[rows][cin] = dp[rows][cout] * w[cout][cin] */
 int fcai_linear_backward_input(const void *dp, int64_t lddp, const void *w, int64_t ldw, void *dx, int64_t lddx,

@@ -83,3 +83,8 @@ def test_forward_mode_is_refused(name):
             call(dual)
         with pytest.raises(ValueError, match="CUDA"):  # a dual level alone changes nothing
             call(x)
+
+
+def test_check_takes_a_cuda_device():
+    with pytest.raises(ValueError, match="CUDA"):
+        layers.check("cpu")

@@ -4,10 +4,12 @@ waits that ran out, large matrices, and calls at the same time."""
 
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 
-from fast_compressai import layers
+from fast_compressai import _native, layers
 from tests import layers_reference as R
 from tests.test_layers_gpu import _randn
 
@@ -125,3 +127,34 @@ def test_layer_norm_of_any_constant_row(cuda_device, dtype, n, keep):
     y = layers.layer_norm_forward(x, keep=keep)
     y = y if keep is None else y[0]
     assert not y.any()
+
+
+# ------------------------------------------------------------- waits that ran out
+
+def test_check_reports_a_wait_that_ran_out(cuda_device):
+    # as a replayed graph or a last product leaves it; the word is set here by the host
+    word = _native.lib().fcai_linear_error_word()
+    x, w = _randn(300, 64, dtype=torch.bfloat16), _randn(40, 64, dtype=torch.bfloat16, seed=1)
+    want = layers.linear_forward(x, w)
+    layers.check()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        y = layers.linear_forward(x, w)
+    for device in (None, 0, "cuda:0", torch.device("cuda", 0)):
+        graph.replay()
+        word[0] = 1
+        with pytest.raises(_native.NativeCallError, match="ran out"):
+            layers.check(device)
+        layers.check(device)  # reported once
+    assert torch.equal(y, want) and torch.equal(layers.linear_forward(x, w), want)
+
+
+def test_the_word_belongs_to_the_device(cuda_device):
+    lib = _native.lib()
+    with torch.cuda.device(0):
+        address = ctypes.addressof(lib.fcai_linear_error_word().contents)
+    assert ctypes.addressof(lib.fcai_linear_error_word().contents) == address  # one for all calls on a device
+    for other in range(1, torch.cuda.device_count()):
+        with torch.cuda.device(other):
+            assert ctypes.addressof(lib.fcai_linear_error_word().contents) != address
