@@ -359,8 +359,9 @@ def layer_norm(x, weight=None, bias=None, *, eps: float = 1e-5, keep: str = "ful
     return _LayerNorm.apply(x, weight, bias, eps, keep)
 
 
-def activation(x, kind: str, *, keep: str = "int8") -> torch.Tensor:
-    """Differentiable ``activation_forward``; keeps x in 8 bits unless asked otherwise."""
+def activation(x, kind: str, *, keep: str = "full") -> torch.Tensor:
+    """Differentiable ``activation_forward``; ``keep`` says how x waits for the
+    backward pass."""
     if keep is None:
         raise ValueError("keep must say how tensors wait for the backward pass (one of 'full', 'int8', 'e4m3')")
     if not _recorded(x):

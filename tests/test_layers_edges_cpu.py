@@ -88,3 +88,26 @@ def test_forward_mode_is_refused(name):
 def test_check_takes_a_cuda_device():
     with pytest.raises(ValueError, match="CUDA"):
         layers.check("cpu")
+
+
+def test_nothing_is_kept_in_fewer_bits_unless_asked(monkeypatch):
+    asked = []
+
+    class Host(_PlainHost):
+        def linear_forward(self, x, w, b, r, act, keep):
+            asked.append(keep)
+            return super().linear_forward(x, w, b, r, act, keep)
+
+        def layer_norm_forward(self, x, w, b, eps, keep):
+            asked.append(keep)
+            return super().layer_norm_forward(x, w, b, eps, keep)
+
+        def activation_forward(self, x, act, keep):
+            asked.append(keep)
+            return super().activation_forward(x, act, keep)
+
+    monkeypatch.setattr(layers, "_host", Host())
+    x = torch.randn(3, 8, requires_grad=True)
+    for call in CALLS.values():
+        call(x, torch.randn(8, 8))
+    assert asked == [1, 1, 1]

@@ -158,3 +158,13 @@ def test_the_word_belongs_to_the_device(cuda_device):
     for other in range(1, torch.cuda.device_count()):
         with torch.cuda.device(other):
             assert ctypes.addressof(lib.fcai_linear_error_word().contents) != address
+
+
+@pytest.mark.parametrize("dtype", T3)
+def test_activation_by_default_has_the_gradient_of_its_input(cuda_device, dtype):
+    x, dy = _randn(33, 200, dtype=dtype, scale=3.0).requires_grad_(), _randn(33, 200, dtype=dtype, seed=5)
+    got = torch.autograd.grad(layers.activation(x, "silu"), x, dy)[0]
+    xd = x.detach().double()
+    want = dy.double() * R.act_grad64(xd, "silu")
+    e = dy.double().abs() * R.act_grad_bound(xd, "silu") + R.U32 * want.abs()
+    R.check(got, want, e + R.half_step(dtype) * (want.abs() + e) + R.tiny(dtype))
