@@ -3,9 +3,11 @@
     python fast-compressai_b200/build_native.py [--force]
 
 Produces fast_compressai/_lib/libfcai_b200.so in-tree with nvcc
-(``-gencode arch=compute_100a,code=sm_100a``) and, beside it with the host
-compiler, _layers_host.so, the module that takes the pointwise layers' calls
-from tensors to that library.  No GPU is needed to build.
+(``-gencode arch=compute_100a,code=sm_100a``) and, where torch is installed, beside
+it with the host compiler the module that takes the pointwise layers' calls from
+tensors to that library: _layers_host-<torch's version>.<the interpreter's ABI>.so,
+so that another torch gets a module of its own.  Callers of the C ABI need the
+library alone.  No GPU is needed to build.
 """
 
 from __future__ import annotations
@@ -15,6 +17,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 ROOT = Path(__file__).resolve().parent
@@ -22,7 +25,6 @@ CSRC = ROOT / "csrc"
 INCLUDE = ROOT.parent / "include"
 LIB_DIR = ROOT / "fast_compressai" / "_lib"
 LIB = LIB_DIR / "libfcai_b200.so"
-HOST = LIB_DIR / "_layers_host.so"
 HOST_SOURCE = "layers_host.cpp"
 
 SOURCES = [
@@ -56,22 +58,36 @@ def up_to_date() -> bool:
     return all(p.stat().st_mtime <= t for p in _inputs())
 
 
-def _host_up_to_date() -> bool:
-    if not HOST.exists():
+def _host_module() -> tuple[Path | None, str]:
+    """The module for the running interpreter and its torch, or None and what is missing to build it."""
+    try:
+        import torch
+    except ImportError:
+        return None, "torch is not installed"
+    if torch.version.cuda is None:
+        return None, "torch is installed without CUDA"
+    for header in (Path(torch.__file__).resolve().parent / "include" / "ATen" / "ATen.h",
+                   Path(sysconfig.get_paths()["include"]) / "Python.h"):
+        if not header.exists():
+            return None, f"{header} is missing"
+    if shutil.which(os.environ.get("CXX", "g++")) is None:
+        return None, "there is no host compiler"
+    return LIB_DIR / f"_layers_host-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so", ""
+
+
+def _host_up_to_date(host: Path) -> bool:
+    if not host.exists():
         return False
-    t = HOST.stat().st_mtime
+    t = host.stat().st_mtime
     return all(p.stat().st_mtime <= t for p in [CSRC / HOST_SOURCE, INCLUDE / "fcai_layers.h", INCLUDE / "fcai_warp_div.h"])
 
 
-def _build_host(verbose: bool) -> None:
-    """_layers_host.so, against the running interpreter and its torch."""
-    import sysconfig
-
+def _build_host(host: Path, verbose: bool) -> None:
     import torch
 
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parents[1]
-    tmp = HOST.with_suffix(f".so.{os.getpid()}.tmp")
+    tmp = host.with_suffix(f".so.{os.getpid()}.tmp")
     cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
            f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
     for inc in (root / "include", root / "include" / "torch" / "csrc" / "api" / "include", cuda / "include",
@@ -82,14 +98,18 @@ def _build_host(verbose: bool) -> None:
     if verbose:
         print(" ".join(cmd), flush=True)
     subprocess.run(cmd, check=True)
-    os.replace(tmp, HOST)
+    os.replace(tmp, host)
 
 
 def build(force: bool = False, verbose: bool = False) -> Path:
     if force or not up_to_date():
         _build_lib(verbose)
-    if force or not _host_up_to_date():
-        _build_host(verbose)
+    host, missing = _host_module()
+    if host is None:
+        if verbose:
+            print(f"the pointwise layers' module is not built: {missing}", flush=True)
+    elif force or not _host_up_to_date(host):
+        _build_host(host, verbose)
     return LIB
 
 

@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import importlib.util
+import sysconfig
 import threading
 from pathlib import Path
 
@@ -225,11 +226,12 @@ _host = None
 
 def layers_host():
     """Load (once) and return the module that takes the pointwise layers'
-    calls from tensors to the native library; the module's own name, beside it."""
+    calls from tensors to the native library: the one built for this torch and
+    interpreter, beside it."""
     global _host
     if _host is None:
         lib()  # the module links against it
-        path = LIB_PATH.with_name("_layers_host.so")
+        path = LIB_PATH.with_name(f"_layers_host-{torch.__version__}.{sysconfig.get_config_var('SOABI')}.so")
         if not path.exists():
             raise NativeLibraryError(f"{path} is not built; run fast-compressai_b200/build_native.py")
         spec = importlib.util.spec_from_file_location("_layers_host", path)
