@@ -34,7 +34,10 @@
 // A forward product that keeps the activation's input in 8 bits makes the
 // codes here: a warp has whole 128-column blocks of its rows, takes their
 // largest magnitudes in a first pass over the accumulator, and the codes leave
-// beside y, so the activation's input never exists in memory in more than 8 bits.
+// beside y, so the activation's input does not go through memory in more than 8
+// bits.  (It does, as fp32 in the workspace, where reduce_kernel makes the codes: up
+// to 32 rows, where K is split, and for small results whose columns are no multiple
+// of 16, which the codes' tensor map asks for.)
 //
 // Work units are (tile, split): when a product has fewer tiles than SMs (few
 // rows, or a weight gradient whose long axis is the contraction), K is split
@@ -102,7 +105,7 @@ struct Params {
     void *y, *pre;
     int64_t ldy, ldr, ldpre;
     float *partial;                      // [splits][M][ldp], or NULL
-    uint8_t *codes;                      // [M][N], or NULL
+    uint8_t *codes;                      // [M][N] (through a tensor map: rows of N up to a multiple of 16), or NULL
     float *scales;                       // [M][nblk]
     int nblk, keep;
     int32_t *error;                      // host memory: set if a wait ran out
@@ -843,44 +846,37 @@ __global__ void __launch_bounds__(256) repack_kernel(const Repacks all) {
 // whose rows start at any element.  A thread's 16 bytes are aligned in dst, so
 // that all but a row's first and last sectors are written whole; the direct narrow
 // stores left most sectors partial, and the backward pass of 28106 x 1730 -> 24 took
-// 197 us instead of 167.
+// 197 us instead of 167.  The padding, to 16 bytes at least, takes the words that
+// reach past the row's end.
 struct Unpad {
-    const uint16_t *src;
-    uint16_t *dst;
+    const void *src;
+    void *dst;
     int64_t lds, ldd, rows;
     int cols;
     FastDiv chunks;  // aligned 16-byte pieces of a row: one more than its length asks for
     int step;        // rows of a CTA and step
 };
+template <typename E>
 __global__ void __launch_bounds__(256) unpad_kernel(const Unpad o) {
+    constexpr int kChunk = 16 / sizeof(E);
     const int chunks = (int)o.chunks.d;
     for (int64_t row0 = (int64_t)blockIdx.x * o.step; row0 < o.rows; row0 += (int64_t)gridDim.x * o.step) {
         const int n = (int)min((int64_t)o.step, o.rows - row0) * chunks;
 #pragma unroll 2
         for (int i = threadIdx.x; i < n; i += 256) {
             const int r = divide(i, o.chunks);
-            uint16_t *dst = o.dst + (row0 + r) * o.ldd;
-            const int col = (i - r * chunks) * 8 - (int)((reinterpret_cast<uintptr_t>(dst) & 15) >> 1);
-            const uint16_t *src = o.src + (row0 + r) * o.lds + col;
-            if (col >= 0 && col + 8 <= o.cols) {
-                uint32_t w[4];
-                if (col & 1) {
-                    const uint32_t first = __ldg(src), end = __ldg(src + 7);
-                    const uint32_t *q = reinterpret_cast<const uint32_t *>(src + 1);
-                    const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2);
-                    w[0] = first | q0 << 16;
-                    w[1] = __funnelshift_r(q0, q1, 16);
-                    w[2] = __funnelshift_r(q1, q2, 16);
-                    w[3] = q2 >> 16 | end << 16;
-                } else {
-                    const uint32_t *q = reinterpret_cast<const uint32_t *>(src);
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) w[e] = __ldg(q + e);
-                }
-                *reinterpret_cast<uint4 *>(dst + col) = make_uint4(w[0], w[1], w[2], w[3]);
+            E *dst = static_cast<E *>(o.dst) + (row0 + r) * o.ldd;
+            const int col = (i - r * chunks) * kChunk - (int)((reinterpret_cast<uintptr_t>(dst) & 15) / sizeof(E));
+            const E *src = static_cast<const E *>(o.src) + (row0 + r) * o.lds + col;
+            if (col >= 0 && col + kChunk <= o.cols) {
+                const uint32_t shift = (uint32_t)(reinterpret_cast<uintptr_t>(src) & 3) * 8;
+                const uint32_t *q = reinterpret_cast<const uint32_t *>(reinterpret_cast<uintptr_t>(src) & ~uintptr_t(3));
+                const uint32_t q0 = __ldg(q), q1 = __ldg(q + 1), q2 = __ldg(q + 2), q3 = __ldg(q + 3), q4 = shift ? __ldg(q + 4) : 0u;
+                *reinterpret_cast<uint4 *>(dst + col) = make_uint4(__funnelshift_r(q0, q1, shift), __funnelshift_r(q1, q2, shift),
+                                                                   __funnelshift_r(q2, q3, shift), __funnelshift_r(q3, q4, shift));
             } else {
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
+                for (int e = 0; e < kChunk; ++e)
                     if (col + e >= 0 && col + e < o.cols) dst[col + e] = __ldg(src + e);
             }
         }
@@ -1223,16 +1219,23 @@ static bool wide_outputs(const Params &p, int N, int dtype) {
            (!p.residual || aligned16(p.residual, p.ldr, dtype)) && (!p.bias || aligned16(p.bias, 0, dtype)) &&
            (reinterpret_cast<uintptr_t>(p.codes) & (N % 16 ? 7 : 15)) == 0;
 }
-// A product with codes runs its epilogue in reduce_kernel when N alone rules
-// tiles of codes out (the workspace is asked for by sizes); otherwise its outputs
-// take them, which the entry point has checked.
+// Codes whose rows the tensor map cannot take: small results make them in
+// reduce_kernel, from at most 4 * kPadFrom bytes of fp32 values (the workspace is
+// asked for by sizes); larger ones send them through rows padded to 16 bytes, as
+// they do y.  Other widths' outputs take tiles of codes, which the entry point has
+// checked.
+static bool codes_padded(int64_t M, int N) { return N % 16 != 0 && M * N >= kPadFrom; }
+static bool codes_by_reduce(int64_t M, int N) { return N % 16 != 0 && M * N < kPadFrom; }
+static int64_t code_row(int N) { return (N + 15) / 16 * 16; }
+static int unpad_grid(const Unpad &o) {
+    return (int)std::min<int64_t>((o.rows + o.step - 1) / o.step, (int64_t)fcai::sm_count() * 16);
+}
 template <typename T, bool kTA, bool kTB>
 static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Params p, unsigned char *ws,
                cudaStream_t stream) {
     p.error = const_cast<int32_t *>(error_word());
     p.vec = wide_outputs(p, N, dtype);
-    const bool reduce = p.codes && N % 16 != 0;
-    const Plan pl = make_plan(M, N, K, reduce, p.codes != nullptr);
+    const Plan pl = make_plan(M, N, K, p.codes && codes_by_reduce(M, N), p.codes != nullptr);
     p.M = (int)M;
     p.N = N;
     p.tiles_m = pl.tiles_m;
@@ -1259,17 +1262,22 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     Operand R{p.tma ? p.residual : nullptr, p.ldr, M, N}, bias{p.tma ? p.bias : nullptr, N, 1, N};
     int rc;
     if ((rc = prepare_operands({&A, &B, &R, &bias}, dtype, ws, stream))) return rc;
-    Unpad back{};
+    Unpad back{}, codes_back{};
     if (p.tma) {
         p.residual = R.ptr;
         p.ldr = R.ld;
         p.bias = bias.ptr;
         if (!y_aligned) {
             const int chunks = (N + 7) / 8 + 1;
-            back = {reinterpret_cast<const uint16_t *>(ws), static_cast<uint16_t *>(p.y), round8(N), p.ldy, M, N, fast_div(chunks),
-                    rows_a_step(M, chunks)};
+            back = {ws, p.y, round8(N), p.ldy, M, N, fast_div(chunks), rows_a_step(M, chunks)};
             p.y = ws;
             p.ldy = round8(N);
+            ws += repack_bytes(M, N);
+        }
+        if (p.codes && N % 16) {
+            const int chunks = (N + 15) / 16 + 1;
+            codes_back = {ws, p.codes, code_row(N), N, M, N, fast_div(chunks), rows_a_step(M, chunks)};
+            p.codes = ws;
         }
     }
     Maps maps;
@@ -1279,7 +1287,7 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
     if (p.tma) {
         if ((rc = make_map(&maps.y, p.y, N, M, p.ldy, 32, dtype, 32))) return rc;
         if (p.residual && (rc = make_map(&maps.res, p.residual, N, M, p.ldr, 32, dtype, 32))) return rc;
-        if (p.codes && (rc = make_map(&maps.extra, p.codes, N, M, N, 32, kCodeType, 32))) return rc;
+        if (p.codes && (rc = make_map(&maps.extra, p.codes, N, M, code_row(N), 32, kCodeType, 32))) return rc;
         if (p.pre && (rc = make_map(&maps.extra, p.pre, N, M, p.ldpre, 32, dtype, 32))) return rc;
     }
 #define LN_LAUNCH(keep_)                                                              \
@@ -1291,7 +1299,11 @@ static int run(Operand A, Operand B, int64_t M, int N, int64_t K, int dtype, Par
 #undef LN_LAUNCH
     if (rc) return rc;
     if (back.src) {
-        unpad_kernel<<<(int)std::min<int64_t>((M + back.step - 1) / back.step, (int64_t)fcai::sm_count() * 16), 256, 0, stream>>>(back);
+        unpad_kernel<uint16_t><<<unpad_grid(back), 256, 0, stream>>>(back);
+        FCAI_CUDA_TRY(cudaGetLastError());
+    }
+    if (codes_back.src) {
+        unpad_kernel<uint8_t><<<unpad_grid(codes_back), 256, 0, stream>>>(codes_back);
         FCAI_CUDA_TRY(cudaGetLastError());
     }
     return p.partial ? launch_reduce<T>(p, stream) : FCAI_OK;
@@ -1353,7 +1365,7 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
     // the product's sizes, and its operands'
     const int64_t M = weight ? cout : rows, K = weight ? rows : forward ? cin : cout, a_rows = rows, b_rows = weight ? rows : cout;
     const int N = forward ? cout : cin, a_cols = forward ? cin : cout, b_cols = cin;
-    const int64_t partial = make_plan(M, N, K, k8 && cout % 16 != 0, k8).partial_bytes;
+    const int64_t partial = make_plan(M, N, K, k8 && codes_by_reduce(M, N), k8).partial_bytes;
     int64_t n = partial;
     if (repack & 1) n += repack_bytes(a_rows, a_cols);
     if (repack & 2) n += repack_bytes(b_rows, b_cols);
@@ -1362,6 +1374,7 @@ static int64_t workspace_bytes(int op, int64_t rows, int cin, int cout, int repa
         if (repack & 4) n += repack_bytes(M, N);
         if (repack & 8) n += repack_bytes(M, N);
     }
+    if (!partial && k8 && codes_padded(M, N)) n += round256(M * code_row(N));
     return n;
 }
 // The last check before a launch.

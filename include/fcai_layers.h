@@ -57,7 +57,8 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
  * alignment; 16-byte aligned addresses and strides (8 elements) are read
  * without a copy.  With an 8-bit keep, more than 32 rows and cout a multiple of
  * 8, the addresses and strides of y, bias and residual, and codes, are 16-byte
- * aligned. */
+ * aligned.  With an 8-bit keep and cout no multiple of 16 the workspace holds p
+ * as fp32 (up to 6 Mi values) or the codes in padded rows. */
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
 /* `repack`: bits set for matrices of the call that are not 16-byte aligned in
  * address and row stride: 1 the first operand (x; dp; dp), 2 the second (w; w;

@@ -8,7 +8,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 from torch.fx.experimental.proxy_tensor import make_fx
 
-from fast_compressai import layers
+from fast_compressai import _native, layers
 
 
 class _PlainHost:
@@ -111,3 +111,15 @@ def test_nothing_is_kept_in_fewer_bits_unless_asked(monkeypatch):
     for call in CALLS.values():
         call(x, torch.randn(8, 8))
     assert asked == [1, 1, 1]
+
+
+@pytest.mark.parametrize("keep", [2, 3])
+@pytest.mark.parametrize("rows,cin,cout", [(147456, 128, 520), (36864, 192, 1032), (1 << 20, 16, 2056), (70001, 64, 333),
+                                           (300, 64, 65), (33, 8, 100001), (5000, 24, 100008)])
+def test_scratch_of_products_kept_in_8_bits(rows, cin, cout, keep):
+    bytes_ = _native.lib().fcai_linear_workspace(0, rows, cin, cout, 0, keep)
+    # fp32 values of small or split products, or the codes once more
+    assert 0 <= bytes_ <= max(32 << 20, rows * (cout + 15) + 256)
+    # unaligned operands add their copies, nothing else
+    more = _native.lib().fcai_linear_workspace(0, rows, cin, cout, 3, keep)
+    assert more - bytes_ <= 2 * (rows + cout) * (cin + 7) + 512

@@ -11,7 +11,7 @@ import torch
 
 from fast_compressai import _native, layers
 from tests import layers_reference as R
-from tests.test_layers_gpu import _randn
+from tests.test_layers_gpu import _randn, _sliced
 
 pytestmark = pytest.mark.gpu
 
@@ -168,3 +168,37 @@ def test_activation_by_default_has_the_gradient_of_its_input(cuda_device, dtype)
     want = dy.double() * R.act_grad64(xd, "silu")
     e = dy.double().abs() * R.act_grad_bound(xd, "silu") + R.U32 * want.abs()
     R.check(got, want, e + R.half_step(dtype) * (want.abs() + e) + R.tiny(dtype))
+
+
+# ------------------------------------------------- products kept in 8 bits
+
+# widths that are no multiple of 16: codes by way of padded rows (from 6 Mi results on) or of fp32 values
+@pytest.mark.parametrize("rows,cin,cout", [(40001, 24, 1030), (65537, 40, 520), (20000, 33, 5003), (33000, 64, 520), (12099, 64, 520),
+                                           (12098, 64, 520), (6291457, 8, 1), (700001, 16, 9), (50, 24, 130001), (400000, 200, 17)])
+@pytest.mark.parametrize("fmt,dtype", [("int8", torch.bfloat16), ("e4m3", torch.float16)])
+@pytest.mark.parametrize("unaligned", [False, True])
+def test_products_kept_in_8_bits_of_any_width(cuda_device, rows, cin, cout, fmt, dtype, unaligned):
+    x, w = _randn(rows, cin, dtype=dtype), _randn(cout, cin, dtype=dtype, seed=1, scale=cin ** -0.5)
+    b, r = _randn(cout, dtype=dtype, seed=2), _randn(rows, cout, dtype=dtype, seed=3)
+    if unaligned:
+        x, r = _sliced(x), _sliced(r)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    y, saved = layers.linear_forward(x, w, b, activation="gelu", residual=r, keep=fmt)
+    held = torch.cuda.memory_allocated() - before
+    # scratch: padded copies of what is not aligned, and the codes once more or 6 Mi fp32 values
+    copies = 2 * (rows + cout) * (cin + 8) + 4 * rows * (cout + 8)
+    assert torch.cuda.max_memory_allocated() - before - held <= copies + max(rows * (cout + 15), 32 << 20) + (4 << 20)
+    if rows * cout >= 6 << 20:  # the same epilogue as without codes
+        assert torch.equal(y, layers.linear_forward(x, w, b, activation="gelu", residual=r))
+    want, bound = R.linear_bound(x, w, b, r, "gelu", dtype)
+    R.check(y, want, bound, "y")
+    p64, _ = R.linear64(x, w, b)
+    e = (cin + 2) * 2.0 ** -23 * (x.double().abs() @ w.double().abs().t() + b.double().abs())
+    R.check(saved.pre.load(torch.float32), p64, e + R.keep8_step(p64.abs() + e, saved.pre.scales, fmt), "pre")
+    # the scales are those of the values: a block's largest one has the largest code
+    amax = torch.nn.functional.pad(p64.abs(), (0, -cout % 128)).reshape(rows, -1, 128).amax(2)
+    top = 127 if fmt == "int8" else 448
+    slack = torch.nn.functional.pad(e, (0, -cout % 128)).reshape(rows, -1, 128).amax(2) / top + amax / top * 2.0 ** -22
+    R.check(saved.pre.scales, amax / top, slack, "scales")
