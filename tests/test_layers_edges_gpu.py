@@ -5,11 +5,13 @@ waits that ran out, large matrices, and calls at the same time."""
 from __future__ import annotations
 
 import ctypes
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 import torch
 
 from fast_compressai import _native, layers
+from fast_compressai.layers import Checkpoint8
 from tests import layers_reference as R
 from tests.test_layers_gpu import _randn, _sliced
 
@@ -202,3 +204,76 @@ def test_products_kept_in_8_bits_of_any_width(cuda_device, rows, cin, cout, fmt,
     top = 127 if fmt == "int8" else 448
     slack = torch.nn.functional.pad(e, (0, -cout % 128)).reshape(rows, -1, 128).amax(2) / top + amax / top * 2.0 ** -22
     R.check(saved.pre.scales, amax / top, slack, "scales")
+
+
+# ------------------------------------------------- offsets past 32 bits, calls at the same time
+
+def _tail(kept, rows):
+    return Checkpoint8(kept.codes[rows].contiguous(), kept.scales[rows].contiguous(),
+                       torch.Size((kept.codes[rows].shape[0], kept.codes.shape[1])), kept.dtype, kept.format)
+
+
+# codes beside y, codes through padded rows, and everything through padded rows
+@pytest.mark.parametrize("cout", [2064, 2056, 2057])
+def test_last_rows_of_large_matrices(cuda_device, cout):
+    dtype, rows, cin = torch.bfloat16, (1 << 20) + 3, 16  # 2.16e9 values
+    tail = slice(rows - 300, rows)
+    x, w, b = _randn(rows, cin, dtype=dtype), _randn(cout, cin, dtype=dtype, seed=1, scale=0.25), _randn(cout, dtype=dtype, seed=2)
+    r, dy = _randn(rows, cout, dtype=dtype, seed=3), _randn(rows, cout, dtype=dtype, seed=4)
+    y, saved = layers.linear_forward(x, w, b, activation="silu", residual=r, keep="int8")
+    want, bound = R.linear_bound(x[tail], w, b, r[tail], "silu", dtype)
+    R.check(y[tail], want, bound, "y")
+    p64, _ = R.linear64(x[tail], w, b)
+    e = (cin + 2) * 2.0 ** -23 * (x[tail].double().abs() @ w.double().abs().t() + b.double().abs())
+    pre = _tail(saved.pre, tail).load(torch.float32)
+    R.check(pre, p64, e + R.keep8_step(p64.abs() + e, saved.pre.scales[tail], "int8"), "pre")
+    assert torch.equal(saved.pre.load()[tail], pre.to(dtype))
+    dx = layers.linear_backward(dy, saved, w, needs=(True, False, False))[0]
+    (g, e), _, _ = R.linear_grads(dy[tail], _tail(saved.kept, tail).load(), w, pre.double(), "silu", dtype)
+    R.check(dx[tail], g, e, "dx")
+    del r, saved, dx
+
+    z, saved = layers.activation_forward(y, "relu", keep="int8")
+    assert torch.equal(z[tail], torch.relu(y[tail]))
+    kept, scales = R.keep8(y[tail], "int8")
+    assert torch.equal(saved.kept.scales[tail], scales)
+    assert torch.equal(_tail(saved.kept, tail).load(torch.float32), kept)
+    dz = layers.activation_backward(dy, saved)
+    assert torch.equal(dz[tail], torch.where(kept > 0, dy[tail], torch.zeros_like(dy[tail])))
+    del z, dz, saved
+
+    z, saved = layers.layer_norm_forward(y, keep="e4m3")
+    want, bound, *_ = R.norm64(y[tail], None, None, 1e-5, dtype)
+    R.check(z[tail], want, bound, "norm")
+    kept, _ = R.keep8(y[tail], "e4m3")
+    assert torch.equal(_tail(saved.kept, tail).load(torch.float32), kept)
+    dx = layers.layer_norm_backward(dy, saved, needs=(True, False, False))[0]
+    (g, e), _, _ = R.norm_grads(dy[tail], kept, y[tail], None, 1e-5, dtype, dtype)
+    R.check(dx[tail], g, e, "norm dx")
+
+
+def test_threads_call_at_the_same_time(cuda_device):
+    x, dy = _randn(700, 200, dtype=torch.bfloat16), _randn(700, 264, dtype=torch.bfloat16, seed=5)
+    w, b = _randn(264, 200, dtype=torch.bfloat16, seed=1, scale=0.07), _randn(264, dtype=torch.bfloat16, seed=2)
+    g = _randn(200, dtype=torch.float32, seed=3)
+
+    def step():
+        h, s0 = layers.layer_norm_forward(x, g, keep="int8")
+        y, s1 = layers.linear_forward(h, w, b, activation="gelu", keep="e4m3")
+        dh, dw, db = layers.linear_backward(dy, s1, w)
+        one = layers.linear_forward(x[:3], w, b)
+        with pytest.raises(ValueError, match="fit"):  # a thread's message is its own
+            layers.linear_forward(x[:, :8], w)
+        return [y, dh, dw, db, one, *layers.layer_norm_backward(dh, s0, g)]
+
+    first = step()
+    torch.cuda.synchronize()
+
+    def many(_):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            results = [step() for _ in range(20)]
+            torch.cuda.current_stream().synchronize()
+        return all(torch.equal(a, e) for got in results for a, e in zip(got, first))
+
+    with ThreadPoolExecutor(4) as pool:
+        assert all(pool.map(many, range(4)))
