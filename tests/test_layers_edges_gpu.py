@@ -277,3 +277,62 @@ def test_threads_call_at_the_same_time(cuda_device):
 
     with ThreadPoolExecutor(4) as pool:
         assert all(pool.map(many, range(4)))
+
+
+# ------------------------------------------------- the smallest sizes, other ways to call
+
+@pytest.mark.parametrize("rows", [1, 2, 33, 300])
+@pytest.mark.parametrize("cin,cout", [(1, 1), (1, 7), (2, 9), (3, 1), (7, 5), (1, 129)])
+@pytest.mark.parametrize("keep", layers.KEEPS)
+def test_linear_of_the_fewest_channels(cuda_device, rows, cin, cout, keep):
+    dtype = torch.bfloat16
+    x, w, b = _randn(rows, cin, dtype=dtype), _randn(cout, cin, dtype=dtype, seed=1), _randn(cout, dtype=dtype, seed=2)
+    dy = _randn(rows, cout, dtype=dtype, seed=4)
+    y, saved = layers.linear_forward(x, w, b, activation="silu", keep=keep)
+    want, bound = R.linear_bound(x, w, b, None, "silu", dtype)
+    R.check(y, want, bound, "y")
+    kept = x if keep == "full" else saved.kept.load()
+    pre = (saved.pre if keep == "full" else saved.pre.load(torch.float32)).double()
+    for name, got, (g, e) in zip(("dx", "dw", "db"), layers.linear_backward(dy, saved, w),
+                                 R.linear_grads(dy, kept, w, pre, "silu", dtype)):
+        R.check(got, g, e, name)
+
+
+@pytest.mark.parametrize("keep", layers.KEEPS)
+def test_a_single_row_without_a_row_dimension(cuda_device, keep):
+    x, w, g = _randn(1, 65, dtype=torch.bfloat16), _randn(41, 65, dtype=torch.bfloat16, seed=1, scale=0.1), _randn(65, dtype=torch.float32)
+
+    def step(x):
+        h, s0 = layers.layer_norm_forward(x, g, keep=keep)
+        a, s1 = layers.activation_forward(h, "gelu", keep=keep)
+        y, s2 = layers.linear_forward(a, w, activation="silu", keep=keep)
+        da, dw, _ = layers.linear_backward(y, s2, w)
+        dh = layers.activation_backward(da, s1)
+        dx, dg, db = layers.layer_norm_backward(dh, s0, g)
+        return h, a, y, da, dh, dx, dw, dg, db
+
+    for flat, rows in zip(step(x[0]), step(x)):
+        assert flat.shape == rows.shape or flat.shape == rows.shape[1:]
+        assert torch.equal(flat.reshape(-1), rows.reshape(-1))
+
+
+@pytest.mark.parametrize("keep", layers.KEEPS)
+def test_saved_tensors_may_wait_elsewhere(cuda_device, keep):
+    x, w = _randn(300, 65, dtype=torch.bfloat16).requires_grad_(), _randn(41, 65, dtype=torch.bfloat16, seed=1).requires_grad_()
+    dy = _randn(300, 41, dtype=torch.bfloat16, seed=2)
+
+    def grads():
+        y = layers.linear(layers.activation(layers.layer_norm(x, keep=keep), "silu", keep=keep), w, activation="gelu", keep=keep)
+        return torch.autograd.grad(y, [x, w], dy)
+
+    want = grads()
+    with torch.autograd.graph.save_on_cpu():
+        got = grads()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_a_second_derivative_is_refused(cuda_device):
+    x = _randn(8, 64, dtype=torch.float32).requires_grad_()
+    dx = torch.autograd.grad(layers.activation(x, "silu").sum(), x, create_graph=True)[0]
+    with pytest.raises(RuntimeError, match="once_differentiable|does not require grad"):
+        torch.autograd.grad(dx.sum(), x)
