@@ -4,7 +4,8 @@
 //
 // A compiled module because these calls are often microseconds of GPU time (one
 // position of a latent through a layer): checking a dozen tensor attributes and
-// converting twenty arguments in Python takes 8 to 13 us a call, here 1 to 2.
+// converting twenty arguments in Python takes 8 to 13 us a call; here a whole call,
+// its launch and Python's side included, takes 4 to 5.
 // Plain CPython functions over torch's C++ tensors; every C++ exception ends in
 // a Python one.
 #include <ATen/ATen.h>
@@ -355,7 +356,9 @@ PyObject *py_linear_forward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         }
         const Rows m = rows_of(x, cin), wm = rows_of(w, cin);
         at::Tensor y = fresh(shape, x), pre;
-        const int64_t ldpre = (cout + 7) / 8 * 8;  // pre: padded rows, which leave the kernel (and enter the backward pass) in wide accesses
+        // pre: the activation's input rounded to the type, as keep "full" says; padded rows, which leave the kernel (and enter
+        // the backward pass) in wide accesses
+        const int64_t ldpre = (cout + 7) / 8 * 8;
         Codes k;
         const int kp = act == FCAI_ACT_NONE ? FCAI_KEEP_NONE : keep;  // what of the activation's input is kept
         if (kp == FCAI_KEEP_FULL) pre = fresh({m.rows, ldpre}, x);
@@ -404,6 +407,8 @@ PyObject *py_linear_backward(PyObject *, PyObject *const *a, Py_ssize_t n) {
         if (act != FCAI_ACT_NONE) {
             const Kept p = kept_of(a[4], a[5], keep, cout, grad);
             if (p.m.rows != g.rows) refuse("linear: grad does not fit what was kept");
+            // dp is rounded to the type: the tensor cores read it in that type.  dx and dw then have the square root of 2 of
+            // the error that exact operands would leave (0.0024 against 0.0017 relative in bf16); db is summed before it.
             const int64_t ld = (cout + 7) / 8 * 8;  // rows that the products read without a copy
             dp = fresh({g.rows, ld}, grad);
             act_backward(grad, g, cout, p, act, dp, db, ld);

@@ -227,7 +227,8 @@ __device__ __forceinline__ float lds32(uint32_t addr) {
 
 // The bias of 32 columns that every lane has alike, 8 at a time (a ragged or
 // unaligned bias was copied: narrow loads here, even where no call takes them,
-// cost every product registers; 36864 x 192 -> 768 took 34.3 us instead of 32.1).
+// cost every product registers; 36864 x 192 -> 768 took 34.3 us in a graph instead
+// of 32.1).
 template <typename T>
 __device__ __forceinline__ void add_bias32(const Params &p, int col0, F2 (&v)[16]) {
     if (!p.bias) return;
@@ -889,9 +890,11 @@ __global__ void __launch_bounds__(256) unpad_kernel(const Unpad o) {
 // Lane (g, t) = (lane / 4, lane % 4) holds 8 consecutive k of w's rows g and g + 8
 // and of x's row g; an MMA takes k in any order as long as both operands agree,
 // so these 8 serve two MMAs as they were loaded.  A CTA owns 16 columns of y;
-// its warps take K in turns of 64, and their sums meet in shared memory in a
-// fixed order.  Bound by reading w; 16 warps times 4 loads of 512 bytes
-// in flight an SM cover the latency.
+// its warps take K in turns of 32, and their sums meet in shared memory in a
+// fixed order.  Bound by reading w, and by the launch: a warp has 8 loads of 512
+// bytes of w in flight (4 above 16 rows), 16 warps a CTA for long rows (1 x 4096 ->
+// 4096 in a graph: 4.8 us with w in L2, 9.1 with w from memory).  Rows that do not
+// take 16-byte accesses are read by single elements.
 template <typename T> __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1);
 template <>
 __device__ __forceinline__ void mma16816<__nv_bfloat16>(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {

@@ -918,7 +918,8 @@ constexpr int backward_rows(int lanes, int chunks) { return lanes <= 32 ? 2 / ch
 // have 6 steps of rows, once there are two CTAs an SM; rows by single elements 3,
 // whose loads more warps hide (fp16 from int8, inputs in memory: 1000 x 1024 10.8 us,
 // with as many CTAs as fit 17.3; 5003 x 1024 20.5 and 23.0; 20000 x 200 12.0 and 14.2;
-// 2000 x 1021 13.7 with 3 steps, 16.1 with 6).
+// 2000 x 1021 13.7 with 3 steps, 16.1 with 6).  The workspace is asked for by sizes,
+// so rows that are unaligned by address or stride alone have the 6 steps too.
 static int norm_backward_grid(int64_t rows, int n) {
     const Held h = held(n);
     const int groups = (h.lanes <= 32 ? kThreads / h.lanes : 1) * backward_rows(h.lanes, h.chunks);

@@ -15,6 +15,14 @@ come in two forms:
   128 channels with one scale each);
 * differentiable calls over them: ``linear``, ``layer_norm``, ``activation``.
 
+A backward pass takes the derivatives of what was kept.  A ReLU input above 0
+that an 8-bit checkpoint rounds to 0 (in int8, below 1 / 254 of the largest of
+its 128 channels) so has the gradient 0; ``"full"`` keeps its sign.
+
+``torch.autocast`` does not reach these calls.  ``linear`` takes tensors of one
+16-bit type; the others take fp32 too, layer norm's weight and bias in x's type
+or fp32; anything else is refused.
+
 Every call runs on the current stream of its tensors' device and allocates its
 outputs and scratch from torch's caching allocator, so calls on different
 streams or in different captured graphs share nothing.  Tensors that belong to

@@ -2,9 +2,9 @@
  * fcai_layers.h -- C ABI of the pointwise layers: the matrix product with
  * bias, activation and residual in its epilogue (tcgen05, fp32 accumulation
  * in tensor memory), layer norm, and activations whose input is kept in 8
- * bits for the backward pass.  They stand beside the convolution layers of
- * fcai_transforms.h for models that also have pointwise layers (context and
- * entropy models over the latents), in the forms serving and training use.
+ * bits for the backward pass, in the forms serving and training use.  They stand
+ * beside the convolution layers of fcai_transforms.h for callers whose models have
+ * pointwise layers too; the codecs of this library have none and do not call them.
  *
  * Tensors are rows of channels, row-major with a row stride in elements
  * (ld >= channels); channels are contiguous.  Rows are the positions of a
@@ -43,7 +43,9 @@ enum { FCAI_ACT_NONE = 0, FCAI_ACT_RELU = 1, FCAI_ACT_GELU = 2, FCAI_ACT_SILU = 
  * q = round(clamp(x * fl(1 / scale), +-top)): int8 (top = 127, ties to even) or
  * e4m3 (top = 448).  They read back as q * scale.  A block that holds an
  * infinity or a NaN gets the scale NaN and reads back as NaN throughout, so a
- * diverged step stays visible.  Codes are [rows][channels] bytes, scales
+ * diverged step stays visible.  Derivatives are those of the value read back: a
+ * ReLU input above 0 that rounds to 0 (below amax / 254 in int8, amax / 458752 in
+ * e4m3) has the derivative 0; keep it in full where that matters.  Codes are [rows][channels] bytes, scales
  * [rows][ceil(channels / 128)] floats, both contiguous. */
 enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M3 = 3 };
 #define FCAI_KEEP_BLOCK 128
