@@ -60,7 +60,8 @@ enum { FCAI_KEEP_NONE = 0, FCAI_KEEP_FULL = 1, FCAI_KEEP_INT8 = 2, FCAI_KEEP_E4M
  * without a copy.  With an 8-bit keep, more than 32 rows and cout a multiple of
  * 8, the addresses and strides of y, bias and residual, and codes, are 16-byte
  * aligned.  With an 8-bit keep and cout no multiple of 16 the workspace holds p
- * as fp32 (up to 6 Mi values) or the codes in padded rows. */
+ * as fp32 (below 6 Mi values) or the codes in padded rows; it also holds p as
+ * fp32 up to 32 rows, and any product's partial sums where cin is split. */
 enum { FCAI_LINEAR_FORWARD = 0, FCAI_LINEAR_BACKWARD_INPUT = 1, FCAI_LINEAR_BACKWARD_WEIGHT = 2 };
 /* `repack`: bits set for matrices of the call that are not 16-byte aligned in
  * address and row stride: 1 the first operand (x; dp; dp), 2 the second (w; w;
